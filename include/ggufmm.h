@@ -82,7 +82,8 @@ int ggufmm_last_cuda_error(void);
 /*
  * Device-side status word: every spin-wait inside the kernels is bounded and,
  * when it gives up, ORs 1 into this word and unwinds instead of hanging; an
- * embedding id out of range ORs 2. Returns the word (>= 0; 0 = nothing seen)
+ * embedding id, cache slot, page or sequence length outside its table ORs 2.
+ * Returns the word (>= 0; 0 = nothing seen)
  * or a negative status.
  * Synchronizes `stream`; clears the word when `clear` is nonzero.
  */
@@ -378,6 +379,119 @@ int ggufmm_mul_mat(const void* q, int qtype, int64_t n, int64_t k,
                    const void* x, int x_dtype, int64_t m, int64_t ldx,
                    void* y, int y_dtype, int64_t ldy,
                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- what lies between a layer's projections ------------------------------------------
+ * Norm, rotary positions, key-value cache and attention. The reference runs them as
+ * separate WGSL dispatches with f16 buffers between them
+ * (vllm_webgpu/models/llama.py:239-367).
+ */
+
+/*
+ * Root-mean-square norm of each of m rows of n values, with the residual's addition in
+ * front of it (shaders/generic/add.wgsl, rms_norm.wgsl):
+ *   s = x + resid,  y = s * (mean(s^2) + eps)^-1/2 * (w + w_add),  resid_out = s
+ * computed in 32 bits; s is rounded once into resid_out and y once into its own type (y
+ * is the norm of the unrounded s). resid may be NULL (s = x; resid_out must be NULL then),
+ * resid_out may be NULL (not kept) and has resid's dtype; w may be NULL (a factor of 1);
+ * w_add serves models that store their weight minus one. x, resid, w and y each have their
+ * own dtype; row strides in elements, any alignment of the element type. resid_out may be
+ * resid, and y may be x when the dtypes and strides are equal; no other overlap. m == 0
+ * does nothing; n is at most GGUFMM_NORM_MAX_N.
+ */
+#define GGUFMM_NORM_MAX_N 65536
+int ggufmm_rms_norm(const void* x, int x_dtype, int64_t m, int64_t n, int64_t ldx,
+                    const void* resid, int r_dtype, int64_t ldr, void* resid_out, int64_t ldro,
+                    const void* w, int w_dtype, float w_add, float eps,
+                    void* y, int y_dtype, int64_t ldy, void* stream);
+
+/*
+ * The paged key-value cache of the calls below: k and v, each [num_pages, kv_heads,
+ * page_size, head_dim] of f16 or bf16 values. Strides are in elements, multiples of 8,
+ * the innermost 1, pointers 16-byte aligned; head_dim is a multiple of 8 up to
+ * GGUFMM_MAX_HEAD_DIM and page_size a multiple of 8. Slot s is offset s % page_size of
+ * page s / page_size. The structs hold 8-byte fields only; every pointer but the struct's
+ * own is a device pointer.
+ */
+#define GGUFMM_MAX_HEAD_DIM 256
+
+/*
+ * Rotary positions on q and k and the append of k and v to the cache, one launch
+ * (shaders/generic/rope.wgsl, kv_cache_store.wgsl). The first rot_dim values of a head are
+ * turned in pairs (i, i + rot_dim/2), or (2i, 2i+1) when interleaved, by
+ * phi = positions[t] * steps[i] * 2^-64 turns (steps in 2^-64 turns per position: exact
+ * modulo one turn at any position), the turned values times `factor`; the rest of the head
+ * passes. k (turned) and v go to slots[t] of the cache, rounded once to its dtype; a
+ * negative slot stores nothing, one past the last page too, and sets bit 2 of the device
+ * status word. Two tokens must not share a slot. q_out may be q when dtypes and strides
+ * are equal. k == NULL: q alone (the cache fields and kv_heads are not read).
+ */
+typedef struct ggufmm_rope_args {
+  const void* q;
+  int64_t q_row, q_head; /* strides of a token and of a head, elements */
+  void* q_out;
+  int64_t qo_row, qo_head;
+  const void* k;
+  int64_t k_row, k_head;
+  const void* v;
+  int64_t v_row, v_head;
+  void* k_cache;
+  int64_t kc_page, kc_head, kc_slot;
+  void* v_cache;
+  int64_t vc_page, vc_head, vc_slot;
+  const void* positions; /* int64 [tokens] */
+  const void* slots;     /* int64 [tokens] */
+  const void* steps;     /* int64 [rot_dim / 2] */
+  int64_t tokens, q_heads, kv_heads, head_dim, rot_dim, interleaved;
+  int64_t x_dtype, q_out_dtype, cache_dtype, page_size, num_pages;
+  double factor;
+} ggufmm_rope_args;
+
+int ggufmm_rope_append(const ggufmm_rope_args* args, void* stream);
+
+/*
+ * Attention over the cache (shaders/generic/{attn_score,softmax,attn_output}.wgsl, one
+ * sequence there): out = softmax(scale * q k^T) v over the cached tokens that a query sees.
+ * q and out [total_q, q_heads, head_dim] in the cache's dtype (strides multiples of 8,
+ * pointers 16-byte aligned); query head h reads kv head h / (q_heads / kv_heads), at most
+ * GGUFMM_MAX_GROUP query heads to one. Token j of sequence b lies in page
+ * tables[b * table_row + j / page_size], offset j % page_size; lens[b] is the sequence's
+ * length with its new tokens, whose keys and values are in the cache already. A query at
+ * position i sees j <= i and, when window > 0, j > i - window; one that sees nothing gives
+ * zeros. A page outside the cache reads as zeros and a length past the table is cut to it;
+ * both set bit 2 of the device status word.
+ *
+ * ggufmm_paged_attention: one new token per sequence, total_q == batch (q_starts and max_q
+ * are not read), at position lens[b] - 1; a length <= 0 gives zeros. The cache's length is
+ * split over the SMs and joined inside the same launch. `workspace`
+ * (ggufmm_paged_attention_workspace_size bytes, 256-byte aligned) must be zero-filled
+ * before its first use; every call leaves it ready for the next one on the same stream.
+ *
+ * ggufmm_paged_prompt_attention: sequence b's new tokens are rows q_starts[b] to
+ * q_starts[b + 1] of q, the last lens[b]-positions of the sequence; max_q is at least the
+ * longest of them (rows past it are not computed, and set bit 2). Rows that belong to no
+ * sequence are not written.
+ */
+#define GGUFMM_MAX_GROUP 64
+typedef struct ggufmm_attention_args {
+  const void* q;
+  int64_t q_row, q_head;
+  void* out;
+  int64_t o_row, o_head;
+  const void* k;
+  int64_t k_page, k_head, k_slot;
+  const void* v;
+  int64_t v_page, v_head, v_slot;
+  const void* tables; /* int32 [batch, table_width], row stride table_row */
+  int64_t table_row, table_width;
+  const void* lens;     /* int32 [batch] */
+  const void* q_starts; /* int32 [batch + 1] */
+  int64_t batch, total_q, max_q, q_heads, kv_heads, head_dim, page_size, num_pages, dtype, window;
+  double scale;
+} ggufmm_attention_args;
+
+size_t ggufmm_paged_attention_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim);
+int ggufmm_paged_attention(const ggufmm_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
+int ggufmm_paged_prompt_attention(const ggufmm_attention_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -42,6 +42,8 @@ cudaError_t launch_gemv_mma(const void* q, int qtype, int64_t n, int64_t k, cons
 cudaError_t gemm_device_error(int* v, int clear, cudaStream_t st);
 cudaError_t gemv_i8_device_error(int* v, int clear, cudaStream_t st);
 cudaError_t dequant_device_error(int* v, int clear, cudaStream_t st);
+cudaError_t rope_device_error(int* v, int clear, cudaStream_t st);
+cudaError_t attn_device_error(int* v, int clear, cudaStream_t st);
 cudaError_t launch_embedding(const void* q, int qtype, int64_t n_vocab, int64_t k, const int32_t* ids, int64_t n_ids,
                              void* out, int out_dtype, int64_t ldo, cudaStream_t st);
 cudaError_t gemv_set_wait_limit(uint32_t polls);
@@ -107,7 +109,9 @@ static int cuda_status(cudaError_t e) {
 // (read back by ggufmm_last_cuda_error) and maps it to a status.
 int record_cuda_status(cudaError_t e) { return cuda_status(e); }
 
-static int check_device() {
+// GGUFMM_OK when the current device is an sm_100 GPU (also for entry points defined in
+// other translation units).
+int check_device() {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_status(e);
@@ -190,10 +194,12 @@ int ggufmm_device_status(int clear, void* stream) {
   if (e == cudaSuccess) e = gemm_fused_device_error(&d, clear, st);
   if (e == cudaSuccess) e = gemv_i8_device_error(&f, clear, st);
   if (e == cudaSuccess) e = dequant_device_error(&h, clear, st);
-  int r = 0;
+  int r = 0, o = 0, t = 0;
   if (e == cudaSuccess) e = allreduce_device_error(&r, clear, st);
+  if (e == cudaSuccess) e = rope_device_error(&o, clear, st);
+  if (e == cudaSuccess) e = attn_device_error(&t, clear, st);
   if (e != cudaSuccess) return cuda_status(e);
-  return a | b | c | d | f | h | r;
+  return a | b | c | d | f | h | r | o | t;
 }
 
 int ggufmm_set_wait_limit(uint32_t polls) {

@@ -68,6 +68,7 @@ static inline cudaError_t tu_device_error(int* out, int clear, cudaStream_t st) 
 }
 
 constexpr int kErrWaitTimeout = 1;
+constexpr int kErrIndex = 2;  // an id, slot, page or length outside its table
 
 __device__ __forceinline__ float half_bits_to_float(uint32_t bits16) {
   return __half2float(__ushort_as_half(static_cast<unsigned short>(bits16 & 0xFFFFu)));

@@ -233,7 +233,6 @@ cudaError_t launch_dequant(const void* q, int qtype, int64_t n_rows, int64_t k, 
 // same bit-exact decode as dequant_kernel; fp32 output is gguf's value, f16 / bf16 its
 // single rounding. An id outside [0, n_vocab) writes a zero row and sets
 // kErrIndex in the device status word (the reference does not check).
-constexpr int kErrIndex = 2;
 
 template <int OT>
 __device__ __forceinline__ void store32(void* out, const float* v) {

@@ -21,7 +21,7 @@ def __getattr__(name: str):
     if name == "B200Platform":
         from .platform import B200Platform
         return B200Platform
-    if name in ("ops", "formats", "platform", "quant", "models", "tp"):
+    if name in ("ops", "formats", "platform", "quant", "models", "tp", "kv_cache"):
         import importlib
         return importlib.import_module(f"{__name__}.{name}")
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

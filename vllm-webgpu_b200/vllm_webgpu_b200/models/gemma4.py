@@ -35,6 +35,11 @@ class Gemma4B200Model(LlamaB200Model):
             self.q_dim = self.num_q_heads * self.head_dim
             self.kv_dim = self.num_kv_heads * self.head_dim
 
+    def forward(self, input_ids, positions, attn_metadata):
+        """Not built: Gemma's block has norms after its projections and an embedding scale
+        that the Llama layer has not."""
+        raise NotImplementedError("the Gemma forward pass is not supported; its projections are")
+
     def lm_head_weight(self):
         """``lm_head.weight`` or, as in the reference (gemma4.py:152), the tied embedding table."""
         return self.weights.get("lm_head.weight", self.weights["model.embed_tokens.weight"])

@@ -8,9 +8,14 @@ one grouped launch (ggufmm_gemv_grouped), as vLLM fuses QKV and gate_up.
 The reference picks ``USE_QUANT = 0 if q_proj.weight is present`` and so never
 runs its quantized branch (llama.py:258); here the branch is chosen by the
 weight's type, so GGUF blocks always take the quantized kernels.
-Attention, norms and RoPE between the projections are outside this path.
+
+``forward`` runs whole layers: norm, q/k/v, rotary positions and the append to a
+paged cache, attention, o, norm, FFN (llama.py:239-367), for any mix of sequences,
+prompts and single tokens, where the reference takes one token of one sequence.
 """
 from __future__ import annotations
+
+import dataclasses
 
 import torch
 
@@ -132,6 +137,100 @@ class LlamaB200Model(BaseB200Model):
         GGUF ``output.weight``), quantized like the other projections (the reference
         forces an f16 head, llama.py:228-235)."""
         return self._linear(hidden, self.weights["lm_head.weight"], logits)
+
+    # ---- whole layers -----------------------------------------------------------------
+    def _cfg(self, name: str, default=None):
+        cfg = self.model_config
+        value = cfg.get(name) if isinstance(cfg, dict) else getattr(cfg, name, None)
+        return default if value is None else value
+
+    def _rope_plan(self):
+        """(steps, factor, interleaved) of the model's rotary positions, made once."""
+        plan = self.__dict__.get("_rope")
+        if plan is None:
+            theta, scaling = float(self._cfg("rope_theta", 10000.0)), self._cfg("rope_scaling")
+            steps, factor = ops.rope_steps(self._rot_dim(), theta, scaling, self.weights.get("rope_freqs.weight"),
+                                           self.device)
+            # GGUF files of the llama architecture store q and k for pairs (2i, 2i + 1),
+            # everything else for pairs (i, i + half)
+            inter = self._cfg("rope_interleaved", self._cfg("_gguf_arch_prefix") == "llama")
+            plan = self._rope = (steps, factor, bool(inter))
+        return plan
+
+    def _rot_dim(self) -> int:
+        return int(self._head_dim() * float(self._cfg("partial_rotary_factor", 1.0)))
+
+    def _head_dim(self) -> int:
+        return int(self._cfg("head_dim") or self._cfg("hidden_size") // self._cfg("num_attention_heads"))
+
+    def transformer_layer(self, layer: int, hidden: torch.Tensor, delta, step) -> tuple[torch.Tensor, torch.Tensor]:
+        """One layer over the tokens of ``step`` (``PagedKVCache.extend``). The residual
+        stream is ``hidden`` [tokens, hidden size] plus ``delta``, the previous layer's FFN
+        output (None before the first layer), added by the norm that reads it: returns the
+        stream after attention and this layer's FFN output, not yet added."""
+        heads, kv_heads, d = int(self._cfg("num_attention_heads")), int(self._cfg("num_key_value_heads")), self._head_dim()
+        eps, t, dev = float(self._cfg("rms_norm_eps", 1e-5)), hidden.shape[0], hidden.device
+        cache, dtype = step.cache, step.cache.dtype
+        base = f"model.layers.{layer}."
+        for name in ("q", "k", "v", "o"):
+            if base + f"self_attn.{name}_proj.bias" in self.weights:
+                raise NotImplementedError("projections with a bias are not supported")
+
+        def norm(x, name, residual):
+            w = self.weights[base + name]
+            if residual is None:
+                return ops.rms_norm(x, w, eps, out_dtype=dtype), x
+            return ops.rms_norm(x, w, eps, residual=residual, out_dtype=dtype)
+        normed, hidden = (norm(hidden, "input_layernorm.weight", None) if delta is None
+                          else norm(delta, "input_layernorm.weight", hidden))
+        qkv = torch.empty(t, (heads + 2 * kv_heads) * d, dtype=dtype, device=dev)
+        parts = qkv.split([heads * d, kv_heads * d, kv_heads * d], dim=1)
+        self.project_qkv(layer, normed, *parts)
+        q, k, v = (p.unflatten(1, (-1, d)) for p in parts)
+        for part, name in ((q, "q_norm"), (k, "k_norm")):  # per-head norms where the model has them
+            w = self.weights.get(base + f"self_attn.{name}.weight")
+            if w is not None:
+                part.copy_(ops.rms_norm(part, w, eps))
+        steps, factor, interleaved = self._rope_plan()
+        q = ops.rope_append(q, k, v, step.positions, steps, step.slots, cache.k[layer], cache.v[layer],
+                            interleaved=interleaved, factor=factor)
+        if step.decode:
+            attn = ops.paged_attention(q, cache.k[layer], cache.v[layer], step.block_tables, step.lens)
+        else:
+            attn = ops.paged_prompt_attention(q, step.q_starts, step.max_q, cache.k[layer], cache.v[layer],
+                                              step.block_tables, step.lens)
+        # the projections' 32-bit sums meet the stream in the norms, rounded once
+        o = self.project_o(layer, attn.view(t, heads * d), torch.empty(t, hidden.shape[1], device=dev))
+        normed, hidden = norm(o, "post_attention_layernorm.weight", hidden)
+        gate = self._w(layer, "gate")
+        act = torch.empty(t, gate.shape[0], dtype=dtype, device=dev)
+        self.project_ffn_act(layer, normed, act)
+        return hidden, self.project_down(layer, act, torch.empty(t, hidden.shape[1], device=dev))
+
+    def forward(self, input_ids: torch.Tensor, positions, attn_metadata) -> torch.Tensor:
+        """Logits [sequences, vocabulary] (float32) after the last new token of each sequence;
+        input_ids [tokens] in the order of ``attn_metadata``, the ``PagedKVCache.extend`` step
+        whose cache takes the tokens' keys and values. ``positions`` None: the step's. The
+        reference's forward (vllm_webgpu/models/llama.py:145-237) runs one token of one
+        sequence and returns its logits."""
+        step = attn_metadata if positions is None else dataclasses.replace(attn_metadata, positions=positions)
+        layers = int(self._cfg("num_hidden_layers"))
+        table = self.weights["model.embed_tokens.weight"]
+        ids = input_ids.reshape(-1)
+        if ids.shape[0] != step.positions.shape[0]:
+            raise ValueError(f"{ids.shape[0]} tokens for a step of {step.positions.shape[0]}")
+        hidden = torch.empty(ids.shape[0], table.shape[1], dtype=step.cache.dtype, device=self.device)
+        self.embed_tokens(ids, hidden)
+        delta = None
+        for layer in range(layers):
+            hidden, delta = self.transformer_layer(layer, hidden, delta, step)
+        last = (step.q_starts[1:] - 1).long()
+        if not step.decode:  # the rest of the prompt has no say in the logits
+            hidden, delta = hidden[last], delta[last]
+        normed, _ = ops.rms_norm(delta, self.weights["model.norm.weight"], float(self._cfg("rms_norm_eps", 1e-5)),
+                                 residual=hidden, out_dtype=step.cache.dtype)
+        head = self.weights.get("lm_head.weight", table)
+        return self._linear(normed, head, torch.empty(normed.shape[0], head.shape[0], device=self.device))
 
     def layer_linears(self, layer: int, normed, attn_out, ffn_normed, ffn_act, bufs: dict) -> dict:
         """All seven projections of one layer into caller-owned ``bufs``

@@ -9,6 +9,8 @@ live on a CUDA device and the native library must be present.
 """
 from __future__ import annotations
 
+import struct
+
 import torch
 
 from . import _lib
@@ -611,3 +613,312 @@ def mul_mat(x: torch.Tensor, w: GGUFQuantTensor, out: torch.Tensor | None = None
     else:
         y = gemm(x2, w, out=out, out_dtype=out_dtype)
     return y.reshape(*lead, w.n)
+
+
+# ---------------------------------------------------------------------------------------------
+# what lies between a layer's projections: norm, rotary positions, key-value cache, attention
+# (the reference's shaders of vllm_webgpu/models/llama.py:239-367)
+# ---------------------------------------------------------------------------------------------
+def _call(dev: torch.device, what: str, fn, *args) -> None:
+    """fn(*args, stream) with ``dev`` current, its status checked."""
+    if torch.cuda.current_device() == dev.index:
+        st = fn(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            st = fn(*args, torch.cuda.current_stream().cuda_stream)
+    if st:
+        _lib.check(st, what)
+
+
+def _norm_buffer(t: torch.Tensor, x: torch.Tensor, what: str, dev: torch.device) -> torch.Tensor:
+    """t, checked as an output of x's shape whose rows the kernel can write."""
+    if t.shape != x.shape or t.device != dev or t.stride(-1) != 1 or not (t.dim() == 2 or t.is_contiguous()):
+        raise ValueError(f"{what} must be a {tuple(x.shape)} tensor of contiguous rows on {dev}")
+    return t
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-5,
+             residual: torch.Tensor | None = None, out: torch.Tensor | None = None,
+             out_dtype: torch.dtype | None = None, residual_out: torch.Tensor | None = None,
+             weight_add: float = 0.0):
+    """Root-mean-square norm over the last dimension, s * (mean(s^2) + eps)^-1/2 *
+    (weight + weight_add) of s = x, or s = x + residual: then (out, residual_out) is
+    returned, residual_out holding s in the residual's dtype. The sum and the norm are
+    computed in 32 bits and rounded once each; x, residual, weight and out may have
+    different dtypes. ``residual_out`` may be ``residual`` and ``out`` may be ``x`` (in
+    place). Replaces the reference's add and rms_norm dispatches
+    (vllm_webgpu/models/llama.py:262-270, 335-341)."""
+    dev = _require_cuda(x) if residual is None else _require_cuda(x, residual)
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError("rms_norm needs at least one value in a row")
+    n = x.shape[-1]
+    x2 = x if x.dim() == 2 and x.stride(1) == 1 else _as_2d(x, n)
+    m = x2.shape[0]
+    if out is None:
+        y = torch.empty(x.shape, dtype=out_dtype or x.dtype, device=dev)
+    else:
+        y = _norm_buffer(out, x, "out", dev)
+    y2 = y if y.dim() == 2 else y.view(m, n)
+    r2 = ro2 = None
+    if residual is not None:
+        if residual.shape != x.shape:
+            raise ValueError(f"residual must be a {tuple(x.shape)} tensor")
+        r2 = residual if residual.dim() == 2 and residual.stride(1) == 1 else _as_2d(residual, n)
+        if residual_out is None:
+            residual_out = torch.empty(x.shape, dtype=residual.dtype, device=dev)
+        elif _norm_buffer(residual_out, x, "residual_out", dev).dtype != residual.dtype:
+            raise ValueError("residual_out must have the residual's dtype")
+        ro2 = residual_out if residual_out.dim() == 2 else residual_out.view(m, n)
+    elif residual_out is not None:
+        raise ValueError("residual_out needs a residual")
+    if weight is not None and (weight.shape != (n,) or weight.device != dev or not weight.is_contiguous()):
+        raise ValueError(f"weight must be a contiguous [{n}] tensor on {dev}")
+
+    def row(t):  # the stride of a single row says nothing
+        return t.stride(0) if m > 1 else n
+    _call(dev, "ggufmm_rms_norm", _lib.lib().ggufmm_rms_norm, x2.data_ptr(), _code(x2.dtype), m, n, row(x2),
+          None if r2 is None else r2.data_ptr(), 0 if r2 is None else _code(r2.dtype), 0 if r2 is None else row(r2),
+          None if ro2 is None else ro2.data_ptr(), 0 if ro2 is None else row(ro2),
+          None if weight is None else weight.data_ptr(), 0 if weight is None else _code(weight.dtype), weight_add, eps,
+          y2.data_ptr(), _code(y2.dtype), row(y2))
+    return y if residual is None else (y, residual_out)
+
+
+def rope_steps(rot_dim: int, theta: float = 10000.0, scaling: dict | None = None,
+               freq_factors=None, device=None) -> tuple[torch.Tensor, float]:
+    """The rotary frequencies as ``rope`` and ``rope_append`` take them, computed in 64
+    bits: (steps, factor), steps int64 [rot_dim / 2] the turn per position of each pair in
+    units of 2^-64 turns, factor the multiplier of the turned values.
+
+    ``scaling`` stretches them to long contexts, by its ``rope_type`` (the keys of Hugging
+    Face's ``rope_scaling``): "linear" (factor), "llama3" (factor, low_freq_factor,
+    high_freq_factor, original_max_position_embeddings) or "yarn" (factor,
+    original_max_position_embeddings, beta_fast, beta_slow, attention_factor).
+    ``freq_factors`` [rot_dim / 2] divides each frequency (GGUF's ``rope_freqs.weight``)."""
+    import math
+
+    import numpy as np
+    if rot_dim < 2 or rot_dim % 2:
+        raise ValueError(f"rot_dim must be a positive even number, not {rot_dim}")
+    if not theta > 0:
+        raise ValueError(f"theta must be positive, not {theta}")
+    half = rot_dim // 2
+    f = np.float64(theta) ** (-np.arange(half, dtype=np.float64) * 2 / rot_dim)  # radians per position
+    factor = 1.0
+    kind = (scaling or {}).get("rope_type", (scaling or {}).get("type", "default"))
+    if kind == "linear":
+        f = f / float(scaling["factor"])
+    elif kind == "llama3":
+        turns = float(scaling["original_max_position_embeddings"]) * f / (2 * math.pi)
+        low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+        if not high > low:
+            raise ValueError("llama3 scaling needs high_freq_factor > low_freq_factor")
+        keep = np.clip((turns - low) / (high - low), 0.0, 1.0)
+        f = keep * f + (1.0 - keep) * f / float(scaling["factor"])
+    elif kind == "yarn":
+        old, by = float(scaling["original_max_position_embeddings"]), float(scaling["factor"])
+
+        def pair_with(turns):  # the pair that makes so many turns over the original context
+            return rot_dim * math.log(old / (turns * 2 * math.pi)) / (2 * math.log(theta))
+        low = max(math.floor(pair_with(float(scaling.get("beta_fast", 32.0)))), 0)
+        high = min(math.ceil(pair_with(float(scaling.get("beta_slow", 1.0)))), rot_dim - 1)
+        ramp = np.clip((np.arange(half) - low) / max(high - low, 0.001), 0.0, 1.0)
+        f = f * (1.0 - ramp) + f / by * ramp
+        given = scaling.get("attention_factor")
+        factor = float(given) if given is not None else (0.1 * math.log(by) + 1.0 if by > 1 else 1.0)
+    elif kind != "default":
+        raise ValueError(f"rope scaling {kind!r} is not supported (supported: default, linear, llama3, yarn)")
+    if freq_factors is not None:
+        ff = np.asarray(torch.as_tensor(freq_factors).cpu(), dtype=np.float64)
+        if ff.shape != (half,):
+            raise ValueError(f"freq_factors must hold {half} values")
+        if not (np.isfinite(ff) & (ff != 0)).all():
+            raise ValueError("freq_factors must be finite and not zero")
+        f = f / ff
+    turns = np.remainder(f / (2 * math.pi), 1.0)  # whole turns change nothing at whole positions
+    steps = np.array([int(round(float(t) * 2.0 ** 64)) % 2 ** 64 for t in turns], dtype=np.uint64).view(np.int64)
+    return torch.from_numpy(steps.copy()).to(device if device is not None else "cuda"), factor
+
+
+def _heads(t: torch.Tensor, what: str, dev: torch.device) -> torch.Tensor:
+    """t as [tokens, heads, head_dim] with a unit stride in the last dimension, on dev."""
+    if t.dim() != 3 or t.device != dev:
+        raise ValueError(f"{what} must be a [tokens, heads, head_dim] tensor on {dev}")
+    return t if t.stride(2) == 1 else t.contiguous()
+
+
+def _index(t: torch.Tensor, dtype: torch.dtype, shape: tuple, what: str, dev: torch.device) -> torch.Tensor:
+    if t.device != dev or t.shape != shape:
+        raise ValueError(f"{what} must be a {list(shape)} tensor on {dev}")
+    return t if t.dtype == dtype and t.is_contiguous() else t.to(dtype).contiguous()
+
+
+def _cache_strides(k_cache: torch.Tensor, v_cache: torch.Tensor, dev: torch.device) -> tuple:
+    """The strides of page, head and slot of both caches [pages, kv heads, page size, head_dim]."""
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
+        raise ValueError("k_cache and v_cache must be [pages, kv heads, page size, head_dim] tensors of one shape and dtype")
+    if k_cache.device != dev or v_cache.device != dev:
+        raise ValueError(f"the cache must lie on {dev}")
+    ks, vs = k_cache.stride(), v_cache.stride()
+    if ks[3] != 1 or vs[3] != 1:
+        raise ValueError("the caches' last dimension must have unit stride")
+    if 1 in k_cache.shape[:3]:  # the stride of a dimension of one says nothing: any valid one does
+        d = k_cache.shape[3]
+        ks, vs = ([d if k_cache.shape[i] == 1 else st[i] for i in range(3)] for st in (ks, vs))
+    return ks[0], ks[1], ks[2], vs[0], vs[1], vs[2]
+
+
+_ROPE_ARGS = struct.Struct("Q2qQ2qQ2qQ2qQ3qQ3q3Q11qd")
+
+
+def _rope(q, k, v, positions, steps, slots, k_cache, v_cache, interleaved, factor, q_out):
+    dev = _require_cuda(q)
+    q = _heads(q, "q", dev)
+    t, hq, d = q.shape
+    if q_out is None:
+        q_out = torch.empty((t, hq, d), dtype=q.dtype, device=dev)
+    elif q_out.shape != q.shape or q_out.device != dev or q_out.stride(2) != 1:
+        raise ValueError(f"q_out must be a {tuple(q.shape)} tensor with unit stride in its last dimension")
+    positions = _index(positions, torch.int64, (t,), "positions", dev)
+    if steps.device != dev or steps.dtype != torch.int64 or steps.dim() != 1 or not steps.is_contiguous():
+        raise ValueError(f"steps must be the int64 tensor of rope_steps on {dev}")
+    if k is None:
+        kv = (0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+        hkv, cache_dtype, page, pages, slot_ptr = 0, 0, 0, 0, 0
+    else:
+        k, v = _heads(k, "k", dev), _heads(v, "v", dev)
+        hkv = k.shape[1]
+        if k.shape != (t, hkv, d) or v.shape != k.shape or k.dtype != q.dtype or v.dtype != q.dtype:
+            raise ValueError(f"k and v must be [{t}, kv heads, {d}] tensors of q's dtype")
+        st = _cache_strides(k_cache, v_cache, dev)
+        pages, page = k_cache.shape[0], k_cache.shape[2]
+        if k_cache.shape[1] != hkv or k_cache.shape[3] != d:
+            raise ValueError(f"the cache holds {k_cache.shape[1]} heads of {k_cache.shape[3]}, k has {hkv} of {d}")
+        slots = _index(slots, torch.int64, (t,), "slots", dev)
+        slot_ptr, cache_dtype = slots.data_ptr(), _code(k_cache.dtype)
+        kv = (k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+              k_cache.data_ptr(), *st[:3], v_cache.data_ptr(), *st[3:])
+    args = _ROPE_ARGS.pack(q.data_ptr(), q.stride(0), q.stride(1), q_out.data_ptr(), q_out.stride(0), q_out.stride(1), *kv,
+                           positions.data_ptr(), slot_ptr, steps.data_ptr(), t, hq, hkv, d, 2 * steps.shape[0],
+                           int(interleaved), _code(q.dtype), _code(q_out.dtype), cache_dtype, page, pages, factor)
+    _call(dev, "ggufmm_rope_append", _lib.lib().ggufmm_rope_append, args)
+    return q_out
+
+
+def rope(x: torch.Tensor, positions: torch.Tensor, steps: torch.Tensor, interleaved: bool = False,
+         factor: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotary positions on x [tokens, heads, head_dim]: the first 2 * len(steps) values of
+    each head turn in pairs (i, i + half) or, ``interleaved`` (as GGUF files of the Llama
+    family order them), (2i, 2i + 1), by positions[t] times the step of ``rope_steps``;
+    the rest passes. ``out`` may be x. Replaces the reference's rope dispatch
+    (vllm_webgpu/models/llama.py:286-298)."""
+    return _rope(x, None, None, positions, steps, None, None, None, interleaved, factor, out)
+
+
+def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, steps: torch.Tensor,
+                slots: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, interleaved: bool = False,
+                factor: float = 1.0, q_out: torch.Tensor | None = None) -> torch.Tensor:
+    """``rope`` on q and on k, with k and v appended to the paged cache, in one launch:
+    returns the turned q [tokens, q heads, head_dim] (in q's dtype, or into ``q_out``,
+    which may be q) and writes the turned k and v to slot slots[t] (offset s % page size of
+    page s // page size) of ``k_cache`` / ``v_cache`` [pages, kv heads, page size,
+    head_dim], f16 or bf16. A negative slot stores nothing; one past the last page too, and
+    sets bit 2 of the device status word. Replaces the reference's rope and kv_cache_store
+    dispatches (vllm_webgpu/models/llama.py:286-312)."""
+    if k is None or v is None or slots is None or k_cache is None or v_cache is None:
+        raise ValueError("rope_append needs k, v, slots and the caches (rope turns q alone)")
+    return _rope(q, k, v, positions, steps, slots, k_cache, v_cache, interleaved, factor, q_out)
+
+
+_ATTENTION_ARGS = struct.Struct("Q2qQ2qQ3qQ3qQ2q2Q10qd")
+_attention_workspaces: dict[tuple[int, int], torch.Tensor] = {}
+
+
+def attention_workspace(batch: int, q_heads: int, kv_heads: int, head_dim: int, device) -> torch.Tensor:
+    """A zero-filled workspace for ``paged_attention`` calls of up to this size, which a
+    program that captures CUDA graphs keeps for them (calls that may run at the same time
+    need one each)."""
+    need = int(_lib.lib().ggufmm_paged_attention_workspace_size(batch, q_heads, kv_heads, head_dim))
+    return torch.zeros(max(need, 256), dtype=torch.uint8, device=device)
+
+
+def _attention_workspace(batch: int, hq: int, hkv: int, d: int, dev: torch.device) -> torch.Tensor:
+    """The workspace of the current stream: one per stream, since calls on different streams
+    may overlap; inside a graph capture one of the capture's own, zeroed in the graph."""
+    if torch.cuda.is_current_stream_capturing():
+        return attention_workspace(batch, hq, hkv, d, dev)
+    key = (dev.index, torch.cuda.current_stream(dev).cuda_stream)
+    need = int(_lib.lib().ggufmm_paged_attention_workspace_size(batch, hq, hkv, d))
+    ws = _attention_workspaces.get(key)
+    if ws is None or ws.numel() < need:
+        ws = torch.zeros(max(need, 256), dtype=torch.uint8, device=dev)
+        _attention_workspaces[key] = ws
+    return ws
+
+
+def _attention_args(q, k_cache, v_cache, tables, lens, scale, window, out, q_starts, max_q):
+    dev = _require_cuda(q)
+    q = _heads(q, "q", dev)
+    t, hq, d = q.shape
+    st = _cache_strides(k_cache, v_cache, dev)
+    pages, hkv, page, dk = k_cache.shape
+    if dk != d or k_cache.dtype != q.dtype:
+        raise ValueError(f"q and the cache must share head_dim and dtype: {d} {q.dtype}, {dk} {k_cache.dtype}")
+    if hkv == 0 or hq % hkv:
+        raise ValueError(f"{hq} query heads are no multiple of {hkv} kv heads")
+    if out is None:
+        out = torch.empty((t, hq, d), dtype=q.dtype, device=dev)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(2) != 1:
+        raise ValueError(f"out must be a {tuple(q.shape)} {q.dtype} tensor with unit stride in its last dimension")
+    if tables.dim() != 2 or tables.device != dev:
+        raise ValueError(f"block_tables must be a [batch, pages] tensor on {dev}")
+    b, width = tables.shape
+    if tables.dtype != torch.int32 or tables.stride(1) != 1:
+        tables = tables.to(torch.int32).contiguous()
+    lens = _index(lens, torch.int32, (b,), "lens", dev)
+    starts = 0
+    if q_starts is not None:
+        q_starts = _index(q_starts, torch.int32, (b + 1,), "q_starts", dev)
+        starts = q_starts.data_ptr()
+    elif t != b:
+        raise ValueError(f"q holds {t} tokens for {b} sequences")
+    qs, os = q.stride(), out.stride()
+    if t == 1 or hq == 1:  # the stride of a dimension of one says nothing: any valid one does
+        qs, os = ((s[0] if t > 1 else hq * d, s[1] if hq > 1 else d) for s in (qs, os))
+    args = _ATTENTION_ARGS.pack(
+        q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], k_cache.data_ptr(), st[0], st[1], st[2],
+        v_cache.data_ptr(), st[3], st[4], st[5], tables.data_ptr(), max(tables.stride(0), width), width,
+        lens.data_ptr(), starts, b, t, max_q, hq, hkv, d, page, pages, _code(q.dtype), window,
+        d ** -0.5 if scale is None else scale)
+    return dev, args, out, (b, hq, hkv, d), (q, tables, lens, q_starts)
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                    lens: torch.Tensor, scale: float | None = None, window: int = 0, out: torch.Tensor | None = None,
+                    workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of one new token per sequence over a paged cache: q and out [batch, q heads,
+    head_dim] in the cache's dtype (f16 / bf16), caches [pages, kv heads, page size,
+    head_dim], block_tables int32 [batch, pages of the longest], lens int32 [batch] (the new
+    token included). ``scale`` defaults to head_dim^-1/2; ``window`` > 0 lets a token see
+    the last ``window`` positions only. A sequence of length 0 gives zeros. ``workspace``
+    (``attention_workspace``) defaults to one kept per stream. Replaces the reference's
+    score, softmax and output dispatches (vllm_webgpu/models/llama.py:314-326)."""
+    dev, args, out, sizes, keep = _attention_args(q, k_cache, v_cache, block_tables, lens, scale, window, out, None, 0)
+    if workspace is None:
+        workspace = _attention_workspace(*sizes, dev)
+    _call(dev, "ggufmm_paged_attention", _lib.lib().ggufmm_paged_attention, args, workspace.data_ptr(), workspace.numel())
+    return out
+
+
+def paged_prompt_attention(q: torch.Tensor, q_starts: torch.Tensor, max_q: int, k_cache: torch.Tensor,
+                           v_cache: torch.Tensor, block_tables: torch.Tensor, lens: torch.Tensor,
+                           scale: float | None = None, window: int = 0,
+                           out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of several new tokens per sequence over a paged cache that holds them
+    already: q and out [tokens, q heads, head_dim], sequence b's new tokens in rows
+    q_starts[b] to q_starts[b + 1] (int32 [batch + 1]), at the last positions of its
+    lens[b]; ``max_q`` is at least the longest run. Otherwise as ``paged_attention``. The
+    reference feeds a prompt token by token (run_inference.py:323-350)."""
+    dev, args, out, _, keep = _attention_args(q, k_cache, v_cache, block_tables, lens, scale, window, out, q_starts, max_q)
+    _call(dev, "ggufmm_paged_prompt_attention", _lib.lib().ggufmm_paged_prompt_attention, args)
+    return out

@@ -123,7 +123,14 @@ _GGUF_BLK = {
 }
 
 
+# Not in the reference's table, but needed for right positions: the divisors of the rotary
+# frequencies that files of long-context models carry.
+_GGUF_ROPE = "rope_freqs.weight"
+
+
 def _gguf_to_hf_name(gguf_name: str) -> str | None:
+    if gguf_name == _GGUF_ROPE:
+        return _GGUF_ROPE
     if gguf_name in _GGUF_TOP:
         return _GGUF_TOP[gguf_name]
     if gguf_name.startswith("blk."):
