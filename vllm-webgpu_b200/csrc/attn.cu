@@ -11,6 +11,9 @@
 
 namespace ggufmm {
 
+size_t paged_decode_workspace(int64_t head_dim);  // attn_decode.cu
+cudaError_t launch_paged_decode(const ggufmm_attention_args& p, void* workspace, cudaStream_t st);
+
 namespace {
 
 struct AttnArgs {
@@ -97,7 +100,7 @@ int check_attention(const ggufmm_attention_args& p, bool prompt) {
   if (s) return s;
   if (p.batch < 0 || p.batch > 65535 || p.total_q < 0 || p.total_q > kI32Max || p.q_heads < 1 || p.q_heads > 65535 ||
       p.q_heads % p.kv_heads || p.q_heads / p.kv_heads > GGUFMM_MAX_GROUP || p.table_width < 0 ||
-      p.table_row < p.table_width || p.table_width * p.page_size > kI32Max || p.window < 0 || p.window > kI32Max)
+      p.table_row < p.table_width || p.table_width * p.page_size > kI32Max / 2 || p.window < 0 || p.window > kI32Max)
     return GGUFMM_ERR_SHAPE;
   if (prompt ? (p.max_q < 0 || p.max_q > p.total_q) : p.total_q != p.batch) return GGUFMM_ERR_SHAPE;
   if (!std::isfinite(p.scale)) return GGUFMM_ERR_ARG;
@@ -130,8 +133,8 @@ using namespace ggufmm;
 
 extern "C" size_t ggufmm_paged_attention_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_heads,
                                                         int64_t head_dim) {
-  if (batch < 1 || q_heads < 1 || kv_heads < 1 || head_dim < 8) return 0;
-  return 256;
+  if (batch < 1 || q_heads < 1 || kv_heads < 1 || head_dim < 8 || head_dim > GGUFMM_MAX_HEAD_DIM) return 0;
+  return paged_decode_workspace(head_dim);
 }
 
 extern "C" int ggufmm_paged_attention(const ggufmm_attention_args* args, void* workspace, size_t workspace_bytes,
@@ -146,7 +149,7 @@ extern "C" int ggufmm_paged_attention(const ggufmm_attention_args* args, void* w
   if (!aligned_to(workspace, 256)) return GGUFMM_ERR_ALIGN;
   s = check_device();
   if (s) return s;
-  return launch_simple(p, 1, static_cast<cudaStream_t>(stream));
+  return record_cuda_status(launch_paged_decode(p, workspace, static_cast<cudaStream_t>(stream)));
 }
 
 extern "C" int ggufmm_paged_prompt_attention(const ggufmm_attention_args* args, void* stream) {
