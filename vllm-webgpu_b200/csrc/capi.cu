@@ -43,9 +43,10 @@ cudaError_t gemm_device_error(int* v, int clear, cudaStream_t st);
 cudaError_t gemv_i8_device_error(int* v, int clear, cudaStream_t st);
 cudaError_t dequant_device_error(int* v, int clear, cudaStream_t st);
 cudaError_t rope_device_error(int* v, int clear, cudaStream_t st);
-cudaError_t attn_device_error(int* v, int clear, cudaStream_t st);
+cudaError_t attn_prompt_device_error(int* v, int clear, cudaStream_t st);
 cudaError_t attn_decode_device_error(int* v, int clear, cudaStream_t st);
 cudaError_t attn_decode_set_wait_limit(uint32_t polls);
+cudaError_t attn_prompt_set_wait_limit(uint32_t polls);
 cudaError_t launch_embedding(const void* q, int qtype, int64_t n_vocab, int64_t k, const int32_t* ids, int64_t n_ids,
                              void* out, int out_dtype, int64_t ldo, cudaStream_t st);
 cudaError_t gemv_set_wait_limit(uint32_t polls);
@@ -199,7 +200,7 @@ int ggufmm_device_status(int clear, void* stream) {
   int r = 0, o = 0, t = 0, u = 0;
   if (e == cudaSuccess) e = allreduce_device_error(&r, clear, st);
   if (e == cudaSuccess) e = rope_device_error(&o, clear, st);
-  if (e == cudaSuccess) e = attn_device_error(&t, clear, st);
+  if (e == cudaSuccess) e = attn_prompt_device_error(&t, clear, st);
   if (e == cudaSuccess) e = attn_decode_device_error(&u, clear, st);
   if (e != cudaSuccess) return cuda_status(e);
   return a | b | c | d | f | h | r | o | t | u;
@@ -214,6 +215,7 @@ int ggufmm_set_wait_limit(uint32_t polls) {
   if (e == cudaSuccess) e = gemv_i8_set_wait_limit(v);
   if (e == cudaSuccess) e = allreduce_set_wait_limit(v);
   if (e == cudaSuccess) e = attn_decode_set_wait_limit(v);
+  if (e == cudaSuccess) e = attn_prompt_set_wait_limit(v);
   return cuda_status(e);
 }
 
