@@ -7,7 +7,7 @@
 // (vllm_webgpu/models/llama.py:262-270, :335-341; shaders/generic/{add,rms_norm}.wgsl),
 // with the stream rounded to f16 between them. Here the sum stays in 32 bits: it is
 // rounded once into r' and, after the norm, once into y.
-#include "common.cuh"
+#include "mma16.cuh"
 
 namespace ggufmm {
 
@@ -23,9 +23,9 @@ struct NormArgs {
   const void* w;
   void* y;
   int64_t ldx, ldr, ldro, ldy;
-  int n;
+  int m, n;
   int xt, rt, wt, yt;
-  float c, eps;
+  float c, eps, inv_n;
 };
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -34,35 +34,212 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// One row per CTA, two passes over it.
-__global__ void __launch_bounds__(256) rms_norm_kernel(NormArgs a) {
-  __shared__ float part[8];
+// The sum over a CTA of up to 32 warps, the same bits in every thread.
+__device__ __forceinline__ float cta_sum(float v, float* part) {
+  v = warp_sum(v);
+  const int nw = blockDim.x >> 5;
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  return warp_sum(lane < nw ? part[lane] : 0.f);
+}
+
+// Eight values of one row: raw bytes first, so that all of a thread's loads are in flight
+// before the first is converted.
+template <int ES>
+struct Raw8 {
+  uint4 v[ES / 2];
+};
+template <>
+struct Raw8<0> {};
+
+template <int ES>
+__device__ __forceinline__ void raw_load(Raw8<ES>& d, const void* p, int64_t i) {
+  const uint4* q = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) + i * ES);
+#pragma unroll
+  for (int k = 0; k < ES / 2; ++k) d.v[k] = q[k];
+}
+
+__device__ __forceinline__ void widen(uint32_t u, int t, float* f) {
+  if (t == GGUFMM_BF16) {
+    f[0] = __uint_as_float(u << 16);
+    f[1] = __uint_as_float(u & 0xFFFF0000u);
+  } else {
+    const float2 h = __half22float2(*reinterpret_cast<__half2*>(&u));
+    f[0] = h.x;
+    f[1] = h.y;
+  }
+}
+
+template <int ES>
+__device__ __forceinline__ void raw_float(const Raw8<ES>& d, int t, float* f) {
+  const uint32_t* u = reinterpret_cast<const uint32_t*>(d.v);
+  if constexpr (ES == 4) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = __uint_as_float(u[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) widen(u[k], t, f + 2 * k);
+  }
+}
+
+__device__ __forceinline__ void store8(void* p, int t, int64_t i, const float* f) {
+  if (t == GGUFMM_F32) {
+    float4* q = reinterpret_cast<float4*>(static_cast<float*>(p) + i);
+    q[0] = make_float4(f[0], f[1], f[2], f[3]);
+    q[1] = make_float4(f[4], f[5], f[6], f[7]);
+  } else {
+    uint4 v;
+    v.x = t == GGUFMM_F16 ? pack16<GGUFMM_F16>(f[0], f[1]) : pack16<GGUFMM_BF16>(f[0], f[1]);
+    v.y = t == GGUFMM_F16 ? pack16<GGUFMM_F16>(f[2], f[3]) : pack16<GGUFMM_BF16>(f[2], f[3]);
+    v.z = t == GGUFMM_F16 ? pack16<GGUFMM_F16>(f[4], f[5]) : pack16<GGUFMM_BF16>(f[4], f[5]);
+    v.w = t == GGUFMM_F16 ? pack16<GGUFMM_F16>(f[6], f[7]) : pack16<GGUFMM_BF16>(f[6], f[7]);
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) = v;
+  }
+}
+
+// Rows of whole 16-byte groups. A row is held in the registers of WARP ? one warp : one
+// CTA, V groups of eight values a thread; XS, RS: bytes of a value of x and of r (0: none).
+template <int XS, int RS, int V, bool WARP>
+__global__ void __launch_bounds__(WARP ? 256 : 1024) rms_norm_vec_kernel(const __grid_constant__ NormArgs a) {
+  __shared__ float part[32];
+  pdl_wait();
+  pdl_trigger();
+  const int64_t row = WARP ? static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5) : blockIdx.x;
+  if (row >= a.m) return;  // whole warps
+  const int tid = WARP ? threadIdx.x & 31 : threadIdx.x, nt = WARP ? 32 : blockDim.x;
+  Raw8<XS> xr[V];
+  Raw8<RS> rr[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    const int i = (tid + k * nt) * 8;
+    if (i < a.n) {
+      raw_load(xr[k], a.x, row * a.ldx + i);
+      if constexpr (RS != 0) raw_load(rr[k], a.r, row * a.ldr + i);
+    }
+  }
+  float s[V][8], ss = 0.f;
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    const int i = (tid + k * nt) * 8;
+    if (i < a.n) {
+      raw_float(xr[k], a.xt, s[k]);
+      if constexpr (RS != 0) {
+        float r[8];
+        raw_float(rr[k], a.rt, r);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[k][e] += r[e];
+        if (a.ro) store8(a.ro, a.rt, row * a.ldro + i, s[k]);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss = fmaf(s[k][e], s[k][e], ss);
+    }
+  }
+  ss = WARP ? warp_sum(ss) : cta_sum(ss, part);
+  const float inv = rsqrtf(fmaf(ss, a.inv_n, a.eps));
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    const int i = (tid + k * nt) * 8;
+    if (i < a.n) {
+      float w[8];
+      if (a.w) {
+        if (a.wt == GGUFMM_F32) {
+          Raw8<4> q;
+          raw_load(q, a.w, i);
+          raw_float(q, a.wt, w);
+        } else {
+          Raw8<2> q;
+          raw_load(q, a.w, i);
+          raw_float(q, a.wt, w);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = s[k][e] * inv * (w[e] + a.c);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = s[k][e] * inv;
+      }
+      store8(a.y, a.yt, row * a.ldy + i, w);
+    }
+  }
+}
+
+// Any width and alignment: one row per CTA, a value at a time, E of them held by a thread.
+// E == 0: wider rows, read twice (each value again by the thread that read it first, so
+// that y may be x and ro may be r).
+template <int E>
+__global__ void __launch_bounds__(E == 0 ? 1024 : 512) rms_norm_any_kernel(const __grid_constant__ NormArgs a) {
+  __shared__ float part[32];
   pdl_wait();
   pdl_trigger();
   const int64_t row = blockIdx.x;
-  float ss = 0.f;
-  for (int i = threadIdx.x; i < a.n; i += 256) {
-    float s = load_y_rt(a.x, a.xt, row * a.ldx + i);
-    if (a.r) s += load_y_rt(a.r, a.rt, row * a.ldr + i);
-    ss = fmaf(s, s, ss);
-  }
-  ss = warp_sum(ss);
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = ss;
-  __syncthreads();
-  float tot = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) tot += part[i];
-  const float inv = rsqrtf(tot / static_cast<float>(a.n) + a.eps);
-  // each element is read again and written by the thread that read it: y may be x and
-  // ro may be r, element for element
-  for (int i = threadIdx.x; i < a.n; i += 256) {
-    float s = load_y_rt(a.x, a.xt, row * a.ldx + i);
-    if (a.r) s += load_y_rt(a.r, a.rt, row * a.ldr + i);
-    if (a.ro) store_y_rt(a.ro, a.rt, row * a.ldro + i, s);
-    float v = s * inv;
+  auto sum_at = [&](int i) {
+    float v = load_y_rt(a.x, a.xt, row * a.ldx + i);
+    if (a.r) v += load_y_rt(a.r, a.rt, row * a.ldr + i);
+    return v;
+  };
+  auto finish = [&](int i, float v, float inv) {
+    if (a.ro) store_y_rt(a.ro, a.rt, row * a.ldro + i, v);
+    v *= inv;
     if (a.w) v *= load_y_rt(a.w, a.wt, i) + a.c;
     store_y_rt(a.y, a.yt, row * a.ldy + i, v);
+  };
+  float s[E ? E : 1], ss = 0.f;
+  if constexpr (E != 0) {
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+      const int i = threadIdx.x + k * blockDim.x;
+      s[k] = i < a.n ? sum_at(i) : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < E; ++k) ss = fmaf(s[k], s[k], ss);
+  } else {
+    for (int i = threadIdx.x; i < a.n; i += blockDim.x) {
+      const float v = sum_at(i);
+      ss = fmaf(v, v, ss);
+    }
   }
+  const float inv = rsqrtf(fmaf(cta_sum(ss, part), a.inv_n, a.eps));
+  if constexpr (E != 0) {
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+      const int i = threadIdx.x + k * blockDim.x;
+      if (i < a.n) finish(i, s[k], inv);
+    }
+  } else {
+    for (int i = threadIdx.x; i < a.n; i += blockDim.x) finish(i, sum_at(i), inv);
+  }
+}
+
+template <int XS, int RS>
+cudaError_t launch_vec(const NormArgs& a, cudaStream_t st) {
+  const int groups = a.n / 8;
+  const dim3 rows8(static_cast<unsigned>((static_cast<int64_t>(a.m) + 7) / 8)), rows(static_cast<unsigned>(a.m));
+  // a warp per row up to 1024 values, above it a CTA with two (up to 16384) or four groups
+  if (groups <= 32) return pdl_launch(rms_norm_vec_kernel<XS, RS, 1, true>, rows8, dim3(256), 0, st, a);
+  if (groups <= 64) return pdl_launch(rms_norm_vec_kernel<XS, RS, 2, true>, rows8, dim3(256), 0, st, a);
+  if (groups <= 128) return pdl_launch(rms_norm_vec_kernel<XS, RS, 4, true>, rows8, dim3(256), 0, st, a);
+  const int v = groups <= 2048 ? 2 : 4;
+  const dim3 block(static_cast<unsigned>(((groups + v - 1) / v + 31) / 32 * 32));
+  if (v == 2) return pdl_launch(rms_norm_vec_kernel<XS, RS, 2, false>, rows, block, 0, st, a);
+  return pdl_launch(rms_norm_vec_kernel<XS, RS, 4, false>, rows, block, 0, st, a);
+}
+
+cudaError_t launch_norm(const NormArgs& a, cudaStream_t st) {
+  auto whole = [](const void* p, int dt, int64_t ld) {  // null, or 16-byte aligned in every row
+    return !p || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * (dt == GGUFMM_F32 ? 4 : 2) % 16 == 0);
+  };
+  if (a.n % 8 == 0 && a.n <= 32768 && whole(a.x, a.xt, a.ldx) && whole(a.r, a.rt, a.ldr) &&
+      whole(a.ro, a.rt, a.ldro) && whole(a.w, a.wt, 0) && whole(a.y, a.yt, a.ldy)) {
+    const bool x4 = a.xt == GGUFMM_F32;
+    if (!a.r) return x4 ? launch_vec<4, 0>(a, st) : launch_vec<2, 0>(a, st);
+    if (a.rt == GGUFMM_F32) return x4 ? launch_vec<4, 4>(a, st) : launch_vec<2, 4>(a, st);
+    return x4 ? launch_vec<4, 2>(a, st) : launch_vec<2, 2>(a, st);
+  }
+  const dim3 grid(static_cast<unsigned>(a.m));
+  auto block = [&](int e) { return dim3(static_cast<unsigned>((((a.n + e - 1) / e) + 31) / 32 * 32)); };
+  if (a.n <= 1024) return pdl_launch(rms_norm_any_kernel<4>, grid, block(4), 0, st, a);
+  if (a.n <= 8192) return pdl_launch(rms_norm_any_kernel<16>, grid, block(16), 0, st, a);
+  return pdl_launch(rms_norm_any_kernel<0>, grid, dim3(1024), 0, st, a);
 }
 
 int elem(int dtype) { return dtype == GGUFMM_F32 ? 4 : dtype == GGUFMM_F16 || dtype == GGUFMM_BF16 ? 2 : 0; }
@@ -89,8 +266,7 @@ extern "C" int ggufmm_rms_norm(const void* x, int x_dtype, int64_t m, int64_t n,
   if (!al(x, xe) || !al(y, ye) || !al(w, we) || !al(resid, re) || !al(resid_out, re)) return GGUFMM_ERR_ALIGN;
   const int s = check_device();
   if (s) return s;
-  const NormArgs a{x, resid, resid_out, w, y, ldx, ldr, ldro, ldy, static_cast<int>(n), x_dtype, r_dtype, w_dtype,
-                   y_dtype, w_add, eps};
-  return record_cuda_status(pdl_launch(rms_norm_kernel, dim3(static_cast<unsigned>(m)), dim3(256), 0,
-                                       static_cast<cudaStream_t>(stream), a));
+  const NormArgs a{x,   resid, resid_out, w,       y,       ldx,     ldr,   ldro, ldy, static_cast<int>(m), static_cast<int>(n),
+                   x_dtype, r_dtype, w_dtype, y_dtype, w_add, eps,  1.f / static_cast<float>(n)};
+  return record_cuda_status(launch_norm(a, static_cast<cudaStream_t>(stream)));
 }

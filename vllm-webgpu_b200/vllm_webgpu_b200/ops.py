@@ -619,22 +619,40 @@ def mul_mat(x: torch.Tensor, w: GGUFQuantTensor, out: torch.Tensor | None = None
 # what lies between a layer's projections: norm, rotary positions, key-value cache, attention
 # (the reference's shaders of vllm_webgpu/models/llama.py:239-367)
 # ---------------------------------------------------------------------------------------------
-def _call(dev: torch.device, what: str, fn, *args) -> None:
-    """fn(*args, stream) with ``dev`` current, its status checked."""
-    if torch.cuda.current_device() == dev.index:
-        st = fn(*args, torch.cuda.current_stream().cuda_stream)
+# These calls are short next to their launch, so their wrappers keep to few tensor attributes.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _call(index: int, what: str, fn, *args) -> None:
+    """fn(*args, stream) with CUDA device ``index`` current, its status checked."""
+    if torch.cuda.current_device() == index:
+        st = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(dev):
-            st = fn(*args, torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(index):
+            st = fn(*args, _raw_stream(index))
     if st:
         _lib.check(st, what)
 
 
-def _norm_buffer(t: torch.Tensor, x: torch.Tensor, what: str, dev: torch.device) -> torch.Tensor:
-    """t, checked as an output of x's shape whose rows the kernel can write."""
-    if t.shape != x.shape or t.device != dev or t.stride(-1) != 1 or not (t.dim() == 2 or t.is_contiguous()):
-        raise ValueError(f"{what} must be a {tuple(x.shape)} tensor of contiguous rows on {dev}")
-    return t
+def _new(shape, dtype: torch.dtype, like: torch.Tensor) -> torch.Tensor:
+    """An uninitialised contiguous tensor beside ``like`` (quickest where like has its form)."""
+    if like.dtype is dtype and like.shape == shape and like.is_contiguous():
+        return torch.empty_like(like)
+    return torch.empty(shape, dtype=dtype, device=like.device)
+
+
+def _norm_rows(t: torch.Tensor, x: torch.Tensor, n: int, m: int, what: str | None) -> tuple[torch.Tensor, int]:
+    """t as rows of n values, and the stride of a row: an input (what None: copied where its
+    layout allows no rows) or an output."""
+    if t.shape != x.shape or t.get_device() != x.get_device():
+        raise ValueError(f"{what or 'residual'} must be a {tuple(x.shape)} tensor on {x.device}")
+    if t.is_contiguous():
+        return t, n
+    if t.dim() == 2 and t.stride(1) == 1:
+        return t, t.stride(0) if m > 1 else n
+    if what is not None:
+        raise ValueError(f"{what} must be contiguous, or two-dimensional with contiguous rows")
+    return t.contiguous(), n
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-5,
@@ -648,40 +666,41 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1
     different dtypes. ``residual_out`` may be ``residual`` and ``out`` may be ``x`` (in
     place). Replaces the reference's add and rms_norm dispatches
     (vllm_webgpu/models/llama.py:262-270, 335-341)."""
-    dev = _require_cuda(x) if residual is None else _require_cuda(x, residual)
-    if x.dim() == 0 or x.shape[-1] == 0:
+    if not x.is_cuda:
+        _require_cuda(x)
+    shape = x.shape
+    if not shape or not shape[-1]:
         raise ValueError("rms_norm needs at least one value in a row")
-    n = x.shape[-1]
-    x2 = x if x.dim() == 2 and x.stride(1) == 1 else _as_2d(x, n)
-    m = x2.shape[0]
-    if out is None:
-        y = torch.empty(x.shape, dtype=out_dtype or x.dtype, device=dev)
-    else:
-        y = _norm_buffer(out, x, "out", dev)
-    y2 = y if y.dim() == 2 else y.view(m, n)
-    r2 = ro2 = None
+    n, index = shape[-1], x.get_device()
+    m = x.numel() // n
+    x2, ldx = _norm_rows(x, x, n, m, None)
+    r2, r_ptr, r_code, ldr, ro_ptr, ldro = None, None, 0, 0, None, 0
     if residual is not None:
-        if residual.shape != x.shape:
-            raise ValueError(f"residual must be a {tuple(x.shape)} tensor")
-        r2 = residual if residual.dim() == 2 and residual.stride(1) == 1 else _as_2d(residual, n)
+        r2, ldr = _norm_rows(residual, x, n, m, None)
+        r_ptr, r_code = r2.data_ptr(), _code(r2.dtype)
         if residual_out is None:
-            residual_out = torch.empty(x.shape, dtype=residual.dtype, device=dev)
-        elif _norm_buffer(residual_out, x, "residual_out", dev).dtype != residual.dtype:
-            raise ValueError("residual_out must have the residual's dtype")
-        ro2 = residual_out if residual_out.dim() == 2 else residual_out.view(m, n)
+            residual_out, ldro = _new(shape, residual.dtype, r2), n
+        else:
+            if residual_out.dtype is not residual.dtype:
+                raise ValueError("residual_out must have the residual's dtype")
+            _, ldro = _norm_rows(residual_out, x, n, m, "residual_out")
+        ro_ptr = residual_out.data_ptr()
     elif residual_out is not None:
         raise ValueError("residual_out needs a residual")
-    if weight is not None and (weight.shape != (n,) or weight.device != dev or not weight.is_contiguous()):
-        raise ValueError(f"weight must be a contiguous [{n}] tensor on {dev}")
-
-    def row(t):  # the stride of a single row says nothing
-        return t.stride(0) if m > 1 else n
-    _call(dev, "ggufmm_rms_norm", _lib.lib().ggufmm_rms_norm, x2.data_ptr(), _code(x2.dtype), m, n, row(x2),
-          None if r2 is None else r2.data_ptr(), 0 if r2 is None else _code(r2.dtype), 0 if r2 is None else row(r2),
-          None if ro2 is None else ro2.data_ptr(), 0 if ro2 is None else row(ro2),
-          None if weight is None else weight.data_ptr(), 0 if weight is None else _code(weight.dtype), weight_add, eps,
-          y2.data_ptr(), _code(y2.dtype), row(y2))
-    return y if residual is None else (y, residual_out)
+    if out is None:
+        dtype = out_dtype or x.dtype
+        out, ldy = _new(shape, dtype, r2 if r2 is not None and r2.dtype is dtype else x2), n
+    else:
+        _, ldy = _norm_rows(out, x, n, m, "out")
+        dtype = out.dtype
+    w_ptr = w_code = 0
+    if weight is not None:
+        if weight.dim() != 1 or weight.numel() != n or weight.get_device() != index or not weight.is_contiguous():
+            raise ValueError(f"weight must be a contiguous [{n}] tensor on {x.device}")
+        w_ptr, w_code = weight.data_ptr(), _code(weight.dtype)
+    _call(index, "ggufmm_rms_norm", _lib.lib().ggufmm_rms_norm, x2.data_ptr(), _code(x2.dtype), m, n, ldx, r_ptr, r_code,
+          ldr, ro_ptr, ldro, w_ptr, w_code, weight_add, eps, out.data_ptr(), _code(dtype), ldy)
+    return out if residual is None else (out, residual_out)
 
 
 def rope_steps(rot_dim: int, theta: float = 10000.0, scaling: dict | None = None,
@@ -740,68 +759,72 @@ def rope_steps(rot_dim: int, theta: float = 10000.0, scaling: dict | None = None
     return torch.from_numpy(steps.copy()).to(device if device is not None else "cuda"), factor
 
 
-def _heads(t: torch.Tensor, what: str, dev: torch.device) -> torch.Tensor:
-    """t as [tokens, heads, head_dim] with a unit stride in the last dimension, on dev."""
-    if t.dim() != 3 or t.device != dev:
-        raise ValueError(f"{what} must be a [tokens, heads, head_dim] tensor on {dev}")
+def _heads(t: torch.Tensor, what: str, index: int) -> torch.Tensor:
+    """t as [tokens, heads, head_dim] with a unit stride in the last dimension, on device ``index``."""
+    if t.dim() != 3 or t.get_device() != index:
+        raise ValueError(f"{what} must be a [tokens, heads, head_dim] tensor on cuda:{index}")
     return t if t.stride(2) == 1 else t.contiguous()
 
 
-def _index(t: torch.Tensor, dtype: torch.dtype, shape: tuple, what: str, dev: torch.device) -> torch.Tensor:
-    if t.device != dev or t.shape != shape:
-        raise ValueError(f"{what} must be a {list(shape)} tensor on {dev}")
-    return t if t.dtype == dtype and t.is_contiguous() else t.to(dtype).contiguous()
+def _index(t: torch.Tensor, dtype: torch.dtype, length: int, what: str, index: int) -> torch.Tensor:
+    if t.dim() != 1 or t.numel() != length or t.get_device() != index:
+        raise ValueError(f"{what} must be a [{length}] tensor on cuda:{index}")
+    return t if t.dtype is dtype and t.is_contiguous() else t.to(dtype).contiguous()
 
 
-def _cache_strides(k_cache: torch.Tensor, v_cache: torch.Tensor, dev: torch.device) -> tuple:
-    """The strides of page, head and slot of both caches [pages, kv heads, page size, head_dim]."""
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
+def _cache_strides(k_cache: torch.Tensor, v_cache: torch.Tensor, index: int) -> tuple:
+    """(shape, strides of page, head and slot of k, of v) of caches [pages, kv heads, page size, head_dim]."""
+    shape = k_cache.shape
+    if len(shape) != 4 or shape != v_cache.shape or k_cache.dtype is not v_cache.dtype:
         raise ValueError("k_cache and v_cache must be [pages, kv heads, page size, head_dim] tensors of one shape and dtype")
-    if k_cache.device != dev or v_cache.device != dev:
-        raise ValueError(f"the cache must lie on {dev}")
+    if k_cache.get_device() != index or v_cache.get_device() != index:
+        raise ValueError(f"the cache must lie on cuda:{index}")
     ks, vs = k_cache.stride(), v_cache.stride()
     if ks[3] != 1 or vs[3] != 1:
         raise ValueError("the caches' last dimension must have unit stride")
-    if 1 in k_cache.shape[:3]:  # the stride of a dimension of one says nothing: any valid one does
-        d = k_cache.shape[3]
-        ks, vs = ([d if k_cache.shape[i] == 1 else st[i] for i in range(3)] for st in (ks, vs))
-    return ks[0], ks[1], ks[2], vs[0], vs[1], vs[2]
+    if 1 in shape:  # the stride of a dimension of one says nothing: any valid one does
+        d = shape[3]
+        ks, vs = ([d if shape[i] == 1 else st[i] for i in range(3)] for st in (ks, vs))
+    return shape, ks[:3], vs[:3]
 
 
 _ROPE_ARGS = struct.Struct("Q2qQ2qQ2qQ2qQ3qQ3q3Q11qd")
 
 
 def _rope(q, k, v, positions, steps, slots, k_cache, v_cache, interleaved, factor, q_out):
-    dev = _require_cuda(q)
-    q = _heads(q, "q", dev)
+    if not q.is_cuda:
+        _require_cuda(q)
+    index = q.get_device()
+    q = _heads(q, "q", index)
     t, hq, d = q.shape
+    dtype = q.dtype
     if q_out is None:
-        q_out = torch.empty((t, hq, d), dtype=q.dtype, device=dev)
-    elif q_out.shape != q.shape or q_out.device != dev or q_out.stride(2) != 1:
+        q_out = _new(q.shape, dtype, q)
+    elif q_out.shape != q.shape or q_out.get_device() != index or q_out.stride(2) != 1:
         raise ValueError(f"q_out must be a {tuple(q.shape)} tensor with unit stride in its last dimension")
-    positions = _index(positions, torch.int64, (t,), "positions", dev)
-    if steps.device != dev or steps.dtype != torch.int64 or steps.dim() != 1 or not steps.is_contiguous():
-        raise ValueError(f"steps must be the int64 tensor of rope_steps on {dev}")
+    positions = _index(positions, torch.int64, t, "positions", index)
+    if steps.get_device() != index or steps.dtype is not torch.int64 or steps.dim() != 1 or not steps.is_contiguous():
+        raise ValueError(f"steps must be the int64 tensor of rope_steps on cuda:{index}")
+    qs, os = q.stride(), q_out.stride()
     if k is None:
         kv = (0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
         hkv, cache_dtype, page, pages, slot_ptr = 0, 0, 0, 0, 0
     else:
-        k, v = _heads(k, "k", dev), _heads(v, "v", dev)
+        k, v = _heads(k, "k", index), _heads(v, "v", index)
         hkv = k.shape[1]
-        if k.shape != (t, hkv, d) or v.shape != k.shape or k.dtype != q.dtype or v.dtype != q.dtype:
+        if k.shape != (t, hkv, d) or v.shape != k.shape or k.dtype is not dtype or v.dtype is not dtype:
             raise ValueError(f"k and v must be [{t}, kv heads, {d}] tensors of q's dtype")
-        st = _cache_strides(k_cache, v_cache, dev)
-        pages, page = k_cache.shape[0], k_cache.shape[2]
-        if k_cache.shape[1] != hkv or k_cache.shape[3] != d:
-            raise ValueError(f"the cache holds {k_cache.shape[1]} heads of {k_cache.shape[3]}, k has {hkv} of {d}")
-        slots = _index(slots, torch.int64, (t,), "slots", dev)
+        (pages, heads, page, dk), kst, vst = _cache_strides(k_cache, v_cache, index)
+        if heads != hkv or dk != d:
+            raise ValueError(f"the cache holds {heads} heads of {dk}, k has {hkv} of {d}")
+        slots = _index(slots, torch.int64, t, "slots", index)
         slot_ptr, cache_dtype = slots.data_ptr(), _code(k_cache.dtype)
-        kv = (k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-              k_cache.data_ptr(), *st[:3], v_cache.data_ptr(), *st[3:])
-    args = _ROPE_ARGS.pack(q.data_ptr(), q.stride(0), q.stride(1), q_out.data_ptr(), q_out.stride(0), q_out.stride(1), *kv,
-                           positions.data_ptr(), slot_ptr, steps.data_ptr(), t, hq, hkv, d, 2 * steps.shape[0],
-                           int(interleaved), _code(q.dtype), _code(q_out.dtype), cache_dtype, page, pages, factor)
-    _call(dev, "ggufmm_rope_append", _lib.lib().ggufmm_rope_append, args)
+        s, u = k.stride(), v.stride()
+        kv = (k.data_ptr(), s[0], s[1], v.data_ptr(), u[0], u[1], k_cache.data_ptr(), *kst, v_cache.data_ptr(), *vst)
+    args = _ROPE_ARGS.pack(q.data_ptr(), qs[0], qs[1], q_out.data_ptr(), os[0], os[1], *kv, positions.data_ptr(), slot_ptr,
+                           steps.data_ptr(), t, hq, hkv, d, 2 * steps.shape[0], 1 if interleaved else 0, _code(dtype),
+                           _code(q_out.dtype), cache_dtype, page, pages, factor)
+    _call(index, "ggufmm_rope_append", _lib.lib().ggufmm_rope_append, args)
     return q_out
 
 
@@ -842,55 +865,63 @@ def attention_workspace(batch: int, q_heads: int, kv_heads: int, head_dim: int, 
     return torch.zeros(max(need, 256), dtype=torch.uint8, device=device)
 
 
-def _attention_workspace(batch: int, hq: int, hkv: int, d: int, dev: torch.device) -> torch.Tensor:
+_attention_workspace_bytes: dict[tuple, int] = {}
+
+
+def _attention_workspace(batch: int, hq: int, hkv: int, d: int, index: int) -> torch.Tensor:
     """The workspace of the current stream: one per stream, since calls on different streams
     may overlap; inside a graph capture one of the capture's own, zeroed in the graph."""
     if torch.cuda.is_current_stream_capturing():
-        return attention_workspace(batch, hq, hkv, d, dev)
-    key = (dev.index, torch.cuda.current_stream(dev).cuda_stream)
-    need = int(_lib.lib().ggufmm_paged_attention_workspace_size(batch, hq, hkv, d))
+        return attention_workspace(batch, hq, hkv, d, torch.device("cuda", index))
+    size = (batch, hq, hkv, d)
+    need = _attention_workspace_bytes.get(size)
+    if need is None:
+        need = _attention_workspace_bytes[size] = int(_lib.lib().ggufmm_paged_attention_workspace_size(*size))
+    key = (index, _raw_stream(index))
     ws = _attention_workspaces.get(key)
     if ws is None or ws.numel() < need:
-        ws = torch.zeros(max(need, 256), dtype=torch.uint8, device=dev)
+        ws = torch.zeros(max(need, 256), dtype=torch.uint8, device=torch.device("cuda", index))
         _attention_workspaces[key] = ws
     return ws
 
 
 def _attention_args(q, k_cache, v_cache, tables, lens, scale, window, out, q_starts, max_q):
-    dev = _require_cuda(q)
-    q = _heads(q, "q", dev)
+    """(device index, packed arguments, out, sizes, the tensors the arguments point to)."""
+    if not q.is_cuda:
+        _require_cuda(q)
+    index = q.get_device()
+    q = _heads(q, "q", index)
     t, hq, d = q.shape
-    st = _cache_strides(k_cache, v_cache, dev)
-    pages, hkv, page, dk = k_cache.shape
-    if dk != d or k_cache.dtype != q.dtype:
-        raise ValueError(f"q and the cache must share head_dim and dtype: {d} {q.dtype}, {dk} {k_cache.dtype}")
+    (pages, hkv, page, dk), ks, vs = _cache_strides(k_cache, v_cache, index)
+    dtype = q.dtype
+    if dk != d or k_cache.dtype is not dtype:
+        raise ValueError(f"q and the cache must share head_dim and dtype: {d} {dtype}, {dk} {k_cache.dtype}")
     if hkv == 0 or hq % hkv:
         raise ValueError(f"{hq} query heads are no multiple of {hkv} kv heads")
     if out is None:
-        out = torch.empty((t, hq, d), dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(2) != 1:
-        raise ValueError(f"out must be a {tuple(q.shape)} {q.dtype} tensor with unit stride in its last dimension")
-    if tables.dim() != 2 or tables.device != dev:
-        raise ValueError(f"block_tables must be a [batch, pages] tensor on {dev}")
+        out = _new(q.shape, dtype, q)
+    elif out.shape != q.shape or out.dtype is not dtype or out.get_device() != index or out.stride(2) != 1:
+        raise ValueError(f"out must be a {tuple(q.shape)} {dtype} tensor with unit stride in its last dimension")
+    if tables.dim() != 2 or tables.get_device() != index:
+        raise ValueError(f"block_tables must be a [batch, pages] tensor on cuda:{index}")
     b, width = tables.shape
-    if tables.dtype != torch.int32 or tables.stride(1) != 1:
+    if tables.dtype is not torch.int32 or (width > 1 and tables.stride(1) != 1):
         tables = tables.to(torch.int32).contiguous()
-    lens = _index(lens, torch.int32, (b,), "lens", dev)
+    lens = _index(lens, torch.int32, b, "lens", index)
     starts = 0
     if q_starts is not None:
-        q_starts = _index(q_starts, torch.int32, (b + 1,), "q_starts", dev)
+        q_starts = _index(q_starts, torch.int32, b + 1, "q_starts", index)
         starts = q_starts.data_ptr()
     elif t != b:
         raise ValueError(f"q holds {t} tokens for {b} sequences")
     qs, os = q.stride(), out.stride()
     if t == 1 or hq == 1:  # the stride of a dimension of one says nothing: any valid one does
-        qs, os = ((s[0] if t > 1 else hq * d, s[1] if hq > 1 else d) for s in (qs, os))
+        qs, os = ((st[0] if t > 1 else hq * d, st[1] if hq > 1 else d) for st in (qs, os))
     args = _ATTENTION_ARGS.pack(
-        q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], k_cache.data_ptr(), st[0], st[1], st[2],
-        v_cache.data_ptr(), st[3], st[4], st[5], tables.data_ptr(), max(tables.stride(0), width), width,
-        lens.data_ptr(), starts, b, t, max_q, hq, hkv, d, page, pages, _code(q.dtype), window,
-        d ** -0.5 if scale is None else scale)
-    return dev, args, out, (b, hq, hkv, d), (q, tables, lens, q_starts)
+        q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], k_cache.data_ptr(), *ks, v_cache.data_ptr(), *vs,
+        tables.data_ptr(), tables.stride(0) if b > 1 else width, width, lens.data_ptr(), starts, b, t, max_q, hq, hkv, d,
+        page, pages, _code(dtype), window, d ** -0.5 if scale is None else scale)
+    return index, args, out, (b, hq, hkv, d), (q, tables, lens, q_starts)
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
@@ -903,10 +934,12 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     the last ``window`` positions only. A sequence of length 0 gives zeros. ``workspace``
     (``attention_workspace``) defaults to one kept per stream. Replaces the reference's
     score, softmax and output dispatches (vllm_webgpu/models/llama.py:314-326)."""
-    dev, args, out, sizes, keep = _attention_args(q, k_cache, v_cache, block_tables, lens, scale, window, out, None, 0)
+    index, args, out, sizes, keep = _attention_args(q, k_cache, v_cache, block_tables, lens, scale, window, out, None, 0)
     if workspace is None:
-        workspace = _attention_workspace(*sizes, dev)
-    _call(dev, "ggufmm_paged_attention", _lib.lib().ggufmm_paged_attention, args, workspace.data_ptr(), workspace.numel())
+        workspace = _attention_workspace(*sizes, index)
+    elif workspace.get_device() != index:
+        raise ValueError(f"workspace must lie on cuda:{index}")
+    _call(index, "ggufmm_paged_attention", _lib.lib().ggufmm_paged_attention, args, workspace.data_ptr(), workspace.numel())
     return out
 
 
@@ -919,6 +952,7 @@ def paged_prompt_attention(q: torch.Tensor, q_starts: torch.Tensor, max_q: int, 
     q_starts[b] to q_starts[b + 1] (int32 [batch + 1]), at the last positions of its
     lens[b]; ``max_q`` is at least the longest run. Otherwise as ``paged_attention``. The
     reference feeds a prompt token by token (run_inference.py:323-350)."""
-    dev, args, out, _, keep = _attention_args(q, k_cache, v_cache, block_tables, lens, scale, window, out, q_starts, max_q)
-    _call(dev, "ggufmm_paged_prompt_attention", _lib.lib().ggufmm_paged_prompt_attention, args)
+    index, args, out, _, keep = _attention_args(q, k_cache, v_cache, block_tables, lens, scale, window, out, q_starts,
+                                                max_q)
+    _call(index, "ggufmm_paged_prompt_attention", _lib.lib().ggufmm_paged_prompt_attention, args)
     return out
