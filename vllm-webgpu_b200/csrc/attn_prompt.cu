@@ -19,7 +19,8 @@
 // stays in TMEM; it is rescaled only when a row's maximum has grown by more than 2^8 since its
 // last rescaling (the weights then reach at most 2^8, harmless in 32-bit sums).
 //
-// Warps: 4 softmax warps per query tile, one that loads, one that issues the products.
+// Warps: 8 softmax warps per query tile (two share a row quadrant and halve its columns), one
+// that loads, one that issues the products.
 #include <algorithm>
 #include <atomic>
 
@@ -36,16 +37,27 @@ struct PShape {
   static constexpr int NQ = DP == 256 ? 1 : 2;     // query tiles
   static constexpr int BN = DP == 256 ? 64 : 128;  // keys of a tile
   static constexpr int NB = DP / 64;               // 128-byte column blocks of a row
-  static constexpr int NS = 2;                     // score buffers: one per query tile, or two in turn
-  static constexpr int KS = 2, VS = 2;             // stages
+  static constexpr int QC = BN / 4;                // a softmax thread's scores of each half of a tile
   static constexpr int QB = 128 * DP * 2, KB = BN * DP * 2;
-  static constexpr int BARS = NQ * QB + (KS + VS) * KB;
-  static constexpr int SMEM = BARS + 256 + 1024;
-  static constexpr int SCOL = BN;                  // TMEM columns of a score buffer
-  static constexpr int OCOL = NS * BN;             // first column of the outputs
-  static constexpr int COLS = OCOL + NQ * DP <= 256 ? 256 : 512;
-  static constexpr int THREADS = NQ * 128 + 64;
+  static constexpr int SLOTS = DP == 64 ? 8 : 5;   // tiles of keys or values in flight
+  static constexpr int XCH = NQ * QB + SLOTS * KB; // [NQ][2][128] exchange between column halves
+  static constexpr int BARS = XCH + NQ * 256 * 4;
+  static constexpr int NBARS = 1 + 2 * SLOTS + 1 + 8;
+  static constexpr int SMEM = BARS + NBARS * 8 + 16;
+  static_assert(SMEM <= 232448, "a CTA's shared memory");
+  static constexpr int OCOL = 2 * BN;              // first TMEM column of the outputs; scores before
+  static constexpr int COLS = 512;
+  static constexpr int OW = NQ * 8;                // first of the other warps
+  static constexpr int THREADS = NQ * 256 + 128;
 };
+
+constexpr int kPoly = 0;  // of 16 pairs
+// 2^f on [-1/2, 1/2], the polynomial of degree 4 with the least relative error
+constexpr float kExpC0 = 0.999999261f;
+constexpr float kExpC1 = 0.693121815f;
+constexpr float kExpC2 = 0.240247448f;
+constexpr float kExpC3 = 0.0559178603f;
+constexpr float kExpC4 = 0.00957010191f;
 
 struct PromptArgs {
   void* out;
@@ -54,17 +66,18 @@ struct PromptArgs {
   const int32_t* starts;
   int64_t o_row, o_head, table_row, room, total_q;
   int batch, hkv, group, toks, tiles, d, page_size, num_pages, window, max_q;
-  int box;   // rows of a K / V box
+  int box;      // rows of a K / V box
+  int one_box;  // a V box holds all column blocks of its rows
   float s2;  // scale * log2(e)
 };
 
 // A [tokens][64 columns] block of 128-byte rows read with the columns as the long (N)
-// dimension: 64-column blocks `block` bytes apart, groups of 8 tokens 1024 apart.
-__device__ __forceinline__ uint64_t umma_smem_desc_mn(uint32_t saddr, uint32_t block) {
+// dimension: 64-column blocks `block` bytes apart, groups of 8 tokens `group` apart.
+__device__ __forceinline__ uint64_t umma_smem_desc_mn(uint32_t saddr, uint32_t block, uint32_t group) {
   uint64_t d = 0;
   d |= static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4);
   d |= static_cast<uint64_t>(block >> 4) << 16;
-  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(group >> 4) << 32;
   d |= static_cast<uint64_t>(1) << 46;
   d |= static_cast<uint64_t>(2) << 61;
   return d;
@@ -100,16 +113,27 @@ __device__ __forceinline__ void tmem_ld32(uint32_t t, uint32_t* r) {
         "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(t));
 }
-__device__ __forceinline__ void tmem_st32(uint32_t t, const uint32_t* r) {
+__device__ __forceinline__ void tmem_st16(uint32_t t, const uint32_t* r) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,"
-      "%31};" ::"r"(r[0]),
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
       "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
-      "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
-      "r"(r[31]), "r"(t)
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(t)
       : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t t, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(t)
+               : "memory");
+}
+template <int N>
+__device__ __forceinline__ void tmem_load(uint32_t t, uint32_t* r) {  // without the wait
+  if constexpr (N == 32) tmem_ld32(t, r);
+  else tmem_ld16_async(t, r);
+}
+template <int N>
+__device__ __forceinline__ void tmem_store(uint32_t t, const uint32_t* r) {
+  if constexpr (N == 16) tmem_st16(t, r);
+  else tmem_st8(t, r);
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -124,28 +148,127 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, i
       : "memory");
 }
 
+// ---- pairs of 32-bit values in one instruction --------------------------------------------
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// The larger of two, of three, NaN if one is.
+__device__ __forceinline__ float fmaxf_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 2^x of a pair, x in [-125, 127], on the FMA units: x = n + f with n whole and f in
+// [-1/2, 1/2] (adding 1.5 * 2^23 leaves n in the low mantissa bits), 2^f by the polynomial
+// of degree 4 that is closest in relative error (Remez exchange; 4e-6 at most), n added to
+// its exponent. Smaller x give 2^-125.
+__device__ __forceinline__ uint64_t exp2_poly2(uint64_t x) {
+  float a, b;
+  unpair(x, a, b);
+  x = pair(fmaxf(a, -125.f), fmaxf(b, -125.f));
+  const uint64_t magic = pair(12582912.f, 12582912.f), unmagic = pair(-12582912.f, -12582912.f);
+  const uint64_t r = add2(x, magic);
+  const uint64_t n = add2(r, unmagic);
+  const uint64_t f = fma2(n, pair(-1.f, -1.f), x);
+  uint64_t y = fma2(pair(kExpC4, kExpC4), f, pair(kExpC3, kExpC3));
+  y = fma2(y, f, pair(kExpC2, kExpC2));
+  y = fma2(y, f, pair(kExpC1, kExpC1));
+  y = fma2(y, f, pair(kExpC0, kExpC0));
+  uint32_t ylo, yhi, rlo, rhi;
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(ylo), "=r"(yhi) : "l"(y));
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(rlo), "=r"(rhi) : "l"(r));
+  ylo += rlo << 23;
+  yhi += rhi << 23;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "r"(ylo), "r"(yhi));
+  return y;
+}
+
+// The weights 2^(s * s2 - z) of N scores, packed to 16 bits, their sum added to `sum`.
+// POLY of every 16 pairs take the polynomial: the special-function units alone would need
+// nearly as long as the products.
+template <int DT, int N, int POLY>
+__device__ __forceinline__ void weights(const float* s, float s2, float z, uint32_t* p, uint64_t* sum) {
+  const uint64_t k = pair(s2, s2), nz = pair(-z, -z);
+#pragma unroll
+  for (int c = 0; c < N / 2; ++c) {
+    uint64_t x = fma2(pair(s[2 * c], s[2 * c + 1]), k, nz);
+    float a, b;
+    if (POLY > 0 && (c * POLY) % 16 + POLY >= 16) {
+      x = exp2_poly2(x);
+      unpair(x, a, b);
+    } else {
+      unpair(x, a, b);
+      a = exp2_fast(a);
+      b = exp2_fast(b);
+      x = pair(a, b);
+    }
+    sum[c & 1] = add2(sum[c & 1], x);
+    // rounded to the cache's type for the product, the sum is not: a relative 2^-9
+    // (2^-12) of each weight, below the rounding of the output
+    p[c] = pack16<DT>(a, b);
+  }
+}
+
+__device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, int c4,
+                                            uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
+      "[%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
+// The two warps that share a row quadrant. Both come here once a tile whatever happened to
+// their waits, so neither waits for a warp that has left.
+__device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+
 template <int DP, int DT>
 __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
     paged_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                         const __grid_constant__ CUtensorMap vmap, const __grid_constant__ PromptArgs a) {
   using C = PShape<DP>;
-  constexpr int NQ = C::NQ, BN = C::BN, NB = C::NB, KS = C::KS, VS = C::VS;
-  extern __shared__ uint8_t raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  constexpr int NQ = C::NQ, BN = C::BN, NB = C::NB, SLOTS = C::SLOTS, QC = C::QC, OW = C::OW;
+  extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* sq = smem;
-  uint8_t* sk = sq + NQ * C::QB;
-  uint8_t* sv = sk + KS * C::KB;
+  uint8_t* ring = sq + NQ * C::QB;  // K(0), V(0), K(1), V(1), ... in turn
+  float* xch = reinterpret_cast<float*>(smem + C::XCH);
   uint64_t* qfull = reinterpret_cast<uint64_t*>(smem + C::BARS);
-  uint64_t* kfull = qfull + 1;
-  uint64_t* kempty = kfull + KS;
-  uint64_t* vfull = kempty + KS;
-  uint64_t* vempty = vfull + VS;
-  uint64_t* vfix = vempty + VS;
+  uint64_t* full = qfull + 1;
+  uint64_t* empty = full + SLOTS;
+  uint64_t* vfix = empty + SLOTS;
   uint64_t* sfull = vfix + 1;   // [2] scores in a buffer
-  uint64_t* pready = sfull + 2; // [2] weights in a buffer
-  uint64_t* odone = pready + 2; // [2] a query tile's product with the values is done
+  uint64_t* pready = sfull + 2; // [2][2] the first, the second half of a buffer's weights
+  uint64_t* odone = pready + 4; // [2] a query tile's product with the values is done
   uint32_t* slot = reinterpret_cast<uint32_t*>(odone + 2);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  static_assert(2 + 2 * SLOTS + 8 == C::NBARS, "the barriers above");
+  // the same in all lanes, and known to be: the products' operands then live in uniform registers
+  const int warp = __shfl_sync(0xFFFFFFFFu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   pdl_wait();
 
   // ---- what this CTA works on: heads fastest, the longest (latest) tiles first -----------
@@ -177,15 +300,19 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
     return;
   }
 
+  if (smem_u32(smem) & 1023) {  // the swizzled tiles need it; the driver places a CTA's memory so
+    if (threadIdx.x == 0) atomicOr(&g_device_error, kErrIndex);
+    return;
+  }
   if (threadIdx.x == 0) {
     mbar_init(qfull, 1);
-    for (int i = 0; i < KS; ++i) mbar_init(kfull + i, 1), mbar_init(kempty + i, 1);
-    for (int i = 0; i < VS; ++i) mbar_init(vfull + i, 1), mbar_init(vempty + i, 1);
+    for (int i = 0; i < SLOTS; ++i) mbar_init(full + i, 1), mbar_init(empty + i, 1);
     mbar_init(vfix, 1);
-    for (int i = 0; i < 2; ++i) mbar_init(sfull + i, 1), mbar_init(pready + i, 4), mbar_init(odone + i, 1);
+    for (int i = 0; i < 2; ++i) mbar_init(sfull + i, 1), mbar_init(odone + i, 1);
+    for (int i = 0; i < 4; ++i) mbar_init(pready + i, 8);
     fence_mbar_init();
   }
-  if (warp == NQ * 4 + 1) {
+  if (warp == OW + 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)),
                  "r"(static_cast<uint32_t>(C::COLS))
                  : "memory");
@@ -194,142 +321,201 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tmem = *slot;
+  const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, *slot, 0);
   // not earlier: a dependent kernel that takes its tensor memory before it waits for this
   // grid must find that all of this grid's CTAs have theirs
   pdl_trigger();
 
-  if (warp == NQ * 4) {
-    // ---- loads -------------------------------------------------------------------------
-    bool ok = true;
-    int kt = 0, vt = 0;  // tiles asked for
-    if (lane == 0) mbar_arrive_expect_tx(qfull, NQ * NB * a.toks * a.group * 128);
-    __syncwarp();
-    if (lane < NQ * NB) {
-      const int i = lane / NB, c = lane % NB;
-      tma_load_4d(sq + i * C::QB + c * (128 * 128), &qmap, c * 64, 0, head, q0 + t0 + i * a.toks, qfull);
-    }
-    const int32_t* row = a.tables + b * a.table_row;
-    const int boxes = NB * (BN / a.box);
-    auto load = [&](uint8_t* dst, const CUtensorMap* map, int j, uint64_t* bar) {
-      if (lane == 0) mbar_arrive_expect_tx(bar, C::KB);
+  // the softmax warps hold half a row's scores in registers: they take what the others
+  // leave (4 x 104 + 64 = 5 x 96, the launch's share)
+  if (warp >= OW) {
+    if (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if (warp == OW) {
+      // ---- loads -----------------------------------------------------------------------
+      bool ok = true;
+      int asked = 0;  // tiles of the ring
+      if (lane == 0) mbar_arrive_expect_tx(qfull, NQ * NB * a.toks * a.group * 128);
       __syncwarp();
-      for (int x = lane; x < boxes; x += 32) {
-        const int c = x % NB, r = x / NB * a.box, tok = j * BN + r;
-        int page = a.num_pages;  // outside the map: the box is filled with zeros
-        if (tok < len && tok + a.box > lo) {
-          const int p = row[tok / a.page_size];
-          if (p >= 0 && p < a.num_pages) page = p;
-          else atomicOr(&g_device_error, kErrIndex);
-        }
-        tma_load_4d(dst + c * (BN * 128) + r * 128, map, c * 64, tok % a.page_size, head, page, bar);
+      if (lane < NQ * NB) {
+        const int i = lane / NB, c = lane % NB;
+        tma_load_4d(sq + i * C::QB + c * (128 * 128), &qmap, c * 64, 0, head, q0 + t0 + i * a.toks, qfull);
       }
-    };
-    for (int t = 0; t < nt && ok; ++t) {
-      const int ks = t % KS, vs = t % VS, j = j0 + t;
-      ok = mbar_wait(kempty + ks, (t / KS & 1) ^ 1);
-      if (!__all_sync(0xFFFFFFFFu, ok)) break;
-      load(sk + ks * C::KB, &kmap, j, kfull + ks);
-      ++kt;
-      ok = mbar_wait(vempty + vs, (t / VS & 1) ^ 1);
-      if (!__all_sync(0xFFFFFFFFu, ok)) break;
-      // tokens past the length that share a box with some before it may hold anything, NaN
-      // too, and a weight of 0 must meet 0: that tile's values are cleared there by hand
-      if ((j + 1) * BN > len && len % a.box) {
-        load(sv + vs * C::KB, &vmap, j, vfix);
-        ok = mbar_wait(vfix, 0);  // at most once: it is the last tile of the sequence
-        if (!__all_sync(0xFFFFFFFFu, ok)) break;
-        const int r0 = len - j * BN, rows = (r0 + a.box - 1) / a.box * a.box - r0;
-        for (int x = lane; x < rows * NB * 8; x += 32)
-          *reinterpret_cast<uint4*>(sv + vs * C::KB + x / 8 % NB * (BN * 128) + (r0 + x / 8 / NB) * 128 + x % 8 * 16) =
-              make_uint4(0, 0, 0, 0);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      const int32_t* row = a.tables + b * a.table_row;
+      // a lane's box of a K tile: column block lane % NB of rows rb * box ..., and that box's page
+      const int kboxes = NB * (BN / a.box), rb = lane / NB;
+      auto page_of = [&](int j) {
+        const int tok = j * BN + rb * a.box;
+        if (lane >= kboxes || tok >= len || tok + a.box <= lo) return a.num_pages;  // the box is filled with zeros
+        const int p = row[tok / a.page_size];
+        if (p >= 0 && p < a.num_pages) return p;
+        atomicOr(&g_device_error, kErrIndex);
+        return a.num_pages;
+      };
+      auto load_v = [&](uint8_t* dst, int j, int page, uint64_t* bar) {
+        if (lane == 0) mbar_arrive_expect_tx(bar, C::KB);
         __syncwarp();
-        if (lane == 0) mbar_arrive(vfull + vs);
-      } else {
-        load(sv + vs * C::KB, &vmap, j, vfull + vs);
-      }
-      ++vt;
-    }
-    if (!__all_sync(0xFFFFFFFFu, ok)) {  // a wait ran out: the copies still in flight
-      mbar_wait(qfull, 0);
-      for (int t = max(0, kt - KS); t < kt; ++t) mbar_wait(kfull + t % KS, t / KS & 1);
-      for (int t = max(0, vt - VS); t < vt; ++t) mbar_wait(vfull + t % VS, t / VS & 1);
-    }
-  } else if (warp == NQ * 4 + 1) {
-    // ---- products ----------------------------------------------------------------------
-    if (lane == 0) {
-      constexpr uint32_t id_qk = idesc16<DT, BN, false>(), id_pv = idesc16<DT, DP, true>();
-      auto qk = [&](int i, int buf, int ks) {  // scores of query tile i
-        const uint32_t qa = smem_u32(sq + i * C::QB), ka = smem_u32(sk + ks * C::KB);
-#pragma unroll
-        for (int c = 0; c < NB; ++c) {
-          const uint64_t qd = umma_smem_desc(qa + c * (128 * 128)), kd = umma_smem_desc(ka + c * (BN * 128));
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_ss(tmem + buf * C::SCOL, qd + 2 * k, kd + 2 * k, id_qk, c > 0 || k > 0);
+        if (a.one_box) {
+          const int pg = __shfl_sync(0xFFFFFFFFu, page, (lane * NB) & 31);
+          if (lane < BN / a.box) {
+            const int tok = j * BN + lane * a.box;
+            tma_load_5d(dst + lane * (a.box * NB * 128), &vmap, 0, tok % a.page_size, 0, head, pg, bar);
+          }
+        } else if (lane < kboxes) {
+          const int tok = j * BN + rb * a.box, c = lane % NB;
+          tma_load_5d(dst + c * (BN * 128) + rb * a.box * 128, &vmap, c * 64, tok % a.page_size, 0, head, page, bar);
         }
-        umma_commit(sfull + buf);
       };
-      auto pv = [&](int i, int buf, int vs, bool acc) {
-        const uint64_t vd = umma_smem_desc_mn(smem_u32(sv + vs * C::KB), BN * 128);
+      int page = page_of(j0);
+      for (int t = 0; t < nt; ++t) {
+        const int j = j0 + t, next = t + 1 < nt ? page_of(j + 1) : 0;
+        int sl = asked % SLOTS;
+        ok = mbar_wait(empty + sl, (asked / SLOTS & 1) ^ 1);
+        if (!__all_sync(0xFFFFFFFFu, ok)) break;
+        if (lane == 0) mbar_arrive_expect_tx(full + sl, C::KB);
+        __syncwarp();
+        if (lane < kboxes) {
+          const int c = lane % NB;
+          tma_load_4d(ring + sl * C::KB + c * (BN * 128) + rb * a.box * 128, &kmap, c * 64,
+                      (j * BN + rb * a.box) % a.page_size, head, page, full + sl);
+        }
+        ++asked;
+        sl = asked % SLOTS;
+        ok = mbar_wait(empty + sl, (asked / SLOTS & 1) ^ 1);
+        if (!__all_sync(0xFFFFFFFFu, ok)) break;
+        uint8_t* dst = ring + sl * C::KB;
+        // tokens past the length that share a box with some before it may hold anything, NaN
+        // too, and a weight of 0 must meet 0: that tile's values are cleared there by hand
+        if ((j + 1) * BN > len && len % a.box) {
+          load_v(dst, j, page, vfix);
+          ok = mbar_wait(vfix, 0);  // at most once: it is the last tile of the sequence
+          if (!__all_sync(0xFFFFFFFFu, ok)) break;
+          const int r0 = len - j * BN, rows = (r0 + a.box - 1) / a.box * a.box - r0;
+          for (int x = lane; x < rows * NB * 8; x += 32) {
+            const int c = x / 8 % NB, r = r0 + x / 8 / NB;
+            const int at = a.one_box ? (r / a.box * NB + c) * (a.box * 128) + r % a.box * 128 : c * (BN * 128) + r * 128;
+            *reinterpret_cast<uint4*>(dst + at + x % 8 * 16) = make_uint4(0, 0, 0, 0);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(full + sl);
+        } else {
+          load_v(dst, j, page, full + sl);
+        }
+        ++asked;
+        page = next;
+      }
+      if (!__all_sync(0xFFFFFFFFu, ok)) {  // a wait ran out: the copies still in flight
+        mbar_wait(qfull, 0);
+        for (int x = max(0, asked - SLOTS); x < asked; ++x) mbar_wait(full + x % SLOTS, x / SLOTS & 1);
+      }
+    } else if (warp == OW + 1) {
+      // ---- products --------------------------------------------------------------------
+      // the whole warp walks the tiles, one elected lane issues
+      constexpr uint32_t id_qk = idesc16<DT, BN, false>(), id_pv = idesc16<DT, DP, true>();
+      // a V tile: boxes of all column blocks one after the other, or one block after the other
+      const uint32_t vblock = a.one_box ? a.box * 128 : BN * 128;
+      const uint32_t vgroup = a.one_box && a.box == 8 ? NB * 1024 : 1024;
+      const uint32_t vlog = __ffs(a.box) - 1;
+      const uint32_t vbox = a.one_box ? a.box * NB * 128 : a.box * 128;  // from box to box
+      const uint64_t q_desc = umma_smem_desc(smem_u32(sq)), k_desc = umma_smem_desc(smem_u32(ring));
+      const uint64_t v_desc = umma_smem_desc_mn(smem_u32(ring), vblock, vgroup);
+      uint32_t v_at[BN / 16];  // of each 16 tokens of a tile, in units of 16 bytes
 #pragma unroll
-        for (int k = 0; k < BN / 16; ++k)
-          umma_ts(tmem + C::OCOL + i * DP, tmem + buf * C::SCOL + 8 * k, vd + k * (2048 >> 4), id_pv, acc || k > 0);
-        umma_commit(odone + i);
+      for (int k = 0; k < BN / 16; ++k)
+        v_at[k] = ((16u * k >> vlog) * vbox + (16u * k & ((1u << vlog) - 1)) * 128) >> 4;
+      auto qk = [&](int i, int buf, int sl) {  // scores of query tile i
+        const uint64_t qd = q_desc + i * (C::QB >> 4), kd = k_desc + static_cast<uint32_t>(sl * (C::KB >> 4));
+        if (elect_one()) {
+#pragma unroll
+          for (int c = 0; c < NB; ++c)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              umma_ss(tmem + buf * BN, qd + (c * (128 * 128 >> 4) + 2 * k), kd + (c * (BN * 128 >> 4) + 2 * k), id_qk,
+                      c > 0 || k > 0);
+          umma_commit(sfull + buf);
+        }
+        __syncwarp();
       };
-      bool ok = mbar_wait(qfull, 0) && mbar_wait(kfull, 0);
-      fence_after();
+      // the output of query tile i takes a value tile; the first half of the weights may be
+      // multiplied while the second is still being made
+      auto pv = [&](int i, int buf, int sl, uint32_t par, bool acc) {
+        const uint64_t vd = v_desc + static_cast<uint32_t>(sl * (C::KB >> 4));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (!mbar_wait(pready + buf * 2 + h, par)) return false;
+          fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int k = h * (BN / 32); k < (h + 1) * (BN / 32); ++k)
+              umma_ts(tmem + C::OCOL + i * DP, tmem + buf * BN + 8 * k, vd + v_at[k], id_pv, acc || k > 0);
+            if (h) umma_commit(odone + i);
+          }
+          __syncwarp();
+        }
+        return true;
+      };
+      int sl = 0;  // the ring's next slot and its parity
+      uint32_t par = 0;
+      auto wait_tile = [&](int& at) {  // the next tile of the ring has arrived
+        at = sl;
+        const bool ok = mbar_wait(full + sl, par);
+        fence_after();
+        if (++sl == SLOTS) sl = 0, par ^= 1;
+        return ok;
+      };
+      auto release = [&](int at) {
+        if (elect_one()) umma_commit(empty + at);
+        __syncwarp();
+      };
+      int ks = 0, vs = 0;
+      bool ok = mbar_wait(qfull, 0) && wait_tile(ks);
       if (ok) {
-        for (int i = 0; i < NQ; ++i) qk(i, i, 0);
-        umma_commit(kempty);
+        for (int i = 0; i < NQ; ++i) qk(i, i, ks);
+        release(ks);
       }
       for (int t = 0; t < nt && ok; ++t) {
-        const int vs = t % VS, kn = (t + 1) % KS;
         const bool more = t + 1 < nt;
+        ok = wait_tile(vs);
+        if (!ok) break;
         if (NQ == 1) {
           if (more) {  // the other score buffer: its weights were read by the last product
-            ok = mbar_wait(kfull + kn, (t + 1) / KS & 1);
+            ok = wait_tile(ks);
             if (!ok) break;
-            fence_after();
-            qk(0, (t + 1) & 1, kn);
-            umma_commit(kempty + kn);
+            qk(0, (t + 1) & 1, ks);
+            release(ks);
           }
-          ok = mbar_wait(vfull + vs, t / VS & 1) && mbar_wait(pready + (t & 1), t >> 1 & 1);
+          ok = pv(0, t & 1, vs, t >> 1 & 1, t > 0);
           if (!ok) break;
-          fence_after();
-          pv(0, t & 1, vs, t > 0);
+          release(vs);
         } else {
-          ok = mbar_wait(vfull + vs, t / VS & 1);
-          for (int i = 0; i < NQ && ok; ++i) {
-            ok = mbar_wait(pready + i, t & 1);
+#pragma unroll
+          for (int i = 0; i < NQ; ++i) {
+            ok = pv(i, i, vs, t & 1, t > 0);
             if (!ok) break;
-            fence_after();
-            pv(i, i, vs, t > 0);
+            if (i == NQ - 1) release(vs);
             if (more) {  // over the weights just read: products run in the order of their issue
-              if (i == 0) {
-                ok = mbar_wait(kfull + kn, (t + 1) / KS & 1);
-                if (!ok) break;
-                fence_after();
-              }
-              qk(i, i, kn);
+              if (i == 0) ok = wait_tile(ks);
+              if (!ok) break;
+              qk(i, i, ks);
             }
           }
           if (!ok) break;
-          if (more) umma_commit(kempty + kn);
+          if (more) release(ks);
         }
-        umma_commit(vempty + vs);
       }
     }
-    __syncwarp();
   } else {
-    // ---- softmax: thread r of a warpgroup has row r of its query tile ---------------------
-    const int i = warp >> 2, r = (warp & 3) * 32 + lane;
+    if (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    // ---- softmax: a thread has half of row r of its query tile ---------------------------
+    const int i = warp >> 3, half = warp >> 2 & 1, r = (warp & 3) * 32 + lane;
     const int tok = t0 + i * a.toks + r / a.group, g = r % a.group;
     const bool live = r < a.toks * a.group && tok < n;
     const int pos = len - n_all + tok;  // this row's position
     const int pos_a = len - n_all + t0 + i * a.toks, pos_b = pos_a + a.toks - 1;  // the tile's first and last
     const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21);
+    const int sync_id = 1 + i * 4 + (warp & 3);
+    float* mine = xch + (i * 2 + half) * 128 + r;
+    const float* other = xch + (i * 2 + (half ^ 1)) * 128 + r;
     // 16-bit floats underflow early: their weights are kept 2^7 larger (the sum too)
     constexpr float kUp = DT == GGUFMM_F16 ? 7.f : 0.f;
     const bool odd_scale = a.s2 <= 0.f;
@@ -338,91 +524,103 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
     bool ok = true;
     for (int t = 0; t < nt; ++t) {
       const int buf = NQ == 1 ? t & 1 : i, par = NQ == 1 ? t >> 1 & 1 : t & 1;
-      ok = mbar_wait(sfull + buf, par);
-      ok = __all_sync(0xFFFFFFFFu, ok);
-      if (!ok) break;
-      fence_after();
-      uint32_t sr[BN];
-      const uint32_t sc = lanes + buf * C::SCOL;
-#pragma unroll
-      for (int c = 0; c < BN; c += 32) tmem_ld32(sc + c, sr + c);
-      tmem_wait_ld();
+      // this thread's columns: QC of each half of the tile
+      const uint32_t sc = lanes + buf * BN;
+      const int jt = (j0 + t) * BN;
+      const bool edge = jt + BN - 1 > pos_a || (a.window > 0 && jt <= pos_b - a.window);
+      uint32_t sr[2][QC];
       float* s = reinterpret_cast<float*>(sr);
-      if (odd_scale) {
+      float top = -INFINITY;
+      ok = ok && mbar_wait(sfull + buf, par);
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      if (ok) {
+        fence_after();
+        tmem_load<QC>(sc + half * QC, sr[0]);
+        tmem_wait_ld();
+        tmem_load<QC>(sc + BN / 2 + half * QC, sr[1]);  // while the first are looked at
+        float mx[4];
 #pragma unroll
-        for (int c = 0; c < BN; ++c) s[c] *= a.s2;
+        for (int h = 0; h < 2; ++h) {
+          if (h) tmem_wait_ld();
+          float* v = s + h * QC;
+          if (odd_scale) {
+#pragma unroll
+            for (int c = 0; c < QC; ++c) v[c] *= a.s2;
+          }
+          if (edge) {
+            const int jb = jt + h * (BN / 2) + half * QC;
+            const int up = pos - jb, dn = a.window > 0 ? pos - a.window - jb : -1;  // visible: dn < c <= up
+#pragma unroll
+            for (int c = 0; c < QC; ++c)
+              if (c > up || c <= dn) v[c] = -INFINITY;
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx[e] = h ? max3(mx[e], v[e], v[4 + e]) : fmaxf_nan(v[e], v[4 + e]);
+#pragma unroll
+          for (int c = 8; c < QC; c += 8)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], v[c + e], v[c + 4 + e]);
+        }
+        top = max3(fmaxf_nan(mx[0], mx[1]), mx[2], mx[3]);
+        *mine = top;  // last read before the other warp's weights of the previous tile were ready
+        fence_before();  // both have read their scores before either's weights take the columns
       }
-      const int jb = (j0 + t) * BN;
-      if (jb + BN - 1 > pos_a || (a.window > 0 && jb <= pos_b - a.window)) {
-        const int up = pos - jb, dn = a.window > 0 ? pos - a.window - jb : -1;  // visible: dn < c <= up
-#pragma unroll
-        for (int c = 0; c < BN; ++c)
-          if (c > up || c <= dn) s[c] = -INFINITY;
-      }
-      float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-      for (int c = 4; c < BN; c += 4)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], s[c + e]);
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * s2;
-      // rescale when the maximum has grown by more than 8 (or is the first)
+      pair_sync(sync_id);
+      if (!ok) continue;
+      fence_after();
+      top = fmaxf_nan(top, *other) * s2;
+      // rescale when the maximum has grown by more than 8 (or is the first; a NaN stays one)
       float f = 1.f;
-      if (top > m + 8.f || (m == -INFINITY && top > m)) {
+      if (!(top <= m + 8.f)) {
         f = exp2_fast(m - top);  // 0 for the first
-        m = top;
+        m = top == INFINITY ? __int_as_float(0x7FFFFFFF) : top;  // inf - inf
         l *= f;
       }
       if (t > 0 && __any_sync(0xFFFFFFFFu, f != 1.f)) {
         ok = mbar_wait(odone + i, (t - 1) & 1);
         ok = __all_sync(0xFFFFFFFFu, ok);
-        if (!ok) break;
+        if (!ok) continue;
         fence_after();
-        const uint32_t oc = lanes + C::OCOL + i * DP;
+        const uint32_t oc = lanes + C::OCOL + i * DP + half * (DP / 2);
 #pragma unroll 1
-        for (int c = 0; c < DP; c += 32) {
-          uint32_t o[32];
-          tmem_ld32(oc + c, o);
-          tmem_wait_ld();
+        for (int c = 0; c < DP / 2; c += 16) {
+          uint32_t o[16];
+          tmem_ld16(oc + c, o);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-          tmem_st32(oc + c, o);
+          for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+          tmem_st16(oc + c, o);
         }
       }
       const float z = (m == -INFINITY ? 0.f : m) - kUp;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      uint64_t sum[2] = {0, 0};
 #pragma unroll
-      for (int h = 0; h < BN; h += 64) {
-        uint32_t p[32];
-#pragma unroll
-        for (int c = 0; c < 64; c += 4) {
-          float e[4];
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            e[x] = exp2_fast(fmaf(s[h + c + x], s2, -z));
-            sum[x] += e[x];
-          }
-          // rounded to the cache's type for the product, the sum is not: a relative 2^-9
-          // (2^-12) of each weight, below the rounding of the output
-          p[c / 2] = pack16<DT>(e[0], e[1]);
-          p[c / 2 + 1] = pack16<DT>(e[2], e[3]);
-        }
-        tmem_st32(sc + h / 2, p);
+      for (int h = 0; h < 2; ++h) {
+        uint32_t p[QC / 2];
+        // a tile with hidden keys needs exact zeros
+        if (edge) weights<DT, QC, 0>(s + h * QC, s2, z, p, sum);
+        else weights<DT, QC, kPoly>(s + h * QC, s2, z, p, sum);
+        tmem_store<QC / 2>(sc + h * (BN / 4) + half * (QC / 2), p);
+        tmem_wait_st();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(pready + buf * 2 + h);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tmem_wait_st();
-      fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(pready + buf);
+      float a0, a1;
+      unpair(add2(sum[0], sum[1]), a0, a1);
+      l += a0 + a1;
     }
     if (ok) ok = mbar_wait(odone + i, (nt - 1) & 1);
     ok = __all_sync(0xFFFFFFFFu, ok);
+    *mine = l;
+    pair_sync(sync_id);
     if (ok) {
       fence_after();
+      l = half ? *other + l : l + *other;
       const float inv = l == 0.f ? 0.f : 1.f / l;
       uint16_t* dst = outp + static_cast<int64_t>(q0 + tok) * a.o_row + g * a.o_head;
       const uint32_t oc = lanes + C::OCOL + i * DP;
 #pragma unroll 1
-      for (int c = 0; c < DP; c += 32) {
+      for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 32) {
         uint32_t o[32];
         tmem_ld32(oc + c, o);
         tmem_wait_ld();
@@ -446,7 +644,7 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
     fence_before();
   }
   __syncthreads();
-  if (warp == NQ * 4 + 1) {
+  if (warp == OW + 1) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
                  "r"(static_cast<uint32_t>(C::COLS))
@@ -454,14 +652,14 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
   }
 }
 
-bool encode4(CUtensorMap* map, int64_t dtype, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
-             const cuuint32_t* box) {
+bool encode(CUtensorMap* map, int64_t dtype, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+            const cuuint32_t* box) {
   PFN_encodeTiled enc = get_encode_fn();
   if (!enc) return false;
-  cuuint32_t estr[4] = {1, 1, 1, 1};
-  return enc(map, dtype == GGUFMM_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
-             const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  return enc(map, dtype == GGUFMM_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+             static_cast<cuuint32_t>(rank), const_cast<void*>(base), dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -503,11 +701,19 @@ cudaError_t launch(const ggufmm_attention_args& p, cudaStream_t st) {
                             static_cast<cuuint64_t>(p.num_pages)};
   const cuuint64_t ks[3] = {static_cast<cuuint64_t>(p.k_slot) * 2, static_cast<cuuint64_t>(p.k_head) * 2,
                             static_cast<cuuint64_t>(p.k_page) * 2};
-  const cuuint64_t vs[3] = {static_cast<cuuint64_t>(p.v_slot) * 2, static_cast<cuuint64_t>(p.v_head) * 2,
+  const cuuint32_t kb[4] = {64, static_cast<cuuint32_t>(a.box), 1, 1};
+  // the values with their 64-column blocks as a dimension of its own, so that one box of
+  // whole rows takes half (a quarter of) the requests: with pages of 16 tokens the loads
+  // are bound by those
+  a.one_box = a.d == DP;
+  const cuuint64_t blocks = a.one_box ? C::NB : 1;
+  const cuuint64_t vd[5] = {a.one_box ? 64 : d, static_cast<cuuint64_t>(p.page_size), blocks,
+                            static_cast<cuuint64_t>(p.kv_heads), static_cast<cuuint64_t>(p.num_pages)};
+  const cuuint64_t vs[4] = {static_cast<cuuint64_t>(p.v_slot) * 2, 128, static_cast<cuuint64_t>(p.v_head) * 2,
                             static_cast<cuuint64_t>(p.v_page) * 2};
-  const cuuint32_t cb[4] = {64, static_cast<cuuint32_t>(a.box), 1, 1};
-  if (!encode4(&qm, p.dtype, p.q, qd, qs, qb) || !encode4(&km, p.dtype, p.k, cd, ks, cb) ||
-      !encode4(&vm, p.dtype, p.v, cd, vs, cb))
+  const cuuint32_t vb[5] = {64, static_cast<cuuint32_t>(a.box), static_cast<cuuint32_t>(blocks), 1, 1};
+  if (!encode(&qm, p.dtype, p.q, 4, qd, qs, qb) || !encode(&km, p.dtype, p.k, 4, cd, ks, kb) ||
+      !encode(&vm, p.dtype, p.v, 5, vd, vs, vb))
     return cudaErrorInvalidValue;
   auto fn = paged_prompt_kernel<DP, DT>;
   int dev = 0;
