@@ -20,7 +20,7 @@
 // last rescaling (the weights then reach at most 2^8, harmless in 32-bit sums).
 //
 // Warps: 8 softmax warps per query tile (two share a row quadrant and halve its columns), one
-// that loads, one that issues the products.
+// that loads queries and values, one that loads keys, one that issues the products.
 #include <algorithm>
 #include <atomic>
 
@@ -61,6 +61,8 @@ constexpr float kExpC4 = 0.00957010191f;
 
 struct PromptArgs {
   void* out;
+  const uint16_t* k;
+  int64_t k_page, k_head, k_slot;
   const int32_t* tables;
   const int32_t* lens;
   const int32_t* starts;
@@ -250,8 +252,7 @@ __device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 6
 
 template <int DP, int DT>
 __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
-    paged_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
-                        const __grid_constant__ CUtensorMap vmap, const __grid_constant__ PromptArgs a) {
+    paged_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ PromptArgs a) {
   using C = PShape<DP>;
   constexpr int NQ = C::NQ, BN = C::BN, NB = C::NB, SLOTS = C::SLOTS, QC = C::QC, OW = C::OW;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -329,64 +330,45 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
   // the softmax warps hold half a row's scores in registers: they take what the others
   // leave (4 x 104 + 64 = 5 x 96, the launch's share)
   if (warp >= OW) {
+    const int32_t* row = a.tables + b * a.table_row;
     if (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp == OW) {
-      // ---- loads -----------------------------------------------------------------------
+      // ---- queries and values, by TMA ----------------------------------------------------
       bool ok = true;
-      int asked = 0;  // tiles of the ring
       if (lane == 0) mbar_arrive_expect_tx(qfull, NQ * NB * a.toks * a.group * 128);
       __syncwarp();
       if (lane < NQ * NB) {
         const int i = lane / NB, c = lane % NB;
         tma_load_4d(sq + i * C::QB + c * (128 * 128), &qmap, c * 64, 0, head, q0 + t0 + i * a.toks, qfull);
       }
-      const int32_t* row = a.tables + b * a.table_row;
-      // a lane's box of a K tile: column block lane % NB of rows rb * box ..., and that box's page
-      const int kboxes = NB * (BN / a.box), rb = lane / NB;
+      // a lane's box of a tile: all column blocks of box rows, or one of them; and its page
+      const int cols = a.one_box ? 1 : NB, boxes = cols * (BN / a.box), rb = lane / cols, cb = lane % cols;
       auto page_of = [&](int j) {
         const int tok = j * BN + rb * a.box;
-        if (lane >= kboxes || tok >= len || tok + a.box <= lo) return a.num_pages;  // the box is filled with zeros
+        if (lane >= boxes || tok >= len || tok + a.box <= lo) return a.num_pages;  // the box is filled with zeros
         const int p = row[tok / a.page_size];
         if (p >= 0 && p < a.num_pages) return p;
         atomicOr(&g_device_error, kErrIndex);
         return a.num_pages;
       };
-      auto load_v = [&](uint8_t* dst, int j, int page, uint64_t* bar) {
+      auto load = [&](uint8_t* dst, int j, int page, uint64_t* bar) {
         if (lane == 0) mbar_arrive_expect_tx(bar, C::KB);
         __syncwarp();
-        if (a.one_box) {
-          const int pg = __shfl_sync(0xFFFFFFFFu, page, (lane * NB) & 31);
-          if (lane < BN / a.box) {
-            const int tok = j * BN + lane * a.box;
-            tma_load_5d(dst + lane * (a.box * NB * 128), &vmap, 0, tok % a.page_size, 0, head, pg, bar);
-          }
-        } else if (lane < kboxes) {
-          const int tok = j * BN + rb * a.box, c = lane % NB;
-          tma_load_5d(dst + c * (BN * 128) + rb * a.box * 128, &vmap, c * 64, tok % a.page_size, 0, head, page, bar);
-        }
+        if (lane < boxes)
+          tma_load_5d(dst + (a.one_box ? rb * (a.box * NB * 128) : cb * (BN * 128) + rb * (a.box * 128)), &vmap, cb * 64,
+                      (j * BN + rb * a.box) % a.page_size, 0, head, page, bar);
       };
-      int page = page_of(j0);
+      int page = page_of(j0), sl = 1, last = -1;  // the values have every other tile of the ring
+      uint32_t par = 1;
       for (int t = 0; t < nt; ++t) {
         const int j = j0 + t, next = t + 1 < nt ? page_of(j + 1) : 0;
-        int sl = asked % SLOTS;
-        ok = mbar_wait(empty + sl, (asked / SLOTS & 1) ^ 1);
-        if (!__all_sync(0xFFFFFFFFu, ok)) break;
-        if (lane == 0) mbar_arrive_expect_tx(full + sl, C::KB);
-        __syncwarp();
-        if (lane < kboxes) {
-          const int c = lane % NB;
-          tma_load_4d(ring + sl * C::KB + c * (BN * 128) + rb * a.box * 128, &kmap, c * 64,
-                      (j * BN + rb * a.box) % a.page_size, head, page, full + sl);
-        }
-        ++asked;
-        sl = asked % SLOTS;
-        ok = mbar_wait(empty + sl, (asked / SLOTS & 1) ^ 1);
+        ok = mbar_wait(empty + sl, par);
         if (!__all_sync(0xFFFFFFFFu, ok)) break;
         uint8_t* dst = ring + sl * C::KB;
         // tokens past the length that share a box with some before it may hold anything, NaN
         // too, and a weight of 0 must meet 0: that tile's values are cleared there by hand
         if ((j + 1) * BN > len && len % a.box) {
-          load_v(dst, j, page, vfix);
+          load(dst, j, page, vfix);
           ok = mbar_wait(vfix, 0);  // at most once: it is the last tile of the sequence
           if (!__all_sync(0xFFFFFFFFu, ok)) break;
           const int r0 = len - j * BN, rows = (r0 + a.box - 1) / a.box * a.box - r0;
@@ -399,14 +381,61 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(full + sl);
         } else {
-          load_v(dst, j, page, full + sl);
+          load(dst, j, page, full + sl);
         }
-        ++asked;
         page = next;
+        last = t;
+        sl += 2;
+        if (sl >= SLOTS) sl -= SLOTS, par ^= 1;
       }
       if (!__all_sync(0xFFFFFFFFu, ok)) {  // a wait ran out: the copies still in flight
         mbar_wait(qfull, 0);
-        for (int x = max(0, asked - SLOTS); x < asked; ++x) mbar_wait(full + x % SLOTS, x / SLOTS & 1);
+        for (int t = max(0, last - SLOTS / 2); t <= last; ++t)
+          mbar_wait(full + (2 * t + 1) % SLOTS, (2 * t + 1) / SLOTS & 1);
+      }
+    } else if (warp >= OW + 2) {
+      // ---- keys, two warps in turn, by 16-byte copies: a TMA box of one 64-column block of a 16-token page is a
+      // request of 2 KB, and the unit takes about 134 clocks for each
+      constexpr int CH = DP / 8, RPI = 32 / CH;  // 16-byte chunks of a row, rows of a warp's copy
+      const int ch = lane % CH, sub = lane / CH;
+      const bool col = ch * 8 < a.d;
+      const uint16_t* base = a.k + head * a.k_head + (col ? ch * 8 : 0);
+      // lane x: where tokens 8 x .. 8 x + 7 of a tile lie, negative where they are not read
+      auto place_of = [&](int j) -> int64_t {
+        const int tok = j * BN + lane * 8;
+        if (lane >= BN / 8 || tok >= len || tok + 8 <= lo) return -1;
+        const int p = row[tok / a.page_size];
+        if (p < 0 || p >= a.num_pages) return -1;  // reads as zeros; the values' warp reports it
+        return p * a.k_page + tok % a.page_size * a.k_slot;
+      };
+      const uint32_t dst0 = smem_u32(ring) + (ch >> 3) * (BN * 128);
+      int64_t place = place_of(j0 + warp - OW - 2);
+      for (int t = warp - OW - 2; t < nt; t += 2) {
+        const int64_t next = t + 2 < nt ? place_of(j0 + t + 2) : 0;
+        const int sl = 2 * t % SLOTS;  // the keys have every other tile of the ring
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait(empty + sl, (2 * t / SLOTS & 1) ^ 1))) break;
+        const uint32_t dst = dst0 + sl * C::KB;
+#pragma unroll 4
+        for (int g = 0; g < BN / 8; ++g) {
+          const int64_t at = __shfl_sync(0xFFFFFFFFu, place, g);
+          const bool in = at >= 0 && col;
+          const uint16_t* src = in ? base + at : a.k;
+          const int64_t step = in ? a.k_slot : 0;
+          const uint32_t bytes = in ? 16 : 0;  // the rest of the 16 is filled with zeros
+#pragma unroll
+          for (int x = 0; x < 8; x += RPI) {
+            const int r = x + sub;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + (g * 8 + r) * 128 +
+                                                                              (((ch & 7) ^ r) << 4)),
+                         "l"(src + r * step), "r"(bytes)
+                         : "memory");
+          }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full + sl);
+        place = next;
       }
     } else if (warp == OW + 1) {
       // ---- products --------------------------------------------------------------------
@@ -672,6 +701,10 @@ cudaError_t launch(const ggufmm_attention_args& p, cudaStream_t st) {
   a.tables = static_cast<const int32_t*>(p.tables);
   a.lens = static_cast<const int32_t*>(p.lens);
   a.starts = static_cast<const int32_t*>(p.q_starts);
+  a.k = static_cast<const uint16_t*>(p.k);
+  a.k_page = p.k_page;
+  a.k_head = p.k_head;
+  a.k_slot = p.k_slot;
   a.o_row = p.o_row;
   a.o_head = p.o_head;
   a.table_row = p.table_row;
@@ -692,16 +725,11 @@ cudaError_t launch(const ggufmm_attention_args& p, cudaStream_t st) {
   while (a.box < C::BN && p.page_size % (2 * a.box) == 0) a.box *= 2;
   const int64_t ctas = static_cast<int64_t>(a.tiles) * a.hkv * a.batch;
   if (ctas > kI32Max) return cudaErrorInvalidConfiguration;
-  CUtensorMap qm, km, vm;
+  CUtensorMap qm, vm;
   const cuuint64_t qd[4] = {d, g, static_cast<cuuint64_t>(p.kv_heads), static_cast<cuuint64_t>(p.total_q)};
   const cuuint64_t qs[3] = {static_cast<cuuint64_t>(p.q_head) * 2, static_cast<cuuint64_t>(p.q_head) * g * 2,
                             static_cast<cuuint64_t>(p.q_row) * 2};
   const cuuint32_t qb[4] = {64, static_cast<cuuint32_t>(g), 1, static_cast<cuuint32_t>(a.toks)};
-  const cuuint64_t cd[4] = {d, static_cast<cuuint64_t>(p.page_size), static_cast<cuuint64_t>(p.kv_heads),
-                            static_cast<cuuint64_t>(p.num_pages)};
-  const cuuint64_t ks[3] = {static_cast<cuuint64_t>(p.k_slot) * 2, static_cast<cuuint64_t>(p.k_head) * 2,
-                            static_cast<cuuint64_t>(p.k_page) * 2};
-  const cuuint32_t kb[4] = {64, static_cast<cuuint32_t>(a.box), 1, 1};
   // the values with their 64-column blocks as a dimension of its own, so that one box of
   // whole rows takes half (a quarter of) the requests: with pages of 16 tokens the loads
   // are bound by those
@@ -712,9 +740,7 @@ cudaError_t launch(const ggufmm_attention_args& p, cudaStream_t st) {
   const cuuint64_t vs[4] = {static_cast<cuuint64_t>(p.v_slot) * 2, 128, static_cast<cuuint64_t>(p.v_head) * 2,
                             static_cast<cuuint64_t>(p.v_page) * 2};
   const cuuint32_t vb[5] = {64, static_cast<cuuint32_t>(a.box), static_cast<cuuint32_t>(blocks), 1, 1};
-  if (!encode(&qm, p.dtype, p.q, 4, qd, qs, qb) || !encode(&km, p.dtype, p.k, 4, cd, ks, kb) ||
-      !encode(&vm, p.dtype, p.v, 5, vd, vs, vb))
-    return cudaErrorInvalidValue;
+  if (!encode(&qm, p.dtype, p.q, 4, qd, qs, qb) || !encode(&vm, p.dtype, p.v, 5, vd, vs, vb)) return cudaErrorInvalidValue;
   auto fn = paged_prompt_kernel<DP, DT>;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -725,7 +751,7 @@ cudaError_t launch(const ggufmm_attention_args& p, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     ready.fetch_or(uint64_t(1) << (dev & 63), std::memory_order_release);
   }
-  return pdl_launch(fn, dim3(static_cast<unsigned>(ctas)), dim3(C::THREADS), C::SMEM, st, qm, km, vm, a);
+  return pdl_launch(fn, dim3(static_cast<unsigned>(ctas)), dim3(C::THREADS), C::SMEM, st, qm, vm, a);
 }
 
 }  // namespace
