@@ -12,15 +12,18 @@
 // Tiles: the G query heads of a kv head and floor(128 / G) consecutive tokens are the 128
 // rows of one query tile (row = token * G + head), so short prompts fill tiles and every key
 // is loaded once for the whole group. A CTA holds two query tiles (one for heads wider than
-// 128): while the softmax warps of one work on its scores, the tensor core multiplies for the
-// other. Keys and values come page by page by TMA into 128-row (64-row) swizzled tiles; q k^T
-// goes to TMEM, thread r of a softmax warpgroup reads row r, writes the weights back over the
-// scores as 16-bit values, and the second product reads them from TMEM. The running output
-// stays in TMEM; it is rescaled only when a row's maximum has grown by more than 2^8 since its
-// last rescaling (the weights then reach at most 2^8, harmless in 32-bit sums).
+// 128) and walks the keys 64 at a time. Keys and values come page by page into swizzled
+// tiles of one ring in shared memory; q k^T goes to TMEM, thread r of a softmax warpgroup
+// reads row r, writes the weights back over the scores as 16-bit values, and the second
+// product reads them from TMEM. Each query tile has two score buffers: the scores of the next
+// keys are made while the softmax warps work on these, which therefore hardly ever wait.
+// (128 keys a tile and one buffer: the softmax, 2370 clocks, and the two products behind it,
+// 1440, took turns, 503 us for 8192 tokens.) The running output stays in TMEM; it is rescaled
+// only when a row's maximum has grown by more than 2^8 since its last rescaling (the weights
+// then reach at most 2^8, harmless in 32-bit sums).
 //
-// Warps: 8 softmax warps per query tile (two share a row quadrant and halve its columns), one
-// that loads queries and values, one that loads keys, one that issues the products.
+// Warps: 4 softmax warps per query tile, one that loads queries and values, one that issues
+// the products, two that load keys.
 #include <algorithm>
 #include <atomic>
 
@@ -35,23 +38,22 @@ namespace {
 template <int DP>
 struct PShape {
   static constexpr int NQ = DP == 256 ? 1 : 2;     // query tiles
-  static constexpr int BN = DP == 256 ? 64 : 128;  // keys of a tile
+  static constexpr int BN = 64;                    // keys of a tile
   static constexpr int NB = DP / 64;               // 128-byte column blocks of a row
-  static constexpr int QC = BN / 4;                // a softmax thread's scores of each half of a tile
   static constexpr int QB = 128 * DP * 2, KB = BN * DP * 2;
-  static constexpr int SLOTS = DP == 64 ? 8 : 5;   // tiles of keys or values in flight
-  static constexpr int XCH = NQ * QB + SLOTS * KB; // [NQ][2][128] exchange between column halves
-  static constexpr int BARS = XCH + NQ * 256 * 4;
-  static constexpr int NBARS = 1 + 2 * SLOTS + 1 + 8;
+  static constexpr int SLOTS = DP == 256 ? 5 : 10; // tiles of keys or values in flight
+  static constexpr int BARS = NQ * QB + SLOTS * KB;
+  static constexpr int NBARS = 1 + 2 * SLOTS + 1 + 7 * NQ;
   static constexpr int SMEM = BARS + NBARS * 8 + 16;
   static_assert(SMEM <= 232448, "a CTA's shared memory");
-  static constexpr int OCOL = 2 * BN;              // first TMEM column of the outputs; scores before
+  static constexpr int OCOL = NQ * 2 * BN;         // first TMEM column of the outputs; scores before
   static constexpr int COLS = 512;
-  static constexpr int OW = NQ * 8;                // first of the other warps
-  static constexpr int THREADS = NQ * 256 + 128;
+  static_assert(OCOL + NQ * DP <= COLS, "tensor memory");
+  static constexpr int OW = NQ * 4;                // first of the other warps
+  static constexpr int THREADS = NQ * 128 + 128;
 };
 
-constexpr int kPoly = 0;  // of 16 pairs
+constexpr int kPoly = 4;  // of 16 pairs
 // 2^f on [-1/2, 1/2], the polynomial of degree 4 with the least relative error
 constexpr float kExpC0 = 0.999999261f;
 constexpr float kExpC1 = 0.693121815f;
@@ -122,21 +124,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t t, const uint32_t* r) {
       "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(t)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st8(uint32_t t, const uint32_t* r) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]),
-               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(t)
-               : "memory");
-}
-template <int N>
-__device__ __forceinline__ void tmem_load(uint32_t t, uint32_t* r) {  // without the wait
-  if constexpr (N == 32) tmem_ld32(t, r);
-  else tmem_ld16_async(t, r);
-}
-template <int N>
-__device__ __forceinline__ void tmem_store(uint32_t t, const uint32_t* r) {
-  if constexpr (N == 16) tmem_st16(t, r);
-  else tmem_st8(t, r);
-}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -206,29 +193,53 @@ __device__ __forceinline__ uint64_t exp2_poly2(uint64_t x) {
   return y;
 }
 
+__device__ __forceinline__ float exp2_ordered(float x) {
+  float y;
+  asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <int DT>
+__device__ __forceinline__ uint32_t pack16_ordered(float lo, float hi) {
+  uint32_t r;
+  if (DT == GGUFMM_F16)
+    asm volatile("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm volatile("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
 // The weights 2^(s * s2 - z) of N scores, packed to 16 bits, their sum added to `sum`.
 // POLY of every 16 pairs take the polynomial: the special-function units alone would need
 // nearly as long as the products.
 template <int DT, int N, int POLY>
 __device__ __forceinline__ void weights(const float* s, float s2, float z, uint32_t* p, uint64_t* sum) {
   const uint64_t k = pair(s2, s2), nz = pair(-z, -z);
+  // in the order in which a warp should issue it: the exponentials of a pair, then the sum and
+  // the rounding of the pair LAG before it, whose exponentials are through by then
+  constexpr int LAG = N / 2 < 4 ? N / 2 : 4;
+  uint64_t e[N / 2];
 #pragma unroll
-  for (int c = 0; c < N / 2; ++c) {
-    uint64_t x = fma2(pair(s[2 * c], s[2 * c + 1]), k, nz);
-    float a, b;
-    if (POLY > 0 && (c * POLY) % 16 + POLY >= 16) {
-      x = exp2_poly2(x);
-      unpair(x, a, b);
-    } else {
-      unpair(x, a, b);
-      a = exp2_fast(a);
-      b = exp2_fast(b);
-      x = pair(a, b);
+  for (int c = 0; c < N / 2 + LAG; ++c) {
+    if (c < N / 2) {
+      uint64_t x = fma2(pair(s[2 * c], s[2 * c + 1]), k, nz);
+      if (POLY > 0 && (c * POLY) % 16 + POLY >= 16) {
+        e[c] = exp2_poly2(x);
+      } else {
+        float a, b;
+        unpair(x, a, b);
+        a = exp2_ordered(a);
+        b = exp2_ordered(b);
+        e[c] = pair(a, b);
+      }
     }
-    sum[c & 1] = add2(sum[c & 1], x);
-    // rounded to the cache's type for the product, the sum is not: a relative 2^-9
-    // (2^-12) of each weight, below the rounding of the output
-    p[c] = pack16<DT>(a, b);
+    if (c >= LAG) {
+      float a, b;
+      sum[c & 1] = add2(sum[c & 1], e[c - LAG]);
+      unpair(e[c - LAG], a, b);
+      // rounded to the cache's type for the product, the sum is not: a relative 2^-9
+      // (2^-12) of each weight, below the rounding of the output
+      p[c - LAG] = pack16_ordered<DT>(a, b);
+    }
   }
 }
 
@@ -246,28 +257,23 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
-// The two warps that share a row quadrant. Both come here once a tile whatever happened to
-// their waits, so neither waits for a warp that has left.
-__device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
-
 template <int DP, int DT>
 __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
     paged_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ PromptArgs a) {
   using C = PShape<DP>;
-  constexpr int NQ = C::NQ, BN = C::BN, NB = C::NB, SLOTS = C::SLOTS, QC = C::QC, OW = C::OW;
+  constexpr int NQ = C::NQ, BN = C::BN, NB = C::NB, SLOTS = C::SLOTS, OW = C::OW;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* sq = smem;
   uint8_t* ring = sq + NQ * C::QB;  // K(0), V(0), K(1), V(1), ... in turn
-  float* xch = reinterpret_cast<float*>(smem + C::XCH);
   uint64_t* qfull = reinterpret_cast<uint64_t*>(smem + C::BARS);
   uint64_t* full = qfull + 1;
   uint64_t* empty = full + SLOTS;
   uint64_t* vfix = empty + SLOTS;
-  uint64_t* sfull = vfix + 1;   // [2] scores in a buffer
-  uint64_t* pready = sfull + 2; // [2][2] the first, the second half of a buffer's weights
-  uint64_t* odone = pready + 4; // [2] a query tile's product with the values is done
-  uint32_t* slot = reinterpret_cast<uint32_t*>(odone + 2);
-  static_assert(2 + 2 * SLOTS + 8 == C::NBARS, "the barriers above");
+  uint64_t* sfull = vfix + 1;         // [NQ][2] scores in a buffer
+  uint64_t* odone = sfull + 2 * NQ;   // [NQ] a query tile's product with the values is done
+  uint64_t* pready = odone + NQ;      // [NQ][2][2] half of the weights in a buffer
+  uint32_t* slot = reinterpret_cast<uint32_t*>(pready + 4 * NQ);
+  static_assert(2 + 2 * SLOTS + 7 * NQ == C::NBARS, "the barriers above");
   // the same in all lanes, and known to be: the products' operands then live in uniform registers
   const int warp = __shfl_sync(0xFFFFFFFFu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   pdl_wait();
@@ -309,8 +315,9 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
     mbar_init(qfull, 1);
     for (int i = 0; i < SLOTS; ++i) mbar_init(full + i, 1), mbar_init(empty + i, 1);
     mbar_init(vfix, 1);
-    for (int i = 0; i < 2; ++i) mbar_init(sfull + i, 1), mbar_init(odone + i, 1);
-    for (int i = 0; i < 4; ++i) mbar_init(pready + i, 8);
+    for (int i = 0; i < 2 * NQ; ++i) mbar_init(sfull + i, 1);
+    for (int i = 0; i < NQ; ++i) mbar_init(odone + i, 1);
+    for (int i = 0; i < 4 * NQ; ++i) mbar_init(pready + i, 4);
     fence_mbar_init();
   }
   if (warp == OW + 1) {
@@ -327,11 +334,8 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
   // grid must find that all of this grid's CTAs have theirs
   pdl_trigger();
 
-  // the softmax warps hold half a row's scores in registers: they take what the others
-  // leave (4 x 104 + 64 = 5 x 96, the launch's share)
   if (warp >= OW) {
     const int32_t* row = a.tables + b * a.table_row;
-    if (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp == OW) {
       // ---- queries and values, by TMA ----------------------------------------------------
       bool ok = true;
@@ -459,9 +463,9 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
           for (int c = 0; c < NB; ++c)
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              umma_ss(tmem + buf * BN, qd + (c * (128 * 128 >> 4) + 2 * k), kd + (c * (BN * 128 >> 4) + 2 * k), id_qk,
-                      c > 0 || k > 0);
-          umma_commit(sfull + buf);
+              umma_ss(tmem + (i * 2 + buf) * BN, qd + (c * (128 * 128 >> 4) + 2 * k), kd + (c * (BN * 128 >> 4) + 2 * k),
+                      id_qk, c > 0 || k > 0);
+          umma_commit(sfull + i * 2 + buf);
         }
         __syncwarp();
       };
@@ -471,12 +475,12 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
         const uint64_t vd = v_desc + static_cast<uint32_t>(sl * (C::KB >> 4));
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          if (!mbar_wait(pready + buf * 2 + h, par)) return false;
+          if (!mbar_wait(pready + (i * 2 + buf) * 2 + h, par)) return false;
           fence_after();
           if (elect_one()) {
 #pragma unroll
             for (int k = h * (BN / 32); k < (h + 1) * (BN / 32); ++k)
-              umma_ts(tmem + C::OCOL + i * DP, tmem + buf * BN + 8 * k, vd + v_at[k], id_pv, acc || k > 0);
+              umma_ts(tmem + C::OCOL + i * DP, tmem + (i * 2 + buf) * BN + 8 * k, vd + v_at[k], id_pv, acc || k > 0);
             if (h) umma_commit(odone + i);
           }
           __syncwarp();
@@ -499,52 +503,33 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
       int ks = 0, vs = 0;
       bool ok = mbar_wait(qfull, 0) && wait_tile(ks);
       if (ok) {
-        for (int i = 0; i < NQ; ++i) qk(i, i, ks);
+        for (int i = 0; i < NQ; ++i) qk(i, 0, ks);
         release(ks);
       }
       for (int t = 0; t < nt && ok; ++t) {
-        const bool more = t + 1 < nt;
-        ok = wait_tile(vs);
-        if (!ok) break;
-        if (NQ == 1) {
-          if (more) {  // the other score buffer: its weights were read by the last product
-            ok = wait_tile(ks);
-            if (!ok) break;
-            qk(0, (t + 1) & 1, ks);
-            release(ks);
-          }
-          ok = pv(0, t & 1, vs, t >> 1 & 1, t > 0);
+        ok = wait_tile(vs);  // tile 2 t + 1 of the ring
+        if (t + 1 < nt && ok) {
+          // into the other buffers: their weights went into products issued before, and
+          // products run in the order of their issue
+          ok = wait_tile(ks);
           if (!ok) break;
-          release(vs);
-        } else {
 #pragma unroll
-          for (int i = 0; i < NQ; ++i) {
-            ok = pv(i, i, vs, t & 1, t > 0);
-            if (!ok) break;
-            if (i == NQ - 1) release(vs);
-            if (more) {  // over the weights just read: products run in the order of their issue
-              if (i == 0) ok = wait_tile(ks);
-              if (!ok) break;
-              qk(i, i, ks);
-            }
-          }
-          if (!ok) break;
-          if (more) release(ks);
+          for (int i = 0; i < NQ; ++i) qk(i, (t + 1) & 1, ks);
+          release(ks);
         }
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) ok = ok && pv(i, t & 1, vs, t >> 1 & 1, t > 0);
+        if (ok) release(vs);
       }
     }
   } else {
-    if (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
-    // ---- softmax: a thread has half of row r of its query tile ---------------------------
-    const int i = warp >> 3, half = warp >> 2 & 1, r = (warp & 3) * 32 + lane;
+    // ---- softmax: thread r of a warpgroup has row r of its query tile ---------------------
+    const int i = warp >> 2, r = (warp & 3) * 32 + lane;
     const int tok = t0 + i * a.toks + r / a.group, g = r % a.group;
     const bool live = r < a.toks * a.group && tok < n;
     const int pos = len - n_all + tok;  // this row's position
     const int pos_a = len - n_all + t0 + i * a.toks, pos_b = pos_a + a.toks - 1;  // the tile's first and last
     const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21);
-    const int sync_id = 1 + i * 4 + (warp & 3);
-    float* mine = xch + (i * 2 + half) * 128 + r;
-    const float* other = xch + (i * 2 + (half ^ 1)) * 128 + r;
     // 16-bit floats underflow early: their weights are kept 2^7 larger (the sum too)
     constexpr float kUp = DT == GGUFMM_F16 ? 7.f : 0.f;
     const bool odd_scale = a.s2 <= 0.f;
@@ -552,52 +537,40 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int t = 0; t < nt; ++t) {
-      const int buf = NQ == 1 ? t & 1 : i, par = NQ == 1 ? t >> 1 & 1 : t & 1;
-      // this thread's columns: QC of each half of the tile
-      const uint32_t sc = lanes + buf * BN;
-      const int jt = (j0 + t) * BN;
-      const bool edge = jt + BN - 1 > pos_a || (a.window > 0 && jt <= pos_b - a.window);
-      uint32_t sr[2][QC];
-      float* s = reinterpret_cast<float*>(sr);
-      float top = -INFINITY;
-      ok = ok && mbar_wait(sfull + buf, par);
+      const int buf = t & 1, par = t >> 1 & 1;
+      ok = mbar_wait(sfull + i * 2 + buf, par);
       ok = __all_sync(0xFFFFFFFFu, ok);
-      if (ok) {
-        fence_after();
-        tmem_load<QC>(sc + half * QC, sr[0]);
-        tmem_wait_ld();
-        tmem_load<QC>(sc + BN / 2 + half * QC, sr[1]);  // while the first are looked at
-        float mx[4];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (h) tmem_wait_ld();
-          float* v = s + h * QC;
-          if (odd_scale) {
-#pragma unroll
-            for (int c = 0; c < QC; ++c) v[c] *= a.s2;
-          }
-          if (edge) {
-            const int jb = jt + h * (BN / 2) + half * QC;
-            const int up = pos - jb, dn = a.window > 0 ? pos - a.window - jb : -1;  // visible: dn < c <= up
-#pragma unroll
-            for (int c = 0; c < QC; ++c)
-              if (c > up || c <= dn) v[c] = -INFINITY;
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) mx[e] = h ? max3(mx[e], v[e], v[4 + e]) : fmaxf_nan(v[e], v[4 + e]);
-#pragma unroll
-          for (int c = 8; c < QC; c += 8)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], v[c + e], v[c + 4 + e]);
-        }
-        top = max3(fmaxf_nan(mx[0], mx[1]), mx[2], mx[3]);
-        *mine = top;  // last read before the other warp's weights of the previous tile were ready
-        fence_before();  // both have read their scores before either's weights take the columns
-      }
-      pair_sync(sync_id);
-      if (!ok) continue;
+      if (!ok) break;
       fence_after();
-      top = fmaxf_nan(top, *other) * s2;
+      const uint32_t sc = lanes + (i * 2 + buf) * BN;
+      uint32_t sr[BN];
+#pragma unroll
+      for (int c = 0; c < BN; c += 32) tmem_ld32(sc + c, sr + c);
+      tmem_wait_ld();
+      float* s = reinterpret_cast<float*>(sr);
+      if (odd_scale) {
+#pragma unroll
+        for (int c = 0; c < BN; ++c) s[c] *= a.s2;
+      }
+      const int jb = (j0 + t) * BN;
+      const bool edge = jb + BN - 1 > pos_a || (a.window > 0 && jb <= pos_b - a.window);
+      if (edge) {
+        const int up = pos - jb, dn = a.window > 0 ? pos - a.window - jb : -1;  // visible: dn < c <= up
+#pragma unroll
+        for (int c = 0; c < BN; ++c)
+          if (c > up || c <= dn) s[c] = -INFINITY;
+      }
+      float mx[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mx[e] = max3(s[e], s[4 + e], s[8 + e]);
+#pragma unroll
+      for (int c = 12; c + 8 <= BN; c += 8)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[c + e], s[c + 4 + e]);
+      static_assert((BN - 12) % 8 == 4, "the last four");
+      mx[0] = max3(mx[0], s[BN - 4], s[BN - 3]);
+      mx[1] = max3(mx[1], s[BN - 2], s[BN - 1]);
+      const float top = max3(fmaxf_nan(mx[0], mx[1]), mx[2], mx[3]) * s2;
       // rescale when the maximum has grown by more than 8 (or is the first; a NaN stays one)
       float f = 1.f;
       if (!(top <= m + 8.f)) {
@@ -608,48 +581,54 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
       if (t > 0 && __any_sync(0xFFFFFFFFu, f != 1.f)) {
         ok = mbar_wait(odone + i, (t - 1) & 1);
         ok = __all_sync(0xFFFFFFFFu, ok);
-        if (!ok) continue;
+        if (!ok) break;
         fence_after();
-        const uint32_t oc = lanes + C::OCOL + i * DP + half * (DP / 2);
+        const uint32_t oc = lanes + C::OCOL + i * DP;
 #pragma unroll 1
-        for (int c = 0; c < DP / 2; c += 16) {
-          uint32_t o[16];
-          tmem_ld16(oc + c, o);
+        for (int c = 0; c < DP; c += 32) {
+          uint32_t o[32];
+          tmem_ld32(oc + c, o);
+          tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
           tmem_st16(oc + c, o);
+          tmem_st16(oc + c + 16, o + 16);
         }
       }
       const float z = (m == -INFINITY ? 0.f : m) - kUp;
       uint64_t sum[2] = {0, 0};
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t p[QC / 2];
-        // a tile with hidden keys needs exact zeros
-        if (edge) weights<DT, QC, 0>(s + h * QC, s2, z, p, sum);
-        else weights<DT, QC, kPoly>(s + h * QC, s2, z, p, sum);
-        tmem_store<QC / 2>(sc + h * (BN / 4) + half * (QC / 2), p);
+      auto handed = [&](int h) {  // half h of the weights is in tensor memory
         tmem_wait_st();
         fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(pready + buf * 2 + h);
+        if (lane == 0) mbar_arrive(pready + (i * 2 + buf) * 2 + h);
+      };
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t p[BN / 4];
+        const float* v = s + h * (BN / 2);
+        // a tile with hidden keys needs exact zeros
+        if (edge) weights<DT, BN / 4, 0>(v, s2, z, p, sum);
+        else weights<DT, BN / 4, kPoly>(v, s2, z, p, sum);
+        if (h) handed(0);  // its store has had time to finish
+        if (edge) weights<DT, BN / 4, 0>(v + BN / 4, s2, z, p + BN / 8, sum);
+        else weights<DT, BN / 4, kPoly>(v + BN / 4, s2, z, p + BN / 8, sum);
+        tmem_st16(sc + h * (BN / 4), p);
       }
+      handed(1);
       float a0, a1;
       unpair(add2(sum[0], sum[1]), a0, a1);
       l += a0 + a1;
     }
     if (ok) ok = mbar_wait(odone + i, (nt - 1) & 1);
     ok = __all_sync(0xFFFFFFFFu, ok);
-    *mine = l;
-    pair_sync(sync_id);
     if (ok) {
       fence_after();
-      l = half ? *other + l : l + *other;
       const float inv = l == 0.f ? 0.f : 1.f / l;
       uint16_t* dst = outp + static_cast<int64_t>(q0 + tok) * a.o_row + g * a.o_head;
       const uint32_t oc = lanes + C::OCOL + i * DP;
 #pragma unroll 1
-      for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 32) {
+      for (int c = 0; c < DP; c += 32) {
         uint32_t o[32];
         tmem_ld32(oc + c, o);
         tmem_wait_ld();
