@@ -12,15 +12,19 @@
 // Tiles: the G query heads of a kv head and floor(128 / G) consecutive tokens are the 128
 // rows of one query tile (row = token * G + head), so short prompts fill tiles and every key
 // is loaded once for the whole group. A CTA holds two query tiles (one for heads wider than
-// 128) and walks the keys 64 at a time. Keys and values come page by page into swizzled
+// 128) and walks the keys 128 (64) at a time. Keys and values come page by page into swizzled
 // tiles of one ring in shared memory; q k^T goes to TMEM, thread r of a softmax warpgroup
-// reads row r, writes the weights back over the scores as 16-bit values, and the second
-// product reads them from TMEM. Each query tile has two score buffers: the scores of the next
-// keys are made while the softmax warps work on these, which therefore hardly ever wait.
-// (128 keys a tile and one buffer: the softmax, 2370 clocks, and the two products behind it,
-// 1440, took turns, 503 us for 8192 tokens.) The running output stays in TMEM; it is rescaled
-// only when a row's maximum has grown by more than 2^8 since its last rescaling (the weights
-// then reach at most 2^8, harmless in 32-bit sums).
+// takes row r into registers, writes the weights to TMEM as 16-bit values, and the second
+// product reads them from there. Tensor memory holds two outputs of 128 columns, two sets of
+// weights of 64 and ONE score buffer of 128: it is free again as soon as a warpgroup has its
+// scores in registers, so the two query tiles take turns with it, each tile's next scores are
+// there when its softmax has done with the last ones, and the products run in between.
+// Measured for 8192 tokens of 32 / 8 heads of 128 on the way: weights written over the scores
+// (so that scores, softmax and output of a tile take turns) 495 us, 64-key tiles with two
+// score buffers per query tile 490 us (a product of 64 columns takes as long as one of 128).
+// The running output stays in TMEM; it is rescaled only when a row's maximum has grown by more
+// than 2^8 since its last rescaling (the weights then reach at most 2^8, harmless in 32-bit
+// sums).
 //
 // Warps: 4 softmax warps per query tile, one that loads queries and values, one that issues
 // the products, two that load keys.
@@ -38,22 +42,23 @@ namespace {
 template <int DP>
 struct PShape {
   static constexpr int NQ = DP == 256 ? 1 : 2;     // query tiles
-  static constexpr int BN = 64;                    // keys of a tile
+  static constexpr int BN = DP == 256 ? 64 : 128;  // keys of a tile
   static constexpr int NB = DP / 64;               // 128-byte column blocks of a row
   static constexpr int QB = 128 * DP * 2, KB = BN * DP * 2;
-  static constexpr int SLOTS = DP == 256 ? 5 : 10; // tiles of keys or values in flight
+  static constexpr int SLOTS = DP == 64 ? 10 : 5;  // tiles of keys or values in flight
   static constexpr int BARS = NQ * QB + SLOTS * KB;
-  static constexpr int NBARS = 1 + 2 * SLOTS + 1 + 7 * NQ;
+  static constexpr int NBARS = 1 + 2 * SLOTS + 2 + 4 * NQ;
   static constexpr int SMEM = BARS + NBARS * 8 + 16;
   static_assert(SMEM <= 232448, "a CTA's shared memory");
-  static constexpr int OCOL = NQ * 2 * BN;         // first TMEM column of the outputs; scores before
-  static constexpr int COLS = 512;
+  // TMEM columns: one score buffer for all query tiles, their weights, their outputs
+  static constexpr int PCOL = BN, OCOL = PCOL + NQ * BN / 2, COLS = 512;
   static_assert(OCOL + NQ * DP <= COLS, "tensor memory");
   static constexpr int OW = NQ * 4;                // first of the other warps
   static constexpr int THREADS = NQ * 128 + 128;
 };
 
-constexpr int kPoly = 4;  // of 16 pairs
+constexpr int kPoly = 0;          // of 16 pairs
+constexpr int kLaunchRegs = 168;  // a thread's at launch, where warps shift registers: (208 + 208 + 88) / 3
 // 2^f on [-1/2, 1/2], the polynomial of degree 4 with the least relative error
 constexpr float kExpC0 = 0.999999261f;
 constexpr float kExpC1 = 0.693121815f;
@@ -269,11 +274,12 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
   uint64_t* full = qfull + 1;
   uint64_t* empty = full + SLOTS;
   uint64_t* vfix = empty + SLOTS;
-  uint64_t* sfull = vfix + 1;         // [NQ][2] scores in a buffer
-  uint64_t* odone = sfull + 2 * NQ;   // [NQ] a query tile's product with the values is done
-  uint64_t* pready = odone + NQ;      // [NQ][2][2] half of the weights in a buffer
-  uint32_t* slot = reinterpret_cast<uint32_t*>(pready + 4 * NQ);
-  static_assert(2 + 2 * SLOTS + 7 * NQ == C::NBARS, "the barriers above");
+  uint64_t* sfree = vfix + 1;     // the score buffer's content is in registers
+  uint64_t* sfull = sfree + 1;    // [NQ] a query tile's scores are in the buffer
+  uint64_t* odone = sfull + NQ;   // [NQ] a query tile's product with the values is done
+  uint64_t* pready = odone + NQ;  // [NQ][2] half of a query tile's weights
+  uint32_t* slot = reinterpret_cast<uint32_t*>(pready + 2 * NQ);
+  static_assert(3 + 2 * SLOTS + 4 * NQ == C::NBARS, "the barriers above");
   // the same in all lanes, and known to be: the products' operands then live in uniform registers
   const int warp = __shfl_sync(0xFFFFFFFFu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   pdl_wait();
@@ -315,9 +321,9 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
     mbar_init(qfull, 1);
     for (int i = 0; i < SLOTS; ++i) mbar_init(full + i, 1), mbar_init(empty + i, 1);
     mbar_init(vfix, 1);
-    for (int i = 0; i < 2 * NQ; ++i) mbar_init(sfull + i, 1);
-    for (int i = 0; i < NQ; ++i) mbar_init(odone + i, 1);
-    for (int i = 0; i < 4 * NQ; ++i) mbar_init(pready + i, 4);
+    mbar_init(sfree, 4);
+    for (int i = 0; i < NQ; ++i) mbar_init(sfull + i, 1), mbar_init(odone + i, 1);
+    for (int i = 0; i < 2 * NQ; ++i) mbar_init(pready + i, 4);
     fence_mbar_init();
   }
   if (warp == OW + 1) {
@@ -334,8 +340,11 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
   // grid must find that all of this grid's CTAs have theirs
   pdl_trigger();
 
+  // the softmax warps hold a row's scores in registers: they take what the others leave
+  // (208 + 208 + 88 = 3 x 168, the launch's share)
   if (warp >= OW) {
     const int32_t* row = a.tables + b * a.table_row;
+    if (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp == OW) {
       // ---- queries and values, by TMA ----------------------------------------------------
       bool ok = true;
@@ -456,31 +465,34 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
 #pragma unroll
       for (int k = 0; k < BN / 16; ++k)
         v_at[k] = ((16u * k >> vlog) * vbox + (16u * k & ((1u << vlog) - 1)) * 128) >> 4;
-      auto qk = [&](int i, int buf, int sl) {  // scores of query tile i
+      auto qk = [&](int i, int t, int sl) {  // scores of query tile i, key tile t
+        const int use = t * NQ + i;  // of the score buffer: the one before must be in registers
+        if (use && !mbar_wait(sfree, (use - 1) & 1)) return false;
+        fence_after();
         const uint64_t qd = q_desc + i * (C::QB >> 4), kd = k_desc + static_cast<uint32_t>(sl * (C::KB >> 4));
         if (elect_one()) {
 #pragma unroll
           for (int c = 0; c < NB; ++c)
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              umma_ss(tmem + (i * 2 + buf) * BN, qd + (c * (128 * 128 >> 4) + 2 * k), kd + (c * (BN * 128 >> 4) + 2 * k),
-                      id_qk, c > 0 || k > 0);
-          umma_commit(sfull + i * 2 + buf);
+              umma_ss(tmem, qd + (c * (128 * 128 >> 4) + 2 * k), kd + (c * (BN * 128 >> 4) + 2 * k), id_qk, c > 0 || k > 0);
+          umma_commit(sfull + i);
         }
         __syncwarp();
+        return true;
       };
       // the output of query tile i takes a value tile; the first half of the weights may be
       // multiplied while the second is still being made
-      auto pv = [&](int i, int buf, int sl, uint32_t par, bool acc) {
+      auto pv = [&](int i, int t, int sl) {
         const uint64_t vd = v_desc + static_cast<uint32_t>(sl * (C::KB >> 4));
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          if (!mbar_wait(pready + (i * 2 + buf) * 2 + h, par)) return false;
+          if (!mbar_wait(pready + i * 2 + h, t & 1)) return false;
           fence_after();
           if (elect_one()) {
 #pragma unroll
             for (int k = h * (BN / 32); k < (h + 1) * (BN / 32); ++k)
-              umma_ts(tmem + C::OCOL + i * DP, tmem + (i * 2 + buf) * BN + 8 * k, vd + v_at[k], id_pv, acc || k > 0);
+              umma_ts(tmem + C::OCOL + i * DP, tmem + C::PCOL + i * (BN / 2) + 8 * k, vd + v_at[k], id_pv, t > 0 || k > 0);
             if (h) umma_commit(odone + i);
           }
           __syncwarp();
@@ -502,27 +514,25 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
       };
       int ks = 0, vs = 0;
       bool ok = mbar_wait(qfull, 0) && wait_tile(ks);
-      if (ok) {
-        for (int i = 0; i < NQ; ++i) qk(i, 0, ks);
-        release(ks);
-      }
+      for (int i = 0; i < NQ; ++i) ok = ok && qk(i, 0, ks);
+      if (ok) release(ks);
       for (int t = 0; t < nt && ok; ++t) {
-        ok = wait_tile(vs);  // tile 2 t + 1 of the ring
-        if (t + 1 < nt && ok) {
-          // into the other buffers: their weights went into products issued before, and
-          // products run in the order of their issue
-          ok = wait_tile(ks);
-          if (!ok) break;
+        const bool more = t + 1 < nt;
+        ok = wait_tile(vs);
+        if (ok && more) ok = wait_tile(ks);
 #pragma unroll
-          for (int i = 0; i < NQ; ++i) qk(i, (t + 1) & 1, ks);
-          release(ks);
+        for (int i = 0; i < NQ; ++i) {
+          if (more) {
+            ok = ok && qk(i, t + 1, ks);
+            if (ok && i == NQ - 1) release(ks);
+          }
+          ok = ok && pv(i, t, vs);
         }
-#pragma unroll
-        for (int i = 0; i < NQ; ++i) ok = ok && pv(i, t & 1, vs, t >> 1 & 1, t > 0);
         if (ok) release(vs);
       }
     }
   } else {
+    if (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ---- softmax: thread r of a warpgroup has row r of its query tile ---------------------
     const int i = warp >> 2, r = (warp & 3) * 32 + lane;
     const int tok = t0 + i * a.toks + r / a.group, g = r % a.group;
@@ -537,16 +547,17 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int t = 0; t < nt; ++t) {
-      const int buf = t & 1, par = t >> 1 & 1;
-      ok = mbar_wait(sfull + i * 2 + buf, par);
+      ok = mbar_wait(sfull + i, t & 1);
       ok = __all_sync(0xFFFFFFFFu, ok);
       if (!ok) break;
       fence_after();
-      const uint32_t sc = lanes + (i * 2 + buf) * BN;
       uint32_t sr[BN];
 #pragma unroll
-      for (int c = 0; c < BN; c += 32) tmem_ld32(sc + c, sr + c);
+      for (int c = 0; c < BN; c += 32) tmem_ld32(lanes + c, sr + c);
       tmem_wait_ld();
+      fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(sfree);
       float* s = reinterpret_cast<float*>(sr);
       if (odd_scale) {
 #pragma unroll
@@ -578,11 +589,13 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
         m = top == INFINITY ? __int_as_float(0x7FFFFFFF) : top;  // inf - inf
         l *= f;
       }
-      if (t > 0 && __any_sync(0xFFFFFFFFu, f != 1.f)) {
+      if (t > 0) {  // the product that reads the last weights, and adds to the output
         ok = mbar_wait(odone + i, (t - 1) & 1);
         ok = __all_sync(0xFFFFFFFFu, ok);
         if (!ok) break;
         fence_after();
+      }
+      if (t > 0 && __any_sync(0xFFFFFFFFu, f != 1.f)) {
         const uint32_t oc = lanes + C::OCOL + i * DP;
 #pragma unroll 1
         for (int c = 0; c < DP; c += 32) {
@@ -601,8 +614,9 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
         tmem_wait_st();
         fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(pready + (i * 2 + buf) * 2 + h);
+        if (lane == 0) mbar_arrive(pready + i * 2 + h);
       };
+      const uint32_t pc = lanes + C::PCOL + i * (BN / 2);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t p[BN / 4];
@@ -613,7 +627,8 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
         if (h) handed(0);  // its store has had time to finish
         if (edge) weights<DT, BN / 4, 0>(v + BN / 4, s2, z, p + BN / 8, sum);
         else weights<DT, BN / 4, kPoly>(v + BN / 4, s2, z, p + BN / 8, sum);
-        tmem_st16(sc + h * (BN / 4), p);
+#pragma unroll
+        for (int c = 0; c < BN / 4; c += 16) tmem_st16(pc + h * (BN / 4) + c, p + c);
       }
       handed(1);
       float a0, a1;
@@ -728,6 +743,12 @@ cudaError_t launch(const ggufmm_attention_args& p, cudaStream_t st) {
   if (!(ready.load(std::memory_order_acquire) >> (dev & 63) & 1)) {
     e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     if (e != cudaSuccess) return e;
+    // the warps' shares of registers must add up to no more than the launch brings: a build
+    // that needs fewer would wait for registers that nobody gives back
+    cudaFuncAttributes fa;
+    e = cudaFuncGetAttributes(&fa, fn);
+    if (e != cudaSuccess) return e;
+    if (C::NQ == 2 && fa.numRegs < kLaunchRegs) return cudaErrorInvalidKernelImage;
     ready.fetch_or(uint64_t(1) << (dev & 63), std::memory_order_release);
   }
   return pdl_launch(fn, dim3(static_cast<unsigned>(ctas)), dim3(C::THREADS), C::SMEM, st, qm, vm, a);
