@@ -10,7 +10,7 @@
 
 namespace ggufmm {
 
-size_t paged_decode_workspace(int64_t head_dim);  // attn_decode.cu
+size_t paged_decode_workspace(int64_t group, int64_t head_dim);  // attn_decode.cu
 cudaError_t launch_paged_decode(const ggufmm_attention_args& p, void* workspace, cudaStream_t st);
 cudaError_t launch_paged_prompt(const ggufmm_attention_args& p, cudaStream_t st);  // attn_prompt.cu
 
@@ -46,7 +46,8 @@ using namespace ggufmm;
 extern "C" size_t ggufmm_paged_attention_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_heads,
                                                         int64_t head_dim) {
   if (batch < 1 || q_heads < 1 || kv_heads < 1 || head_dim < 8 || head_dim > GGUFMM_MAX_HEAD_DIM) return 0;
-  return paged_decode_workspace(head_dim);
+  if (q_heads % kv_heads) return 0;
+  return paged_decode_workspace(q_heads / kv_heads, head_dim);
 }
 
 extern "C" int ggufmm_paged_attention(const ggufmm_attention_args* args, void* workspace, size_t workspace_bytes,

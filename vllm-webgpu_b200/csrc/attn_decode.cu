@@ -15,7 +15,9 @@
 // over the lengths on the device. An item inside one run is written directly. An item that
 // crosses runs leaves fp32 partials (m, sum, o) in the workspace, and the last of its CTAs
 // to finish (a counter) adds them in the order of the CTAs, so the result does not depend
-// on which was last.
+// on which was last. (Handing part of the work out in short runs as CTAs finish was measured:
+// 196 to 208 us for 64 sequences up to 8192 tokens against 195, 124 to 152 us for one of 131035
+// against 105, since every run costs a join.)
 //
 // Inside a CTA each warp owns every W-th group of 16 tokens and its own ring of stages,
 // filled by TMA two pages' worth at a time ahead of use, across items: no barrier between
@@ -38,8 +40,10 @@ DevInfo device_info(int dev);  // capi.cu
 
 namespace {
 
-constexpr int kMaxGrid = 256;                      // CTAs a workspace has room for
-constexpr size_t kCounterBytes = kMaxGrid * 4;     // one arrival counter per CTA that an item may start in
+constexpr int kMaxGrid = 160;               // CTAs a workspace has room for
+constexpr int kMinRun = 1;                  // blocks of a run at least
+constexpr size_t kCounterBytes = 1024;      // one arrival counter per CTA
+static_assert(kMaxGrid * 4 <= kCounterBytes, "counters");
 
 template <int DP>
 struct Shape {
@@ -50,8 +54,13 @@ struct Shape {
   static constexpr int S = 196608 / (W * STAGE);    // stages per warp
   static constexpr int BLOCK = 16 * W;              // tokens
   static constexpr int RING = W * S * STAGE;
-  static constexpr int JOIN = W * 8 * DP * 4;       // 8 rows of every warp's sums
-  static constexpr int SMEM = RING + JOIN + W * 32 * 4 + 64 * 4 + W * S * 8 + 64 + 1024;
+  static constexpr int JOIN = RING;                 // 8 rows of every warp's sums
+  static constexpr int ML = JOIN + W * 8 * DP * 4;  // [W][16][2] every warp's max and sum per row
+  static constexpr int PRE = ML + W * 128;          // [128] blocks per item before each group of sequences
+  static constexpr int MISC = PRE + 1024;           // [8] scan scratch
+  static constexpr int BARS = MISC + 64;
+  static constexpr int SMEM = BARS + W * S * 8;
+  static_assert(SMEM <= 232448, "a CTA's shared memory");
 };
 
 struct DecodeArgs {
@@ -59,8 +68,10 @@ struct DecodeArgs {
   void* out;
   const int32_t* tables;
   const int32_t* lens;
-  float* part;      // [2 * grid][16][DP] sums, then [2 * grid][16][2] (max, sum)
-  uint32_t* count;  // [grid]
+  float* part;      // two for each CTA: [slots][prows][DP] sums, then [slots][prows][2] (max, sum)
+  uint32_t* count;  // kCounterBytes
+  int64_t slots;
+  int prows;        // rows of a partial: 8 or 16
   int64_t q_row, q_head, o_row, o_head, table_row;
   int64_t room;     // tokens a table row has room for
   int batch, hkv, group, hblocks, d, page_size, num_pages, window;
@@ -68,9 +79,29 @@ struct DecodeArgs {
   float s2;         // scale * log2(e)
 };
 
-// A walk over the blocks [u, end) of the work list: where the current item's blocks lie.
+// x / y for whole numbers whose quotient is below 2^22, by way of 32-bit floats: a 64-bit
+// division is some 150 clocks, and every CTA goes through a few before it can load anything.
+__device__ __forceinline__ int64_t small_quotient(int64_t x, int64_t y) {
+  int64_t q = static_cast<int64_t>(__fdividef(static_cast<float>(x), static_cast<float>(y)));
+  while (q * y > x) --q;
+  while ((q + 1) * y <= x) ++q;
+  return q;
+}
+
+// The work list cut into runs, the first `extra` of them one block longer than `size`.
+struct Runs {
+  int64_t size, extra;
+  __device__ __forceinline__ int64_t begin(int r) const { return r * size + min(static_cast<int64_t>(r), extra); }
+  __device__ __forceinline__ int holding(int64_t block) const {  // the run of a block
+    const int64_t longer = extra * (size + 1);
+    return static_cast<int>(block < longer ? small_quotient(block, size + 1)
+                                           : extra + small_quotient(block - longer, size));
+  }
+};
+
+// A walk over the blocks of a run: where the current item's blocks lie.
 struct Walk {
-  int64_t u, end, base;  // next block, end of the run, first block of the current sequence
+  int64_t left, base;    // blocks of the run to come, first block of the current sequence
   int b, nb, f, len, lo; // sequence: index, blocks per item, first block's index, length, first visible token
   int item, k0, n;       // current segment: item within the sequence, its first block and their number
   bool starts, ends;     // whether the segment holds the item's first / last block
@@ -99,22 +130,26 @@ __device__ __forceinline__ void walk_load(const DecodeArgs& a, Walk& w) {
 // The next segment of the run; false at its end.
 template <int BLOCK>
 __device__ __forceinline__ bool walk_next(const DecodeArgs& a, Walk& w, int hi) {
-  if (w.u >= w.end) return false;
-  while (w.nb == 0 || w.u >= w.base + static_cast<int64_t>(w.nb) * hi) {
-    w.base += static_cast<int64_t>(w.nb) * hi;
-    if (++w.b >= a.batch) {  // only if the lengths changed under the kernel
-      w.u = w.end;
-      return false;
+  if (w.left <= 0) return false;
+  w.k0 += w.n;
+  if (w.k0 >= w.nb) {
+    w.k0 = 0;
+    if (++w.item >= hi) {
+      w.item = 0;
+      do {
+        w.base += static_cast<int64_t>(w.nb) * hi;
+        if (++w.b >= a.batch) {  // only if the lengths changed under the kernel
+          w.left = 0;
+          return false;
+        }
+        walk_load<BLOCK>(a, w);
+      } while (w.nb == 0);
     }
-    walk_load<BLOCK>(a, w);
   }
-  const int64_t off = w.u - w.base;
-  w.item = static_cast<int>(off / w.nb);
-  w.k0 = static_cast<int>(off - static_cast<int64_t>(w.item) * w.nb);
-  w.n = static_cast<int>(min(static_cast<int64_t>(w.nb - w.k0), w.end - w.u));
+  w.n = static_cast<int>(min(static_cast<int64_t>(w.nb - w.k0), w.left));
   w.starts = w.k0 == 0;
   w.ends = w.k0 + w.n == w.nb;
-  w.u += w.n;
+  w.left -= w.n;
   return true;
 }
 
@@ -127,6 +162,36 @@ __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, i
       : "memory");
 }
 
+// To the first block of run r: the group of sequences that holds it, by all lanes of a warp.
+template <int BLOCK>
+__device__ __forceinline__ void walk_to(const DecodeArgs& a, Walk& w, const Runs& runs, int r, const int64_t* pre, int gs,
+                                        int hi, int lane) {
+  const int64_t u = runs.begin(r);
+  w.left = runs.begin(r + 1) - u;
+  int g = -1;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) g += __popc(__ballot_sync(0xFFFFFFFFu, pre[x * 32 + lane] * hi <= u));
+  g = max(g, 0);
+  w.b = min(g * gs, a.batch - 1);
+  w.base = pre[g] * hi;
+  walk_load<BLOCK>(a, w);
+  while (u >= w.base + static_cast<int64_t>(w.nb) * hi && w.b + 1 < a.batch) {
+    w.base += static_cast<int64_t>(w.nb) * hi;
+    ++w.b;
+    walk_load<BLOCK>(a, w);
+  }
+  const int64_t off = u - w.base;
+  w.item = w.nb ? static_cast<int>(small_quotient(off, w.nb)) : 0;
+  w.k0 = static_cast<int>(off - static_cast<int64_t>(w.item) * w.nb);
+  w.n = 0;  // the first segment starts here
+}
+
+__device__ __forceinline__ uint32_t arrive_acq_rel(uint32_t* p) {
+  uint32_t old;
+  asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(old) : "l"(p) : "memory");
+  return old;
+}
+
 // R: rows of a TMA box, 16, or 8 where the page size is an odd multiple of 8.
 template <int DP, int DT, int R>
 __global__ void __launch_bounds__(Shape<DP>::W * 32, 1)
@@ -136,91 +201,62 @@ __global__ void __launch_bounds__(Shape<DP>::W * 32, 1)
   constexpr int W = C::W, S = C::S, NB = C::NB, BLOCK = C::BLOCK, T = W * 32;
   // row r, column block c of a 16-token half: (r / 8) * HS + c * BS + (r % 8) * 128
   constexpr int HS = R == 16 ? 1024 : NB * 1024, BS = R == 16 ? 2048 : 1024;
-  extern __shared__ uint8_t raw[];
-  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  float* join = reinterpret_cast<float*>(ring + C::RING);
-  float* ml = join + C::JOIN / 4;      // [W][16][2]: each warp's max and sum per row
-  float* misc = ml + W * 32;           // [64]: scan scratch
-  uint64_t* bars = reinterpret_cast<uint64_t*>(misc + 64);
+  extern __shared__ __align__(1024) uint8_t ring[];
+  float* join = reinterpret_cast<float*>(ring + C::JOIN);
+  float* ml = reinterpret_cast<float*>(ring + C::ML);
+  int64_t* pre = reinterpret_cast<int64_t*>(ring + C::PRE);
+  int64_t* misc = reinterpret_cast<int64_t*>(ring + C::MISC);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + C::BARS);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint64_t* full = bars + warp * S;
   uint8_t* mine = ring + warp * S * C::STAGE;
-  if (tid == 0)
-    for (int i = 0; i < W * S; ++i) mbar_init(bars + i, 1);
-  fence_mbar_init();
-  __syncthreads();
+  if (smem_u32(ring) & 1023) {  // the swizzled tiles need it; the driver places a CTA's memory so
+    if (tid == 0) atomicOr(&g_device_error, kErrIndex);
+    return;
+  }
+  if (tid < W * S) {
+    mbar_init(bars + tid, 1);
+    fence_mbar_init();
+  }
   pdl_wait();
   pdl_trigger();
 
-  // ---- this CTA's run of blocks ----------------------------------------------------
+  // ---- the work: blocks per item before each of 128 groups of sequences ----------------
   const int hi = a.hkv * a.hblocks;  // items per sequence
-  int64_t* scan = reinterpret_cast<int64_t*>(misc);  // [W + 2]
-  int64_t total = 0;
-  {
-    int64_t s = 0;
-    for (int b = tid; b < a.batch; b += T) {
+  const int gs = (a.batch + 127) / 128;
+  int64_t mine_b = 0, inc;
+  if (tid < 128) {
+    for (int b = tid * gs; b < min((tid + 1) * gs, a.batch); ++b) {
       int lo;
       bool cut;
       const int len = seq_len(a, b, &cut);
       if (cut && blockIdx.x == 0) atomicOr(&g_device_error, kErrIndex);
-      s += seq_blocks<BLOCK>(a, len, &lo);
+      mine_b += seq_blocks<BLOCK>(a, len, &lo);
     }
+    inc = mine_b;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-    if (lane == 0) scan[warp] = s;
-    if (tid == 0) scan[W] = scan[W + 1] = 0;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < W; ++i) total += scan[i];
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    if (lane == 31) misc[warp] = inc;
   }
+  __syncthreads();
+  int64_t total = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (tid < 128 && i == warp) pre[tid] = total + inc - mine_b;
+    total += misc[i];
+  }
+  __syncthreads();
   const int64_t blocks = total * hi;
-  const int64_t runs = min(static_cast<int64_t>(gridDim.x), blocks);
-  const int64_t me = blockIdx.x;
-  auto run_begin = [&](int64_t c) { return c * blocks / runs; };
-  Walk cw;
-  cw.u = me < runs ? run_begin(me) : 0;
-  cw.end = me < runs ? run_begin(me + 1) : 0;
-  cw.b = 0;
-  cw.base = 0;
-  cw.nb = 0;
-  if (cw.u < cw.end) {
-    // the sequence of the run's first block: sums of blocks over tiles of T sequences
-    int64_t before = 0;
-    for (int b0 = 0;; b0 += T) {
-      int lo, nb = 0;
-      bool cut;
-      if (b0 + tid < a.batch) nb = seq_blocks<BLOCK>(a, seq_len(a, b0 + tid, &cut), &lo);
-      int64_t inc = nb;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
-        if (lane >= o) inc += v;
-      }
-      __syncthreads();  // the last reads of scan
-      if (lane == 31) scan[warp] = inc;
-      __syncthreads();
-      int64_t tile = 0, front = 0;
-#pragma unroll
-      for (int i = 0; i < W; ++i) {
-        if (i < warp) front += scan[i];
-        tile += scan[i];
-      }
-      const int64_t first = before + front + inc - nb;  // blocks per item before this thread's sequence
-      if (nb > 0 && cw.u >= first * hi && cw.u < (first + nb) * hi) {
-        scan[W] = b0 + tid;
-        scan[W + 1] = first * hi;
-      }
-      const bool here = cw.u < (before + tile) * hi;
-      before += tile;
-      if (here || b0 + T >= a.batch) break;  // the total says that it is found by the last tile
-    }
-    __syncthreads();
-    cw.b = static_cast<int>(scan[W]);
-    cw.base = scan[W + 1];
-    walk_load<BLOCK>(a, cw);
-  }
+  const int me = static_cast<int>(blockIdx.x);
+  const int nruns = static_cast<int>(min(static_cast<int64_t>(gridDim.x), (blocks + kMinRun - 1) / kMinRun));
+  Runs runs;
+  runs.size = nruns == 0 ? 0 : blocks < (int64_t(1) << 22) ? small_quotient(blocks, nruns) : blocks / nruns;
+  runs.extra = blocks - runs.size * nruns;
   // sequences that see nothing: zeros
-  for (int b = static_cast<int>(me); b < a.batch; b += gridDim.x) {
+  for (int b = me; b < a.batch; b += gridDim.x) {
     int lo;
     bool cut;
     if (seq_blocks<BLOCK>(a, seq_len(a, b, &cut), &lo)) continue;
@@ -229,10 +265,10 @@ __global__ void __launch_bounds__(Shape<DP>::W * 32, 1)
       *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + b * a.o_row + i / per * a.o_head + i % per * 8) =
           make_uint4(0, 0, 0, 0);
   }
-  __syncthreads();
-  if (cw.u >= cw.end) return;
-
-  // ---- the producer half of each warp: the chunks of its walk, S stages ahead ---------
+  if (me >= nruns) return;
+  Walk cw;
+  walk_to<BLOCK>(a, cw, runs, me, pre, gs, hi, lane);
+  // ---- the producer half of each warp: the chunks of its walk, S stages ahead ---------------
   Walk pw = cw;
   int pk = 0, pn = 0, pbase = 0;  // next block of the segment, their number, block of pid's lane 0
   int pid0 = 0, pid1 = 0;         // lane i: pages of the chunk's first (and second) 8 tokens, block pbase + i
@@ -304,6 +340,7 @@ __global__ void __launch_bounds__(Shape<DP>::W * 32, 1)
   const uint32_t mine_u = smem_u32(mine);
   // ldmatrix row addresses inside a 16-token half; lane l supplies row l % 16 of an x4
   const int lr = lane & 7, lq = lane >> 3;
+  bool opening = true;  // the run's first segment
   while (walk_next<BLOCK>(a, cw, hi)) {
     const int head = cw.item / a.hblocks, hb = cw.item % a.hblocks;
     const int rows = min(a.group - hb * 16, 16);
@@ -421,49 +458,43 @@ __global__ void __launch_bounds__(Shape<DP>::W * 32, 1)
     l0 += __shfl_xor_sync(0xFFFFFFFFu, l0, 2);
     l1 += __shfl_xor_sync(0xFFFFFFFFu, l1, 2);
     if (t4 == 0) {
-      ml[(warp * 16 + g) * 2] = m0;
-      ml[(warp * 16 + g) * 2 + 1] = l0;
-      ml[(warp * 16 + g + 8) * 2] = m1;
-      ml[(warp * 16 + g + 8) * 2 + 1] = l1;
+      *reinterpret_cast<float2*>(ml + (warp * 16 + g) * 2) = make_float2(m0, l0);
+      *reinterpret_cast<float2*>(ml + (warp * 16 + g + 8) * 2) = make_float2(m1, l1);
     }
-    __syncthreads();
     const bool whole = cw.starts && cw.ends;
-    const int64_t seg0 = cw.u - cw.n;                               // first block of the segment
     const int64_t item0 = cw.base + static_cast<int64_t>(cw.item) * cw.nb;  // first block of the item
-    const int slot = static_cast<int>(me) * 2 + (seg0 == run_begin(me) ? 0 : 1);
-    float* part_o = a.part + static_cast<int64_t>(slot) * 16 * DP;
-    float* part_ml = a.part + static_cast<int64_t>(2 * gridDim.x) * 16 * DP + slot * 32;
+    const int slot = me * 2 + (opening ? 0 : 1);
+    float* const part_ml = a.part + a.slots * a.prows * DP;
     uint16_t* outp = static_cast<uint16_t*>(a.out) + cw.b * a.o_row + qh0 * a.o_head;
 #pragma unroll 1
     for (int h = 0; h * 8 < rows; ++h) {
-      float mx = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < W; ++w) mx = fmaxf(mx, ml[(w * 16 + h * 8 + g) * 2]);
-      const float z = mx == -INFINITY ? 0.f : mx;
-      const float f = exp2_fast((h ? m1 : m0) - z);
-#pragma unroll
-      for (int i = 0; i < DP / 8; ++i) {
-        const float x = h ? o[i][2] : o[i][0], y = h ? o[i][3] : o[i][1];
-        *reinterpret_cast<float2*>(join + (warp * 8 + g) * DP + i * 8 + t4 * 2) = make_float2(x * f, y * f);
-      }
+      for (int i = 0; i < DP / 8; ++i)
+        *reinterpret_cast<float2*>(join + (warp * 8 + g) * DP + i * 8 + t4 * 2) =
+            make_float2(h ? o[i][2] : o[i][0], h ? o[i][3] : o[i][1]);
       __syncthreads();
       for (int e = tid; e < 8 * DP / 4; e += T) {
         const int r = e / (DP / 4), c = e % (DP / 4) * 4, row = h * 8 + r;
         if (row >= rows) continue;
+        float2 w[W];
         float mr = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < W; ++w) mr = fmaxf(mr, ml[(w * 16 + row) * 2]);
+        for (int x = 0; x < W; ++x) {
+          w[x] = *reinterpret_cast<const float2*>(ml + (x * 16 + row) * 2);
+          mr = fmaxf(mr, w[x].x);
+        }
         const float zr = mr == -INFINITY ? 0.f : mr;
         float l = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-          l += ml[(w * 16 + row) * 2 + 1] * exp2_fast(ml[(w * 16 + row) * 2] - zr);
-          const float4 v = *reinterpret_cast<const float4*>(join + (w * 8 + r) * DP + c);
-          acc.x += v.x;
-          acc.y += v.y;
-          acc.z += v.z;
-          acc.w += v.w;
+        for (int x = 0; x < W; ++x) {
+          const float f = exp2_fast(w[x].x - zr);
+          const float4 v = *reinterpret_cast<const float4*>(join + (x * 8 + r) * DP + c);
+          l += w[x].y * f;
+          acc.x += v.x * f;
+          acc.y += v.y * f;
+          acc.z += v.z * f;
+          acc.w += v.w * f;
         }
         if (whole) {
           const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -471,53 +502,53 @@ __global__ void __launch_bounds__(Shape<DP>::W * 32, 1)
             *reinterpret_cast<uint2*>(outp + row * a.o_head + c) =
                 make_uint2(pack16<DT>(acc.x * inv, acc.y * inv), pack16<DT>(acc.z * inv, acc.w * inv));
         } else {
-          __stcg(reinterpret_cast<float4*>(part_o + row * DP + c), acc);
-          if (c == 0) __stcg(reinterpret_cast<float2*>(part_ml + row * 2), make_float2(mr, l));
+          __stcg(reinterpret_cast<float4*>(a.part + (static_cast<int64_t>(slot) * a.prows + row) * DP + c), acc);
+          if (c == 0) __stcg(reinterpret_cast<float2*>(part_ml + (static_cast<int64_t>(slot) * a.prows + row) * 2), make_float2(mr, l));
         }
       }
       __syncthreads();
     }
+    opening = false;
     if (whole) continue;
-    // ---- join the CTAs of this item: the last one to arrive adds the partials ----------
-    auto run_of = [&](int64_t block) {  // the run that holds a block
-      int64_t c = block * runs / blocks;
-      while (run_begin(c + 1) <= block) ++c;
-      while (run_begin(c) > block) --c;
-      return c;
-    };
-    const int64_t c0 = run_of(item0), c1 = run_of(item0 + cw.nb - 1);
-    if (tid == 0) {
-      __threadfence();
-      misc[63] = __uint_as_float(atomicAdd(a.count + c0, 1u));
-      __threadfence();
-    }
+    // ---- join the CTAs of this item: the last one to arrive adds the partials ---------------
+    const int c0 = cw.starts ? me : runs.holding(item0), c1 = cw.ends ? me : runs.holding(item0 + cw.nb - 1);
+    if (tid == 0) misc[7] = arrive_acq_rel(a.count + c0) + 1 == static_cast<uint32_t>(c1 - c0 + 1);
     __syncthreads();
-    if (__float_as_uint(misc[63]) + 1 != static_cast<uint32_t>(c1 - c0 + 1)) continue;
+    const bool last = misc[7] != 0;
+    __syncthreads();  // misc[7] is written again at the next item
+    if (!last) continue;
     if (tid == 0) a.count[c0] = 0;
-    const int slot0 = static_cast<int>(c0) * 2 + (item0 == run_begin(c0) ? 0 : 1);
-    const float* po = a.part;
-    const float* pm = a.part + static_cast<int64_t>(2 * gridDim.x) * 16 * DP;
+    const int64_t slot0 = static_cast<int64_t>(c0) * 2 + (item0 == runs.begin(c0) ? 0 : 1);
     for (int e = tid; e < rows * (DP / 4); e += T) {
       const int row = e / (DP / 4), c = e % (DP / 4) * 4;
-      float mr = -INFINITY;
-      for (int64_t k = c0; k <= c1; ++k) {
-        const int64_t sl = k == c0 ? slot0 : 2 * k;
-        mr = fmaxf(mr, __ldcg(pm + sl * 32 + row * 2));
-      }
-      const float zr = mr == -INFINITY ? 0.f : mr;
-      float l = 0.f;
+      float mr = -INFINITY, l = 0.f;
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-      for (int64_t k = c0; k <= c1; ++k) {
-        const int64_t sl = k == c0 ? slot0 : 2 * k;
-        const float2 mk = __ldcg(reinterpret_cast<const float2*>(pm + sl * 32 + row * 2));
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(po + (sl * 16 + row) * DP + c));
-        const float f = exp2_fast(mk.x - zr);
-        l += mk.y * f;
-        acc.x += v.x * f;
-        acc.y += v.y * f;
-        acc.z += v.z * f;
-        acc.w += v.w * f;
+      constexpr int K = 8;  // partials under way at a time
+      for (int k = c0; k <= c1; k += K) {
+        float2 w[K];
+        float4 v[K];
+        float mk = mr;
+#pragma unroll
+        for (int x = 0; x < K; ++x) {
+          const int64_t at = (k + x == c0 ? slot0 : 2 * static_cast<int64_t>(k + x)) * a.prows + row;
+          w[x] = k + x <= c1 ? __ldcg(reinterpret_cast<const float2*>(part_ml + at * 2)) : make_float2(-INFINITY, 0.f);
+          v[x] = k + x <= c1 ? __ldcg(reinterpret_cast<const float4*>(a.part + at * DP + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int x = 0; x < K; ++x) mk = fmaxf(mk, w[x].x);
+        const float z = mk == -INFINITY ? 0.f : mk, f0 = exp2_fast(mr - z);
+        l *= f0;
+        acc = make_float4(acc.x * f0, acc.y * f0, acc.z * f0, acc.w * f0);
+#pragma unroll
+        for (int x = 0; x < K; ++x) {
+          const float f = exp2_fast(w[x].x - z);
+          l += w[x].y * f;
+          acc.x += v[x].x * f;
+          acc.y += v[x].y * f;
+          acc.z += v[x].z * f;
+          acc.w += v[x].w * f;
+        }
+        mr = mk;
       }
       const float inv = l == 0.f ? 0.f : 1.f / l;
       if (c < a.d)
@@ -581,8 +612,8 @@ int padded_dim(int64_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
 }  // namespace
 
-size_t paged_decode_workspace(int64_t head_dim) {
-  return kCounterBytes + static_cast<size_t>(2 * kMaxGrid) * 16 * (padded_dim(head_dim) + 2) * 4;
+size_t paged_decode_workspace(int64_t group, int64_t head_dim) {
+  return kCounterBytes + static_cast<size_t>(2 * kMaxGrid) * (group <= 8 ? 8 : 16) * (padded_dim(head_dim) + 2) * 4;
 }
 
 cudaError_t launch_paged_decode(const ggufmm_attention_args& p, void* workspace, cudaStream_t st) {
@@ -597,6 +628,8 @@ cudaError_t launch_paged_decode(const ggufmm_attention_args& p, void* workspace,
   a.lens = static_cast<const int32_t*>(p.lens);
   a.count = static_cast<uint32_t*>(workspace);
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + kCounterBytes);
+  a.slots = static_cast<int64_t>(2) * kMaxGrid;
+  a.prows = p.q_heads / p.kv_heads <= 8 ? 8 : 16;
   a.q_row = p.q_row;
   a.q_head = p.q_head;
   a.o_row = p.o_row;
