@@ -19,16 +19,17 @@
 // 196 to 208 us for 64 sequences up to 8192 tokens against 195, 124 to 152 us for one of 131035
 // against 105, since every run costs a join.)
 //
-// Inside a CTA each warp owns every W-th group of 16 tokens and its own ring of stages,
-// filled by TMA two pages' worth at a time ahead of use, across items: no barrier between
-// warps except where an item ends, and the ring keeps streaming over that too.
+// Inside a CTA each warp owns every W-th group of 16 tokens and its own ring of stages, filled
+// by 16-byte asynchronous copies S groups ahead of use, across items: no barrier between warps
+// except where an item ends, and the ring keeps streaming over that too. (TMA boxes of whole
+// 16-token pages did as well at head width 128, but the unit takes about 134 clocks for every
+// request: pages of 8 or 24 tokens, or heads that are no multiple of 64 wide, got 2.4 TB/s.)
 #include <algorithm>
 #include <atomic>
 #include <cmath>
 
 #include "mma16.cuh"
 #include "paged.cuh"
-#include "tcgen05.cuh"
 
 namespace ggufmm {
 
@@ -48,7 +49,6 @@ static_assert(kMaxGrid * 4 <= kCounterBytes, "counters");
 template <int DP>
 struct Shape {
   static constexpr int W = DP == 256 ? 4 : 8;       // warps
-  static constexpr int NB = DP / 64;                // 128-byte column blocks of a row
   static constexpr int HALF = 16 * DP * 2;          // bytes of 16 tokens of K (or V)
   static constexpr int STAGE = 2 * HALF;
   static constexpr int S = 196608 / (W * STAGE);    // stages per warp
@@ -58,14 +58,16 @@ struct Shape {
   static constexpr int ML = JOIN + W * 8 * DP * 4;  // [W][16][2] every warp's max and sum per row
   static constexpr int PRE = ML + W * 128;          // [128] blocks per item before each group of sequences
   static constexpr int MISC = PRE + 1024;           // [8] scan scratch
-  static constexpr int BARS = MISC + 64;
-  static constexpr int SMEM = BARS + W * S * 8;
+  static constexpr int SMEM = MISC + 64;
   static_assert(SMEM <= 232448, "a CTA's shared memory");
 };
 
 struct DecodeArgs {
   const void* q;
   void* out;
+  const uint16_t* k;
+  const uint16_t* v;
+  int64_t k_page, k_head, k_slot, v_page, v_head, v_slot;
   const int32_t* tables;
   const int32_t* lens;
   float* part;      // two for each CTA: [slots][prows][DP] sums, then [slots][prows][2] (max, sum)
@@ -75,7 +77,6 @@ struct DecodeArgs {
   int64_t q_row, q_head, o_row, o_head, table_row;
   int64_t room;     // tokens a table row has room for
   int batch, hkv, group, hblocks, d, page_size, num_pages, window;
-  int one_box;      // a box holds all column blocks of its rows
   float s2;         // scale * log2(e)
 };
 
@@ -153,15 +154,6 @@ __device__ __forceinline__ bool walk_next(const DecodeArgs& a, Walk& w, int hi) 
   return true;
 }
 
-__device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, int c4,
-                                            uint64_t* bar, uint64_t policy) {
-  asm volatile(
-      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], "
-      "[%1, {%2, %3, %4, %5, %6}], [%7], %8;" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(smem_u32(bar)), "l"(policy)
-      : "memory");
-}
-
 // To the first block of run r: the group of sequences that holds it, by all lanes of a warp.
 template <int BLOCK>
 __device__ __forceinline__ void walk_to(const DecodeArgs& a, Walk& w, const Runs& runs, int r, const int64_t* pre, int gs,
@@ -186,38 +178,32 @@ __device__ __forceinline__ void walk_to(const DecodeArgs& a, Walk& w, const Runs
   w.n = 0;  // the first segment starts here
 }
 
+// 16 bytes to shared memory, the first `bytes` (0 or 16) of them from p, the rest zeros.
+__device__ __forceinline__ void copy16(uint32_t dst, const uint16_t* p, uint32_t bytes, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(p), "r"(bytes), "l"(policy)
+               : "memory");
+}
+
 __device__ __forceinline__ uint32_t arrive_acq_rel(uint32_t* p) {
   uint32_t old;
   asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(old) : "l"(p) : "memory");
   return old;
 }
 
-// R: rows of a TMA box, 16, or 8 where the page size is an odd multiple of 8.
-template <int DP, int DT, int R>
-__global__ void __launch_bounds__(Shape<DP>::W * 32, 1)
-    paged_decode_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
-                        const __grid_constant__ DecodeArgs a) {
+template <int DP, int DT>
+__global__ void __launch_bounds__(Shape<DP>::W * 32, 1) paged_decode_kernel(const __grid_constant__ DecodeArgs a) {
   using C = Shape<DP>;
-  constexpr int W = C::W, S = C::S, NB = C::NB, BLOCK = C::BLOCK, T = W * 32;
-  // row r, column block c of a 16-token half: (r / 8) * HS + c * BS + (r % 8) * 128
-  constexpr int HS = R == 16 ? 1024 : NB * 1024, BS = R == 16 ? 2048 : 1024;
+  constexpr int W = C::W, S = C::S, BLOCK = C::BLOCK, T = W * 32;
+  // a stage: K, then V, 16 tokens each: row r, 128-byte column block c at (r / 8) * 1024 +
+  // c * 2048 + (r % 8) * 128, its 16-byte chunks in the order chunk ^ (r % 8)
+  constexpr int HS = 1024, BS = 2048;
   extern __shared__ __align__(1024) uint8_t ring[];
   float* join = reinterpret_cast<float*>(ring + C::JOIN);
   float* ml = reinterpret_cast<float*>(ring + C::ML);
   int64_t* pre = reinterpret_cast<int64_t*>(ring + C::PRE);
   int64_t* misc = reinterpret_cast<int64_t*>(ring + C::MISC);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + C::BARS);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  uint64_t* full = bars + warp * S;
   uint8_t* mine = ring + warp * S * C::STAGE;
-  if (smem_u32(ring) & 1023) {  // the swizzled tiles need it; the driver places a CTA's memory so
-    if (tid == 0) atomicOr(&g_device_error, kErrIndex);
-    return;
-  }
-  if (tid < W * S) {
-    mbar_init(bars + tid, 1);
-    fence_mbar_init();
-  }
   pdl_wait();
   pdl_trigger();
 
@@ -270,34 +256,52 @@ __global__ void __launch_bounds__(Shape<DP>::W * 32, 1)
   walk_to<BLOCK>(a, cw, runs, me, pre, gs, hi, lane);
   // ---- the producer half of each warp: the chunks of its walk, S stages ahead ---------------
   Walk pw = cw;
-  int pk = 0, pn = 0, pbase = 0;  // next block of the segment, their number, block of pid's lane 0
-  int pid0 = 0, pid1 = 0;         // lane i: pages of the chunk's first (and second) 8 tokens, block pbase + i
-  int stage_p = 0;
-  bool alive = true;              // no wait has run out
   const uint64_t policy = l2_evict_first_policy();
+  int pk = 0, pn = 0, pbase = 0;  // next block of the segment, their number, block of pid's lane 0
+  int pid0 = 0, pid1 = 0;         // lane i: pages of the chunk's first and second 8 tokens, block pbase + i,
+  int off0 = 0, off1 = 0;         // and their slots there; a negative page is not read
+  int stage_p = 0;
   auto load_pages = [&]() {
     pbase = pk;
     const int t = (pw.f + pw.k0 + pk + lane) * BLOCK + warp * 16;
     const int32_t* row = a.tables + pw.b * a.table_row;
-    auto page_of = [&](int tok) {
-      if (tok >= pw.len || tok + R <= pw.lo) return a.num_pages;
-      const int p = row[tok / a.page_size];
+    auto page_of = [&](int tok, int* off) {
+      if (tok >= pw.len || tok + 8 <= pw.lo) return -1;
+      const int at = tok / a.page_size, p = row[at];
+      *off = tok - at * a.page_size;
       if (p >= 0 && p < a.num_pages) return p;
       atomicOr(&g_device_error, kErrIndex);
-      return a.num_pages;  // outside the map: the box is filled with zeros
+      return -1;
     };
     if (pk + lane < pn) {
-      pid0 = page_of(t);
-      pid1 = R == 8 ? page_of(t + 8) : 0;
+      pid0 = page_of(t, &off0);
+      pid1 = page_of(t + 8, &off1);
     }
   };
+  // a lane copies chunk lane % CH of a row, RPI rows of the warp at a time; columns past the
+  // head's are zeros
+  constexpr int CH = DP / 8, RPI = 32 / CH, NSWZ = 8 / RPI;
+  const int ch = lane % CH, sub = lane / CH;
+  const bool col = ch * 8 < a.d;
+  const uint32_t bytes_l = col ? 16 : 0;
+  const int64_t lane_k = sub * a.k_slot + (col ? ch * 8 : 0), lane_v = sub * a.v_slot + (col ? ch * 8 : 0);
+  const int64_t k_step = RPI * a.k_slot, v_step = RPI * a.v_slot;
+  const uint16_t* k_l = a.k;  // of the segment's head
+  const uint16_t* v_l = a.v;
+  const uint32_t mine_u = smem_u32(mine), dst_l = mine_u + (ch >> 3) * BS + sub * 128;
+  uint32_t swz[NSWZ];  // of rows x + sub
+#pragma unroll
+  for (int x = 0; x < NSWZ; ++x) swz[x] = ((ch & 7) ^ (x * RPI + sub)) << 4;
   auto produce = [&]() {  // the next chunk of this warp into its next stage, if there is one
     for (;;) {
       if (pk >= pn) {
-        if (!walk_next<BLOCK>(a, pw, hi)) return;
+        if (!walk_next<BLOCK>(a, pw, hi)) break;
         pk = 0;
         pn = pw.n;
         load_pages();
+        const int head = pw.item / a.hblocks;
+        k_l = a.k + head * a.k_head + lane_k;
+        v_l = a.v + head * a.v_head + lane_v;
       } else if (pk - pbase == 32) {
         load_pages();
       }
@@ -305,30 +309,40 @@ __global__ void __launch_bounds__(Shape<DP>::W * 32, 1)
       const int sel = pk - pbase;
       ++pk;
       if (t >= pw.len || t + 16 <= pw.lo) continue;
-      const int p0 = __shfl_sync(0xFFFFFFFFu, pid0, sel), p1 = __shfl_sync(0xFFFFFFFFu, pid1, sel);
-      if (lane == 0) {
-        uint8_t* dst = mine + stage_p * C::STAGE;
-        uint64_t* bar = full + stage_p;
-        const int head = pw.item / a.hblocks;
-        mbar_arrive_expect_tx(bar, C::STAGE);
+      const uint32_t dst = dst_l + stage_p * C::STAGE;
+      const bool inside = t >= pw.lo && t + 16 <= pw.len;
 #pragma unroll
-        for (int h = 0; h < 16 / R; ++h) {
-          const int slot = (t + 8 * h) % a.page_size, page = h ? p1 : p0;
-          if (a.one_box) {
-            tma_load_5d(dst + h * HS, &kmap, 0, slot, 0, head, page, bar, policy);
-            tma_load_5d(dst + C::HALF + h * HS, &vmap, 0, slot, 0, head, page, bar, policy);
-          } else {
+      for (int h = 0; h < 2; ++h) {
+        const int page = __shfl_sync(0xFFFFFFFFu, h ? pid1 : pid0, sel), off = __shfl_sync(0xFFFFFFFFu, h ? off1 : off0, sel);
+        if (inside && page >= 0) {
+          const uint16_t* ks = k_l + page * a.k_page + off * a.k_slot;
+          const uint16_t* vs = v_l + page * a.v_page + off * a.v_slot;
 #pragma unroll
-            for (int c = 0; c < NB; ++c) {
-              tma_load_5d(dst + h * HS + c * BS, &kmap, c * 64, slot, 0, head, page, bar, policy);
-              tma_load_5d(dst + C::HALF + h * HS + c * BS, &vmap, c * 64, slot, 0, head, page, bar, policy);
-            }
+          for (int x = 0; x < 8; x += RPI) {
+            const uint32_t at = dst + h * HS + x * 128 + swz[x / RPI % NSWZ];
+            copy16(at, ks, bytes_l, policy);
+            copy16(at + C::HALF, vs, bytes_l, policy);
+            ks += k_step;
+            vs += v_step;
+          }
+        } else {
+          // tokens that are not seen are zeros: what lies there may be anything, NaN too, and a
+          // weight of 0 must meet 0
+#pragma unroll
+          for (int x = 0; x < 8; x += RPI) {
+            const int tok = t + h * 8 + x + sub;
+            const bool in = page >= 0 && tok >= pw.lo && tok < pw.len;
+            const int64_t pg = in ? page : 0, of = in ? off + x : 0;
+            const uint32_t at = dst + h * HS + x * 128 + swz[x / RPI % NSWZ];
+            copy16(at, in ? k_l + pg * a.k_page + of * a.k_slot : a.k, in ? bytes_l : 0, policy);
+            copy16(at + C::HALF, in ? v_l + pg * a.v_page + of * a.v_slot : a.v, in ? bytes_l : 0, policy);
           }
         }
       }
       stage_p = stage_p + 1 == S ? 0 : stage_p + 1;
-      return;
+      break;
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");  // one group a call, empty at the end
   };
 #pragma unroll 1
   for (int i = 0; i < S; ++i) produce();
@@ -336,8 +350,6 @@ __global__ void __launch_bounds__(Shape<DP>::W * 32, 1)
   // ---- the consumer half -------------------------------------------------------------
   const int g = lane >> 2, t4 = lane & 3;
   int stage_c = 0;
-  uint32_t phase = 0;
-  const uint32_t mine_u = smem_u32(mine);
   // ldmatrix row addresses inside a 16-token half; lane l supplies row l % 16 of an x4
   const int lr = lane & 7, lq = lane >> 3;
   bool opening = true;  // the run's first segment
@@ -365,38 +377,26 @@ __global__ void __launch_bounds__(Shape<DP>::W * 32, 1)
       const int t = (cw.f + cw.k0 + k) * BLOCK + warp * 16;
       if (t >= cw.len || t + 16 <= cw.lo) continue;
       const uint32_t kb = mine_u + stage_c * C::STAGE, vb = kb + C::HALF;
-      if (alive) alive = mbar_wait(full + stage_c, phase);
-      alive = __all_sync(0xFFFFFFFFu, alive);
-      if (alive) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
+      __syncwarp();
+      {
         const bool edge = t < cw.lo || t + 16 > cw.len;
-        if (edge) {  // values past the end may be anything, NaN too: a weight of 0 must meet 0
-          for (int r = max(0, cw.len - t); r < 16; ++r)
-            for (int c = lane; c < NB * 8; c += 32)
-              *reinterpret_cast<uint4*>(mine + stage_c * C::STAGE + C::HALF + (r >> 3) * HS + (c >> 3) * BS + (r & 7) * 128 +
-                                        (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-          for (int r = 0; r < min(16, cw.lo - t); ++r)
-            for (int c = lane; c < NB * 8; c += 32)
-              *reinterpret_cast<uint4*>(mine + stage_c * C::STAGE + C::HALF + (r >> 3) * HS + (c >> 3) * BS + (r & 7) * 128 +
-                                        (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-          __syncwarp();
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the next copy into this stage
-        }
         // scores: 16 query heads x 16 tokens
-        float s[2][4] = {};
+        float s[2][4] = {}, s_odd[2][4] = {};  // even and odd steps apart: half as long a chain
 #pragma unroll
         for (int k16 = 0; k16 < DP / 16; ++k16) {
           // matrices: tokens 0-7 / 8-15 x columns k16*16 + 0-7 / 8-15
           const int c = k16 * 2 + (lq & 1), cc = c & 7;
           uint32_t b[4];
           ldsm4(kb + (lq >> 1) * HS + (c >> 3) * BS + lr * 128 + ((cc ^ lr) << 4), b);
-          mma_16816<DT>(s[0], qf[k16], b[0], b[1]);
-          mma_16816<DT>(s[1], qf[k16], b[2], b[3]);
+          mma_16816<DT>(k16 & 1 ? s_odd[0] : s[0], qf[k16], b[0], b[1]);
+          mma_16816<DT>(k16 & 1 ? s_odd[1] : s[1], qf[k16], b[2], b[3]);
         }
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            s[n][i] *= a.s2;
+            s[n][i] = (s[n][i] + s_odd[n][i]) * a.s2;
             const int tok = t + n * 8 + t4 * 2 + (i & 1);
             if (edge && (tok < cw.lo || tok >= cw.len)) s[n][i] = -INFINITY;
           }
@@ -449,8 +449,7 @@ __global__ void __launch_bounds__(Shape<DP>::W * 32, 1)
       }
       __syncwarp();
       stage_c = stage_c + 1 == S ? 0 : stage_c + 1;
-      if (stage_c == 0) phase ^= 1;
-      if (alive) produce();
+      produce();
     }
     // ---- join the warps --------------------------------------------------------------
     l0 += __shfl_xor_sync(0xFFFFFFFFu, l0, 1);
@@ -556,56 +555,18 @@ __global__ void __launch_bounds__(Shape<DP>::W * 32, 1)
             make_uint2(pack16<DT>(acc.x * inv, acc.y * inv), pack16<DT>(acc.z * inv, acc.w * inv));
     }
   }
-  // every copy this warp issued was waited for unless a wait ran out: those left, with a limit
-  if (!alive)
-    for (int i = 0; i < S; ++i) {
-      mbar_wait(full + stage_c, phase);
-      stage_c = stage_c + 1 == S ? 0 : stage_c + 1;
-      if (stage_c == 0) phase ^= 1;
-    }
 }
 
-// The cache as [pages][heads][column blocks][slots][64], or, where the head is no multiple
-// of 64 wide, [pages][heads][1][slots][d] with boxes that reach past d (filled with zeros).
-bool make_cache_map(CUtensorMap* map, const void* base, int64_t dtype, const ggufmm_attention_args& p, int64_t page,
-                    int64_t head, int64_t slot, int rows, bool one_box) {
-  PFN_encodeTiled enc = get_encode_fn();
-  if (!enc) return false;
-  const cuuint64_t d = static_cast<cuuint64_t>(p.head_dim), cols = one_box ? d / 64 : 1;
-  cuuint64_t dims[5] = {one_box ? 64 : d, static_cast<cuuint64_t>(p.page_size), cols,
-                        static_cast<cuuint64_t>(p.kv_heads), static_cast<cuuint64_t>(p.num_pages)};
-  cuuint64_t strides[4] = {static_cast<cuuint64_t>(slot) * 2, 128, static_cast<cuuint64_t>(head) * 2,
-                           static_cast<cuuint64_t>(page) * 2};
-  cuuint32_t box[5] = {64, static_cast<cuuint32_t>(rows), static_cast<cuuint32_t>(cols), 1, 1};
-  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
-  return enc(map, dtype == GGUFMM_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
-             const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-template <int DP, int DT, int R>
-cudaError_t launch(const ggufmm_attention_args& p, DecodeArgs& a, int grid, int dev, cudaStream_t st) {
-  CUtensorMap km, vm;
-  if (!make_cache_map(&km, p.k, p.dtype, p, p.k_page, p.k_head, p.k_slot, R, a.one_box) ||
-      !make_cache_map(&vm, p.v, p.dtype, p, p.v_page, p.v_head, p.v_slot, R, a.one_box))
-    return cudaErrorInvalidValue;
-  auto fn = paged_decode_kernel<DP, DT, R>;
+template <int DP, int DT>
+cudaError_t launch(const DecodeArgs& a, int grid, int dev, cudaStream_t st) {
+  auto fn = paged_decode_kernel<DP, DT>;
   static std::atomic<uint64_t> ready{0};  // devices whose shared-memory limit is raised
   if (!(ready.load(std::memory_order_acquire) >> (dev & 63) & 1)) {
     const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<DP>::SMEM);
     if (e != cudaSuccess) return e;
     ready.fetch_or(uint64_t(1) << (dev & 63), std::memory_order_release);
   }
-  return pdl_launch(fn, dim3(static_cast<unsigned>(grid)), dim3(Shape<DP>::W * 32), Shape<DP>::SMEM, st, km, vm, a);
-}
-
-template <int DP>
-cudaError_t launch_dp(const ggufmm_attention_args& p, DecodeArgs& a, int grid, int dev, cudaStream_t st) {
-  const bool f16 = p.dtype == GGUFMM_F16;
-  if (p.page_size % 16 == 0)
-    return f16 ? launch<DP, GGUFMM_F16, 16>(p, a, grid, dev, st) : launch<DP, GGUFMM_BF16, 16>(p, a, grid, dev, st);
-  return f16 ? launch<DP, GGUFMM_F16, 8>(p, a, grid, dev, st) : launch<DP, GGUFMM_BF16, 8>(p, a, grid, dev, st);
+  return pdl_launch(fn, dim3(static_cast<unsigned>(grid)), dim3(Shape<DP>::W * 32), Shape<DP>::SMEM, st, a);
 }
 
 int padded_dim(int64_t d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
@@ -624,6 +585,14 @@ cudaError_t launch_paged_decode(const ggufmm_attention_args& p, void* workspace,
   DecodeArgs a;
   a.q = p.q;
   a.out = p.out;
+  a.k = static_cast<const uint16_t*>(p.k);
+  a.v = static_cast<const uint16_t*>(p.v);
+  a.k_page = p.k_page;
+  a.k_head = p.k_head;
+  a.k_slot = p.k_slot;
+  a.v_page = p.v_page;
+  a.v_head = p.v_head;
+  a.v_slot = p.v_slot;
   a.tables = static_cast<const int32_t*>(p.tables);
   a.lens = static_cast<const int32_t*>(p.lens);
   a.count = static_cast<uint32_t*>(workspace);
@@ -644,16 +613,15 @@ cudaError_t launch_paged_decode(const ggufmm_attention_args& p, void* workspace,
   a.page_size = static_cast<int>(p.page_size);
   a.num_pages = static_cast<int>(p.num_pages);
   a.window = static_cast<int>(p.window);
-  a.one_box = a.d % 64 == 0 && a.d == padded_dim(a.d);
   a.s2 = static_cast<float>(p.scale * 1.4426950408889634);
+  const bool f16 = p.dtype == GGUFMM_F16;
   switch (padded_dim(p.head_dim)) {
-    case 64: return launch_dp<64>(p, a, grid, dev, st);
-    case 128: return launch_dp<128>(p, a, grid, dev, st);
-    default: return launch_dp<256>(p, a, grid, dev, st);
+    case 64: return f16 ? launch<64, GGUFMM_F16>(a, grid, dev, st) : launch<64, GGUFMM_BF16>(a, grid, dev, st);
+    case 128: return f16 ? launch<128, GGUFMM_F16>(a, grid, dev, st) : launch<128, GGUFMM_BF16>(a, grid, dev, st);
+    default: return f16 ? launch<256, GGUFMM_F16>(a, grid, dev, st) : launch<256, GGUFMM_BF16>(a, grid, dev, st);
   }
 }
 
 cudaError_t attn_decode_device_error(int* v, int clear, cudaStream_t st) { return tu_device_error(v, clear, st); }
-cudaError_t attn_decode_set_wait_limit(uint32_t polls) { return tu_set_wait_limit(polls); }
 
 }  // namespace ggufmm

@@ -45,7 +45,6 @@ cudaError_t dequant_device_error(int* v, int clear, cudaStream_t st);
 cudaError_t rope_device_error(int* v, int clear, cudaStream_t st);
 cudaError_t attn_prompt_device_error(int* v, int clear, cudaStream_t st);
 cudaError_t attn_decode_device_error(int* v, int clear, cudaStream_t st);
-cudaError_t attn_decode_set_wait_limit(uint32_t polls);
 cudaError_t attn_prompt_set_wait_limit(uint32_t polls);
 cudaError_t launch_embedding(const void* q, int qtype, int64_t n_vocab, int64_t k, const int32_t* ids, int64_t n_ids,
                              void* out, int out_dtype, int64_t ldo, cudaStream_t st);
@@ -214,7 +213,6 @@ int ggufmm_set_wait_limit(uint32_t polls) {
   if (e == cudaSuccess) e = gemm_fused_set_wait_limit(v);
   if (e == cudaSuccess) e = gemv_i8_set_wait_limit(v);
   if (e == cudaSuccess) e = allreduce_set_wait_limit(v);
-  if (e == cudaSuccess) e = attn_decode_set_wait_limit(v);
   if (e == cudaSuccess) e = attn_prompt_set_wait_limit(v);
   return cuda_status(e);
 }
