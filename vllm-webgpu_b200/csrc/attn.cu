@@ -57,6 +57,9 @@ extern "C" int ggufmm_paged_attention(const ggufmm_attention_args* args, void* w
   p.q_starts = nullptr;
   int s = check_attention(p, false);
   if (s || p.batch == 0) return s;
+  // the kernel counts blocks of at least 64 tokens of every (sequence, kv head, 16 query heads)
+  if (p.batch * p.kv_heads * ((p.q_heads / p.kv_heads + 15) / 16) > kI32Max / (p.table_width * p.page_size / 64 + 3))
+    return GGUFMM_ERR_SHAPE;
   if (!workspace || workspace_bytes < ggufmm_paged_attention_workspace_size(p.batch, p.q_heads, p.kv_heads, p.head_dim))
     return GGUFMM_ERR_WORKSPACE;
   if (!aligned_to(workspace, 256)) return GGUFMM_ERR_ALIGN;

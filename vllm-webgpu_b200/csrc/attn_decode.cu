@@ -10,9 +10,10 @@
 // and the time is the cache's bytes over the HBM rate.
 //
 // Split: the work is the list of all (sequence, kv head) items, cut into blocks of W * 16
-// tokens. Every CTA (one per SM) takes an equal run of consecutive blocks, whatever
-// sequences they belong to, so ragged lengths leave no SM idle; it finds its run by a sum
-// over the lengths on the device. An item inside one run is written directly. An item that
+// tokens; an item counts as one block more, for what it costs to begin and to end one. Every
+// CTA (one per SM) takes an equal run of consecutive blocks, whatever sequences they belong
+// to, so ragged lengths leave no SM idle; it finds its run by a sum over the lengths on the
+// device. An item inside one run is written directly. An item that
 // crosses runs leaves fp32 partials (m, sum, o) in the workspace, and the last of its CTAs
 // to finish (a counter) adds them in the order of the CTAs, so the result does not depend
 // on which was last. (Handing part of the work out in short runs as CTAs finish was measured:
@@ -42,7 +43,6 @@ DevInfo device_info(int dev);  // capi.cu
 namespace {
 
 constexpr int kMaxGrid = 160;               // CTAs a workspace has room for
-constexpr int kMinRun = 1;                  // blocks of a run at least
 constexpr size_t kCounterBytes = 1024;      // one arrival counter per CTA
 static_assert(kMaxGrid * 4 <= kCounterBytes, "counters");
 
@@ -57,8 +57,8 @@ struct Shape {
   static constexpr int JOIN = RING;                 // 8 rows of every warp's sums
   static constexpr int ML = JOIN + W * 8 * DP * 4;  // [W][16][2] every warp's max and sum per row
   static constexpr int PRE = ML + W * 128;          // [128] blocks per item before each group of sequences
-  static constexpr int MISC = PRE + 1024;           // [8] scan scratch
-  static constexpr int SMEM = MISC + 64;
+  static constexpr int MISC = PRE + 512;            // [8] scan scratch
+  static constexpr int SMEM = MISC + 32;
   static_assert(SMEM <= 232448, "a CTA's shared memory");
 };
 
@@ -80,29 +80,21 @@ struct DecodeArgs {
   float s2;         // scale * log2(e)
 };
 
-// x / y for whole numbers whose quotient is below 2^22, by way of 32-bit floats: a 64-bit
-// division is some 150 clocks, and every CTA goes through a few before it can load anything.
-__device__ __forceinline__ int64_t small_quotient(int64_t x, int64_t y) {
-  int64_t q = static_cast<int64_t>(__fdividef(static_cast<float>(x), static_cast<float>(y)));
-  while (q * y > x) --q;
-  while ((q + 1) * y <= x) ++q;
-  return q;
-}
-
-// The work list cut into runs, the first `extra` of them one block longer than `size`.
+// The work list cut into runs, the first `extra` of them one block longer than `size`. (The
+// host refuses lists of 2^31 blocks and more.)
 struct Runs {
-  int64_t size, extra;
-  __device__ __forceinline__ int64_t begin(int r) const { return r * size + min(static_cast<int64_t>(r), extra); }
-  __device__ __forceinline__ int holding(int64_t block) const {  // the run of a block
-    const int64_t longer = extra * (size + 1);
-    return static_cast<int>(block < longer ? small_quotient(block, size + 1)
-                                           : extra + small_quotient(block - longer, size));
+  int size, extra;
+  __device__ __forceinline__ int begin(int r) const { return r * size + min(r, extra); }
+  __device__ __forceinline__ int holding(int block) const {  // the run of a block
+    const int longer = extra * (size + 1);
+    return block < longer ? block / (size + 1) : extra + (block - longer) / size;
   }
 };
 
-// A walk over the blocks of a run: where the current item's blocks lie.
+// A walk over the blocks of a run: where the current item's blocks lie. An item has nb blocks
+// of tokens, then one that stands for its own cost.
 struct Walk {
-  int64_t left, base;    // blocks of the run to come, first block of the current sequence
+  int left, base;        // blocks of the run to come, first block of the current sequence
   int b, nb, f, len, lo; // sequence: index, blocks per item, first block's index, length, first visible token
   int item, k0, n;       // current segment: item within the sequence, its first block and their number
   bool starts, ends;     // whether the segment holds the item's first / last block
@@ -131,34 +123,35 @@ __device__ __forceinline__ void walk_load(const DecodeArgs& a, Walk& w) {
 // The next segment of the run; false at its end.
 template <int BLOCK>
 __device__ __forceinline__ bool walk_next(const DecodeArgs& a, Walk& w, int hi) {
-  if (w.left <= 0) return false;
   w.k0 += w.n;
-  if (w.k0 >= w.nb) {
+  for (;;) {
+    if (w.left <= 0) return false;
+    if (w.k0 < w.nb) break;
+    // past the item's last block
+    if (w.nb > 0) --w.left;
     w.k0 = 0;
-    if (++w.item >= hi) {
+    if (w.nb == 0 || ++w.item >= hi) {
       w.item = 0;
-      do {
-        w.base += static_cast<int64_t>(w.nb) * hi;
-        if (++w.b >= a.batch) {  // only if the lengths changed under the kernel
-          w.left = 0;
-          return false;
-        }
-        walk_load<BLOCK>(a, w);
-      } while (w.nb == 0);
+      w.base += (w.nb ? w.nb + 1 : 0) * hi;
+      if (++w.b >= a.batch) {  // the end, or the lengths changed under the kernel
+        w.left = 0;
+        return false;
+      }
+      walk_load<BLOCK>(a, w);
     }
   }
-  w.n = static_cast<int>(min(static_cast<int64_t>(w.nb - w.k0), w.left));
+  w.n = min(w.nb - w.k0, w.left);
   w.starts = w.k0 == 0;
   w.ends = w.k0 + w.n == w.nb;
   w.left -= w.n;
   return true;
 }
 
-// To the first block of run r: the group of sequences that holds it, by all lanes of a warp.
+// To block 0 of run r: the group of sequences that holds it, by all lanes of a warp.
 template <int BLOCK>
-__device__ __forceinline__ void walk_to(const DecodeArgs& a, Walk& w, const Runs& runs, int r, const int64_t* pre, int gs,
+__device__ __forceinline__ void walk_to(const DecodeArgs& a, Walk& w, const Runs& runs, int r, const int* pre, int gs,
                                         int hi, int lane) {
-  const int64_t u = runs.begin(r);
+  const int u = runs.begin(r);
   w.left = runs.begin(r + 1) - u;
   int g = -1;
 #pragma unroll
@@ -167,14 +160,13 @@ __device__ __forceinline__ void walk_to(const DecodeArgs& a, Walk& w, const Runs
   w.b = min(g * gs, a.batch - 1);
   w.base = pre[g] * hi;
   walk_load<BLOCK>(a, w);
-  while (u >= w.base + static_cast<int64_t>(w.nb) * hi && w.b + 1 < a.batch) {
-    w.base += static_cast<int64_t>(w.nb) * hi;
+  while (w.b + 1 < a.batch && (w.nb == 0 || u >= w.base + (w.nb + 1) * hi)) {
+    w.base += (w.nb ? w.nb + 1 : 0) * hi;
     ++w.b;
     walk_load<BLOCK>(a, w);
   }
-  const int64_t off = u - w.base;
-  w.item = w.nb ? static_cast<int>(small_quotient(off, w.nb)) : 0;
-  w.k0 = static_cast<int>(off - static_cast<int64_t>(w.item) * w.nb);
+  w.item = (u - w.base) / (w.nb + 1);
+  w.k0 = u - w.base - w.item * (w.nb + 1);
   w.n = 0;  // the first segment starts here
 }
 
@@ -200,8 +192,8 @@ __global__ void __launch_bounds__(Shape<DP>::W * 32, 1) paged_decode_kernel(cons
   extern __shared__ __align__(1024) uint8_t ring[];
   float* join = reinterpret_cast<float*>(ring + C::JOIN);
   float* ml = reinterpret_cast<float*>(ring + C::ML);
-  int64_t* pre = reinterpret_cast<int64_t*>(ring + C::PRE);
-  int64_t* misc = reinterpret_cast<int64_t*>(ring + C::MISC);
+  int* pre = reinterpret_cast<int*>(ring + C::PRE);
+  int* misc = reinterpret_cast<int*>(ring + C::MISC);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint8_t* mine = ring + warp * S * C::STAGE;
   pdl_wait();
@@ -210,36 +202,37 @@ __global__ void __launch_bounds__(Shape<DP>::W * 32, 1) paged_decode_kernel(cons
   // ---- the work: blocks per item before each of 128 groups of sequences ----------------
   const int hi = a.hkv * a.hblocks;  // items per sequence
   const int gs = (a.batch + 127) / 128;
-  int64_t mine_b = 0, inc;
+  int mine_b = 0, inc;
   if (tid < 128) {
     for (int b = tid * gs; b < min((tid + 1) * gs, a.batch); ++b) {
       int lo;
       bool cut;
       const int len = seq_len(a, b, &cut);
       if (cut && blockIdx.x == 0) atomicOr(&g_device_error, kErrIndex);
-      mine_b += seq_blocks<BLOCK>(a, len, &lo);
+      const int nb = seq_blocks<BLOCK>(a, len, &lo);
+      mine_b += nb ? nb + 1 : 0;
     }
     inc = mine_b;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+      const int v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
       if (lane >= o) inc += v;
     }
     if (lane == 31) misc[warp] = inc;
   }
   __syncthreads();
-  int64_t total = 0;
+  int total = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if (tid < 128 && i == warp) pre[tid] = total + inc - mine_b;
     total += misc[i];
   }
   __syncthreads();
-  const int64_t blocks = total * hi;
+  const int blocks = total * hi;
   const int me = static_cast<int>(blockIdx.x);
-  const int nruns = static_cast<int>(min(static_cast<int64_t>(gridDim.x), (blocks + kMinRun - 1) / kMinRun));
+  const int nruns = min(static_cast<int>(gridDim.x), blocks);
   Runs runs;
-  runs.size = nruns == 0 ? 0 : blocks < (int64_t(1) << 22) ? small_quotient(blocks, nruns) : blocks / nruns;
+  runs.size = nruns ? blocks / nruns : 0;
   runs.extra = blocks - runs.size * nruns;
   // sequences that see nothing: zeros
   for (int b = me; b < a.batch; b += gridDim.x) {
@@ -352,7 +345,6 @@ __global__ void __launch_bounds__(Shape<DP>::W * 32, 1) paged_decode_kernel(cons
   int stage_c = 0;
   // ldmatrix row addresses inside a 16-token half; lane l supplies row l % 16 of an x4
   const int lr = lane & 7, lq = lane >> 3;
-  bool opening = true;  // the run's first segment
   while (walk_next<BLOCK>(a, cw, hi)) {
     const int head = cw.item / a.hblocks, hb = cw.item % a.hblocks;
     const int rows = min(a.group - hb * 16, 16);
@@ -461,8 +453,9 @@ __global__ void __launch_bounds__(Shape<DP>::W * 32, 1) paged_decode_kernel(cons
       *reinterpret_cast<float2*>(ml + (warp * 16 + g + 8) * 2) = make_float2(m1, l1);
     }
     const bool whole = cw.starts && cw.ends;
-    const int64_t item0 = cw.base + static_cast<int64_t>(cw.item) * cw.nb;  // first block of the item
-    const int slot = me * 2 + (opening ? 0 : 1);
+    const int item0 = cw.base + cw.item * (cw.nb + 1);  // first block of the item
+    // a run has at most one piece of an item begun before it, and one of an item that goes on after it
+    const int slot = me * 2 + (cw.starts ? 1 : 0);
     float* const part_ml = a.part + a.slots * a.prows * DP;
     uint16_t* outp = static_cast<uint16_t*>(a.out) + cw.b * a.o_row + qh0 * a.o_head;
 #pragma unroll 1
@@ -507,7 +500,6 @@ __global__ void __launch_bounds__(Shape<DP>::W * 32, 1) paged_decode_kernel(cons
       }
       __syncthreads();
     }
-    opening = false;
     if (whole) continue;
     // ---- join the CTAs of this item: the last one to arrive adds the partials ---------------
     const int c0 = cw.starts ? me : runs.holding(item0), c1 = cw.ends ? me : runs.holding(item0 + cw.nb - 1);
@@ -517,7 +509,6 @@ __global__ void __launch_bounds__(Shape<DP>::W * 32, 1) paged_decode_kernel(cons
     __syncthreads();  // misc[7] is written again at the next item
     if (!last) continue;
     if (tid == 0) a.count[c0] = 0;
-    const int64_t slot0 = static_cast<int64_t>(c0) * 2 + (item0 == runs.begin(c0) ? 0 : 1);
     for (int e = tid; e < rows * (DP / 4); e += T) {
       const int row = e / (DP / 4), c = e % (DP / 4) * 4;
       float mr = -INFINITY, l = 0.f;
@@ -529,7 +520,7 @@ __global__ void __launch_bounds__(Shape<DP>::W * 32, 1) paged_decode_kernel(cons
         float mk = mr;
 #pragma unroll
         for (int x = 0; x < K; ++x) {
-          const int64_t at = (k + x == c0 ? slot0 : 2 * static_cast<int64_t>(k + x)) * a.prows + row;
+          const int64_t at = (2 * static_cast<int64_t>(k + x) + (k + x == c0)) * a.prows + row;
           w[x] = k + x <= c1 ? __ldcg(reinterpret_cast<const float2*>(part_ml + at * 2)) : make_float2(-INFINITY, 0.f);
           v[x] = k + x <= c1 ? __ldcg(reinterpret_cast<const float4*>(a.part + at * DP + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
