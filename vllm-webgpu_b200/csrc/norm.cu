@@ -163,11 +163,49 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) rms_norm_vec_kernel(const _
   }
 }
 
-// Any width and alignment: one row per CTA, a value at a time, E of them held by a thread.
-// E == 0: wider rows, read twice (each value again by the thread that read it first, so
-// that y may be x and ro may be r).
-template <int E>
-__global__ void __launch_bounds__(E == 0 ? 1024 : 512) rms_norm_any_kernel(const __grid_constant__ NormArgs a) {
+// Any width and alignment: one row per CTA, value by value, E of them held by a thread (raw
+// first, as above). XS, RS: bytes of a value of x and of r (0: none).
+template <int E, int XS, int RS>
+__global__ void __launch_bounds__(512) rms_norm_any_kernel(const __grid_constant__ NormArgs a) {
+  __shared__ float part[32];
+  pdl_wait();
+  pdl_trigger();
+  const int64_t row = blockIdx.x;
+  auto raw = [](const void* p, int es, int64_t i) -> uint32_t {
+    return es == 4 ? static_cast<const uint32_t*>(p)[i] : static_cast<const uint16_t*>(p)[i];
+  };
+  auto value = [](uint32_t u, int t) {
+    return t == GGUFMM_F16 ? half_bits_to_float(u) : __uint_as_float(t == GGUFMM_BF16 ? u << 16 : u);
+  };
+  uint32_t x[E], r[E];
+#pragma unroll
+  for (int k = 0; k < E; ++k) {
+    const int i = threadIdx.x + k * blockDim.x;
+    x[k] = i < a.n ? raw(a.x, XS, row * a.ldx + i) : 0u;
+    if (RS) r[k] = i < a.n ? raw(a.r, RS, row * a.ldr + i) : 0u;
+  }
+  float s[E], ss = 0.f;
+#pragma unroll
+  for (int k = 0; k < E; ++k) {
+    s[k] = value(x[k], a.xt);
+    if (RS) s[k] += value(r[k], a.rt);
+    ss = fmaf(s[k], s[k], ss);
+  }
+  const float inv = rsqrtf(fmaf(cta_sum(ss, part), a.inv_n, a.eps));
+#pragma unroll
+  for (int k = 0; k < E; ++k) {
+    const int i = threadIdx.x + k * blockDim.x;
+    if (i >= a.n) break;
+    if (RS && a.ro) store_y_rt(a.ro, a.rt, row * a.ldro + i, s[k]);
+    float v = s[k] * inv;
+    if (a.w) v *= load_y_rt(a.w, a.wt, i) + a.c;
+    store_y_rt(a.y, a.yt, row * a.ldy + i, v);
+  }
+}
+
+// Wider rows yet: read twice, each value again by the thread that read it first (so that y may
+// be x and ro may be r).
+__global__ void __launch_bounds__(1024) rms_norm_wide_kernel(const __grid_constant__ NormArgs a) {
   __shared__ float part[32];
   pdl_wait();
   pdl_trigger();
@@ -177,37 +215,28 @@ __global__ void __launch_bounds__(E == 0 ? 1024 : 512) rms_norm_any_kernel(const
     if (a.r) v += load_y_rt(a.r, a.rt, row * a.ldr + i);
     return v;
   };
-  auto finish = [&](int i, float v, float inv) {
+  float ss = 0.f;
+  for (int i = threadIdx.x; i < a.n; i += blockDim.x) {
+    const float v = sum_at(i);
+    ss = fmaf(v, v, ss);
+  }
+  const float inv = rsqrtf(fmaf(cta_sum(ss, part), a.inv_n, a.eps));
+  for (int i = threadIdx.x; i < a.n; i += blockDim.x) {
+    float v = sum_at(i);
     if (a.ro) store_y_rt(a.ro, a.rt, row * a.ldro + i, v);
     v *= inv;
     if (a.w) v *= load_y_rt(a.w, a.wt, i) + a.c;
     store_y_rt(a.y, a.yt, row * a.ldy + i, v);
-  };
-  float s[E ? E : 1], ss = 0.f;
-  if constexpr (E != 0) {
-#pragma unroll
-    for (int k = 0; k < E; ++k) {
-      const int i = threadIdx.x + k * blockDim.x;
-      s[k] = i < a.n ? sum_at(i) : 0.f;
-    }
-#pragma unroll
-    for (int k = 0; k < E; ++k) ss = fmaf(s[k], s[k], ss);
-  } else {
-    for (int i = threadIdx.x; i < a.n; i += blockDim.x) {
-      const float v = sum_at(i);
-      ss = fmaf(v, v, ss);
-    }
   }
-  const float inv = rsqrtf(fmaf(cta_sum(ss, part), a.inv_n, a.eps));
-  if constexpr (E != 0) {
-#pragma unroll
-    for (int k = 0; k < E; ++k) {
-      const int i = threadIdx.x + k * blockDim.x;
-      if (i < a.n) finish(i, s[k], inv);
-    }
-  } else {
-    for (int i = threadIdx.x; i < a.n; i += blockDim.x) finish(i, sum_at(i), inv);
-  }
+}
+
+template <int XS, int RS>
+cudaError_t launch_any(const NormArgs& a, cudaStream_t st) {
+  const dim3 grid(static_cast<unsigned>(a.m));
+  auto block = [&](int e) { return dim3(static_cast<unsigned>((((a.n + e - 1) / e) + 31) / 32 * 32)); };
+  if (a.n <= 4096) return pdl_launch(rms_norm_any_kernel<8, XS, RS>, grid, block(8), 0, st, a);
+  if (a.n <= 8192) return pdl_launch(rms_norm_any_kernel<16, XS, RS>, grid, block(16), 0, st, a);
+  return pdl_launch(rms_norm_wide_kernel, grid, dim3(1024), 0, st, a);
 }
 
 template <int XS, int RS>
@@ -235,11 +264,10 @@ cudaError_t launch_norm(const NormArgs& a, cudaStream_t st) {
     if (a.rt == GGUFMM_F32) return x4 ? launch_vec<4, 4>(a, st) : launch_vec<2, 4>(a, st);
     return x4 ? launch_vec<4, 2>(a, st) : launch_vec<2, 2>(a, st);
   }
-  const dim3 grid(static_cast<unsigned>(a.m));
-  auto block = [&](int e) { return dim3(static_cast<unsigned>((((a.n + e - 1) / e) + 31) / 32 * 32)); };
-  if (a.n <= 1024) return pdl_launch(rms_norm_any_kernel<4>, grid, block(4), 0, st, a);
-  if (a.n <= 8192) return pdl_launch(rms_norm_any_kernel<16>, grid, block(16), 0, st, a);
-  return pdl_launch(rms_norm_any_kernel<0>, grid, dim3(1024), 0, st, a);
+  const bool x4 = a.xt == GGUFMM_F32;
+  if (!a.r) return x4 ? launch_any<4, 0>(a, st) : launch_any<2, 0>(a, st);
+  if (a.rt == GGUFMM_F32) return x4 ? launch_any<4, 4>(a, st) : launch_any<2, 4>(a, st);
+  return x4 ? launch_any<4, 2>(a, st) : launch_any<2, 2>(a, st);
 }
 
 int elem(int dtype) { return dtype == GGUFMM_F32 ? 4 : dtype == GGUFMM_F16 || dtype == GGUFMM_BF16 ? 2 : 0; }

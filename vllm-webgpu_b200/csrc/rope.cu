@@ -11,7 +11,8 @@
 // product with the position, reduced modulo one turn by the integer's own overflow, is
 // exact for every position: an fp32 product of a position near 10^6 and a frequency
 // would be off by hundredths of a radian.
-#include <initializer_list>
+#include <algorithm>
+#include <type_traits>
 
 #include "mma16.cuh"
 #include "paged.cuh"
@@ -22,7 +23,6 @@ namespace {
 
 struct RopeArgs {
   ggufmm_rope_args p;
-  int per_cta;  // tokens of a CTA
 };
 
 __device__ __forceinline__ float2 turn(int64_t pos, int64_t step, float factor) {
@@ -34,9 +34,9 @@ __device__ __forceinline__ float2 turn(int64_t pos, int64_t step, float factor) 
   return make_float2(c * factor, s * factor);
 }
 
-// N consecutive values as they lie in memory (16-byte aligned where N * ES is).
+// N consecutive values as they lie in memory, aligned to 16 bytes or to all of them.
 template <int ES, int N>
-struct Vals {
+struct alignas(N * ES >= 16 ? 16 : N * ES >= 8 ? 8 : 4) Vals {
   uint32_t u[N * ES >= 4 ? N * ES / 4 : 1];
 };
 
@@ -45,6 +45,8 @@ __device__ __forceinline__ void load_vals(Vals<ES, N>& d, const void* p, int64_t
   const uint8_t* q = static_cast<const uint8_t*>(p) + i * ES;
   if constexpr (N == 1) {
     d.u[0] = ES == 4 ? *reinterpret_cast<const uint32_t*>(q) : *reinterpret_cast<const uint16_t*>(q);
+  } else if constexpr (N * ES == 8) {
+    *reinterpret_cast<uint2*>(d.u) = *reinterpret_cast<const uint2*>(q);
   } else {
 #pragma unroll
     for (int k = 0; k < N * ES / 16; ++k) reinterpret_cast<uint4*>(d.u)[k] = reinterpret_cast<const uint4*>(q)[k];
@@ -70,6 +72,10 @@ __device__ __forceinline__ void store_vals(void* p, int dt, int64_t i, const flo
 #pragma unroll
     for (int k = 0; k < N / 4; ++k)
       reinterpret_cast<float4*>(static_cast<float*>(p) + i)[k] = make_float4(f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]);
+  } else if constexpr (N == 4) {
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) =
+        dt == GGUFMM_F16 ? make_uint2(pack16<GGUFMM_F16>(f[0], f[1]), pack16<GGUFMM_F16>(f[2], f[3]))
+                         : make_uint2(pack16<GGUFMM_BF16>(f[0], f[1]), pack16<GGUFMM_BF16>(f[2], f[3]));
   } else {
 #pragma unroll
     for (int k = 0; k < N / 8; ++k) {
@@ -84,95 +90,102 @@ __device__ __forceinline__ void store_vals(void* p, int dt, int64_t i, const flo
   }
 }
 
-// A CTA takes per_cta tokens: it makes their sines and cosines once, in shared memory, for
-// all heads, then runs over the units of q, k and v: N pairs (2 N values) that turn, or 2 N
-// values that pass. N is 8, where whole 16-byte groups allow it, or 1.
-template <int XT, int N>
-__global__ void __launch_bounds__(256) rope_append_kernel(const __grid_constant__ RopeArgs a) {
-  extern __shared__ float2 table[];  // [per_cta][half]
+// A CTA takes TB tokens: it makes their sines and cosines once, in shared memory, for all
+// heads, then runs over the units of q, k and v: N pairs (2 N values) that turn, or 2 N values
+// that pass. A thread has the same unit of all TB tokens, so that several loads are under way at
+// a time and the unit's place is found once; the first ones go out before the sines are made. N is
+// 8 or 4, where the widths and strides allow whole groups of 16 (8) bytes, or 1.
+// HBM bound: 8192 tokens of 32 / 8 heads of 128 (201 MB) in 35 us, 5.7 TB/s, 89% of the measured
+// copy rate, with two tokens and 128 threads a CTA; 256 threads 45 us (their waits coincide), four
+// tokens 36 us, sines before loads 47 us. A few tokens take 3 us, a launch and two memory latencies.
+template <int XT, int N, int TB, int NT>
+__global__ void __launch_bounds__(NT) rope_append_kernel(const __grid_constant__ RopeArgs a) {
+  extern __shared__ float2 table[];  // [TB][half]
+  __shared__ int64_t place[2][TB];   // where a token's k and v go, negative for nowhere
   constexpr int ES = XT == GGUFMM_F32 ? 4 : 2;
   pdl_wait();
   pdl_trigger();
   const ggufmm_rope_args& p = a.p;
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.per_cta;
-  const int nt = static_cast<int>(min(static_cast<int64_t>(a.per_cta), p.tokens - t0));
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * TB;
+  const int nt = static_cast<int>(min(static_cast<int64_t>(TB), p.tokens - t0));
   const int d = static_cast<int>(p.head_dim), half = static_cast<int>(p.rot_dim) / 2;
   const int hq = static_cast<int>(p.q_heads), hkv = p.k ? static_cast<int>(p.kv_heads) : 0;
-  const int ct = static_cast<int>(p.cache_dtype);
-  const int64_t* positions = static_cast<const int64_t*>(p.positions) + t0;
-  for (int i = threadIdx.x; i < nt * half; i += 256)
-    table[i] = turn(positions[i / half], static_cast<const int64_t*>(p.steps)[i % half], static_cast<float>(p.factor));
-  __syncthreads();
   // units of a head that turns: pairs first, then what passes; a head of v passes whole
   const int ut = half / N, uh = ut + (d - 2 * half) / (2 * N), uv = d / (2 * N);
   const int turning = (hq + hkv) * uh, per = turning + hkv * uv;
-  for (int i = threadIdx.x; i < nt * per; i += 256) {
-    const int t = i / per, j = i - t * per;
+  for (int j0 = 0; j0 < per; j0 += NT) {
+    const int j = min(j0 + static_cast<int>(threadIdx.x), per - 1);
+    const int rows = j0 + static_cast<int>(threadIdx.x) < per ? nt : 0;  // 0: past the last unit
     const bool isv = j >= turning;
     int h = isv ? (j - turning) / uv : j / uh;
     const int u = isv ? (j - turning) - h * uv : j - h * uh;
-    const bool isk = !isv && h >= hq;
+    const bool isk = !isv && h >= hq, cached = isk || isv;
     if (isk) h -= hq;
-    const void* src;
-    void* dst;
-    int64_t in, out;
-    int dt;
-    if (!isk && !isv) {
-      src = p.q;
-      dst = p.q_out;
-      dt = static_cast<int>(p.q_out_dtype);
-      in = (t0 + t) * p.q_row + h * p.q_head;
-      out = (t0 + t) * p.qo_row + h * p.qo_head;
-    } else {
-      const int64_t slot = static_cast<const int64_t*>(p.slots)[t0 + t];
-      if (slot < 0) continue;
-      const int64_t page = slot / p.page_size, off = slot - page * p.page_size;
-      if (page >= p.num_pages) {
-        atomicOr(&g_device_error, kErrIndex);
-        continue;
-      }
-      dt = ct;
-      src = isk ? p.k : p.v;
-      dst = isk ? p.k_cache : p.v_cache;
-      in = (t0 + t) * (isk ? p.k_row : p.v_row) + h * (isk ? p.k_head : p.v_head);
-      out = isk ? page * p.kc_page + h * p.kc_head + off * p.kc_slot : page * p.vc_page + h * p.vc_head + off * p.vc_slot;
-    }
-    if (isv || u >= ut) {
-      const int e = isv ? u * 2 * N : 2 * half + (u - ut) * 2 * N;
-      Vals<ES, N> x, y;
-      load_vals(x, src, in + e);
-      load_vals(y, src, in + e + N);
-      float f[2 * N];
-      to_float<XT>(x, f);
-      to_float<XT>(y, f + N);
-      store_vals<N>(dst, dt, out + e, f);
-      store_vals<N>(dst, dt, out + e + N, f + N);
-      continue;
-    }
-    const float2* cs = table + t * half + u * N;
-    const int e0 = p.interleaved ? u * 2 * N : u * N, e1 = p.interleaved ? e0 + N : e0 + half;
-    Vals<ES, N> x, y;
-    load_vals(x, src, in + e0);
-    load_vals(y, src, in + e1);
-    float f[2 * N], g[2 * N];
-    to_float<XT>(x, f);
-    to_float<XT>(y, f + N);
+    const bool turns = !isv && u < ut;
+    // two groups of N values, each in a row with those of the lanes beside: the halves of what
+    // turns (in either order of pairs), of what passes, of a head of v; N == 1 and interleaved: a pair
+    const bool apart = !(N == 1 && turns && p.interleaved);
+    const int first = isv || turns ? 0 : 2 * half, span = isv ? d / 2 : turns ? half : d / 2 - half;
+    const int e0 = first + (apart ? (turns || isv ? u : u - ut) * N : 2 * u), e1 = apart ? e0 + span : e0 + 1;
+    const void* src = isv ? p.v : isk ? p.k : p.q;
+    const int64_t in_row = isv ? p.v_row : isk ? p.k_row : p.q_row;
+    const int64_t in = t0 * in_row + h * (isv ? p.v_head : isk ? p.k_head : p.q_head);
+    void* dst = isv ? p.v_cache : isk ? p.k_cache : p.q_out;
+    const int dt = static_cast<int>(cached ? p.cache_dtype : p.q_out_dtype);
+    const int64_t out_head = h * (isv ? p.vc_head : isk ? p.kc_head : p.qo_head);
+    Vals<ES, N> x[TB], y[TB];
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const float2 w = cs[k];
-      // both orders by selects: the arrays stay in registers
-      const float v0 = p.interleaved ? f[2 * k] : f[k], v1 = p.interleaved ? f[2 * k + 1] : f[k + N];
-      const float r0 = v0 * w.x - v1 * w.y, r1 = v0 * w.y + v1 * w.x;
-      if (p.interleaved) {
-        g[2 * k] = r0;
-        g[2 * k + 1] = r1;
-      } else {
-        g[k] = r0;
-        g[k + N] = r1;
+    for (int t = 0; t < TB; ++t)
+      if (t < rows) {
+        load_vals(x[t], src, in + t * in_row + e0);
+        load_vals(y[t], src, in + t * in_row + e1);
       }
+    if (j0 == 0) {  // while the first loads are under way
+      const int64_t* positions = static_cast<const int64_t*>(p.positions) + t0;
+      if (hkv && threadIdx.x < nt) {
+        const int64_t slot = static_cast<const int64_t*>(p.slots)[t0 + threadIdx.x];
+        const int64_t page = slot < 0 ? 0 : slot / p.page_size, off = slot - page * p.page_size;
+        const bool in = slot >= 0 && page < p.num_pages;
+        if (slot >= 0 && !in) atomicOr(&g_device_error, kErrIndex);
+        place[0][threadIdx.x] = in ? page * p.kc_page + off * p.kc_slot : -1;
+        place[1][threadIdx.x] = in ? page * p.vc_page + off * p.vc_slot : -1;
+      }
+      for (int i = threadIdx.x; i < nt * half; i += NT)
+        table[i] = turn(positions[i / half], static_cast<const int64_t*>(p.steps)[i % half], static_cast<float>(p.factor));
+      __syncthreads();
     }
-    store_vals<N>(dst, dt, out + e0, g);
-    store_vals<N>(dst, dt, out + e1, g + N);
+#pragma unroll
+    for (int t = 0; t < TB; ++t) {
+      if (t >= rows) break;
+      const int64_t at = cached ? place[isv][t] : (t0 + t) * p.qo_row;
+      if (at < 0) continue;
+      const int64_t out = at + out_head;
+      float f[2 * N], g[2 * N];
+      to_float<XT>(x[t], f);
+      to_float<XT>(y[t], f + N);
+      if (!turns) {
+#pragma unroll
+        for (int k = 0; k < 2 * N; ++k) g[k] = f[k];
+      } else if (N > 1 && p.interleaved) {  // pairs inside each group
+        const float2* cs = table + t * half + e0 / 2;
+#pragma unroll
+        for (int k = 0; k < 2 * N; k += 2) {
+          const float2 w = cs[k < N ? k / 2 : half / 2 + (k - N) / 2];
+          g[k] = f[k] * w.x - f[k + 1] * w.y;
+          g[k + 1] = f[k] * w.y + f[k + 1] * w.x;
+        }
+      } else {
+        const float2* cs = table + t * half + u * N;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          const float2 w = cs[k];
+          g[k] = f[k] * w.x - f[k + N] * w.y;
+          g[k + N] = f[k] * w.y + f[k + N] * w.x;
+        }
+      }
+      store_vals<N>(dst, dt, out + e0, g);
+      store_vals<N>(dst, dt, out + e1, g + N);
+    }
   }
 }
 
@@ -209,22 +222,32 @@ extern "C" int ggufmm_rope_append(const ggufmm_rope_args* args, void* stream) {
     return GGUFMM_ERR_ALIGN;
   const int s = check_device();
   if (s) return s;
-  // whole 16-byte groups: units of 8 pairs
-  auto whole = [](const void* ptr, int64_t e, std::initializer_list<int64_t> strides) {
-    bool ok = aligned_to(ptr, 16);
-    for (const int64_t v : strides) ok = ok && v * e % 16 == 0;
-    return ok;
+  // the widest groups of values that all widths, strides and addresses allow
+  auto whole = [&](int n) {
+    auto fits = [n](const void* ptr, int64_t e, int64_t row, int64_t head) {
+      const int64_t bytes = std::min<int64_t>(n * e, 16);
+      return reinterpret_cast<uintptr_t>(ptr) % bytes == 0 && row * e % bytes == 0 && head * e % bytes == 0;
+    };
+    return p.rot_dim % (2 * n) == 0 && d % (2 * n) == 0 && fits(p.q, xe, p.q_row, p.q_head) &&
+           fits(p.q_out, qe, p.qo_row, p.qo_head) &&
+           (!p.k || (fits(p.k, xe, p.k_row, p.k_head) && fits(p.v, xe, p.v_row, p.v_head)));
   };
-  const bool vec = d % 16 == 0 && p.rot_dim % 16 == 0 && whole(p.q, xe, {p.q_row, p.q_head}) &&
-                   whole(p.q_out, qe, {p.qo_row, p.qo_head}) &&
-                   (!p.k || (whole(p.k, xe, {p.k_row, p.k_head}) && whole(p.v, xe, {p.v_row, p.v_head})));
-  RopeArgs a{p, 1};
-  if (p.tokens > 2048) a.per_cta = 4;
-  const dim3 grid(static_cast<unsigned>((p.tokens + a.per_cta - 1) / a.per_cta));
-  const size_t smem = static_cast<size_t>(a.per_cta) * (p.rot_dim / 2) * sizeof(float2);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  auto go = [&](auto* fn) { return record_cuda_status(pdl_launch(fn, grid, dim3(256), smem, st, a)); };
-  if (p.x_dtype == GGUFMM_F32) return vec ? go(rope_append_kernel<GGUFMM_F32, 8>) : go(rope_append_kernel<GGUFMM_F32, 1>);
-  if (p.x_dtype == GGUFMM_F16) return vec ? go(rope_append_kernel<GGUFMM_F16, 8>) : go(rope_append_kernel<GGUFMM_F16, 1>);
-  return vec ? go(rope_append_kernel<GGUFMM_BF16, 8>) : go(rope_append_kernel<GGUFMM_BF16, 1>);
+  const bool many = p.tokens >= 592;  // two tokens a CTA leave several CTAs to every SM
+  const int tb = many ? 2 : 1;
+  const dim3 grid(static_cast<unsigned>((p.tokens + tb - 1) / tb));
+  const size_t smem = static_cast<size_t>(tb) * (p.rot_dim / 2) * sizeof(float2);
+  auto typed = [&](auto xt, auto n) {
+    constexpr int XT = decltype(xt)::value, N = decltype(n)::value;
+    return many ? pdl_launch(rope_append_kernel<XT, N, 2, 128>, grid, dim3(128), smem, st, RopeArgs{p})
+                : pdl_launch(rope_append_kernel<XT, N, 1, 256>, grid, dim3(256), smem, st, RopeArgs{p});
+  };
+  auto sized = [&](auto n) {
+    return record_cuda_status(p.x_dtype == GGUFMM_F32   ? typed(std::integral_constant<int, GGUFMM_F32>{}, n)
+                              : p.x_dtype == GGUFMM_F16 ? typed(std::integral_constant<int, GGUFMM_F16>{}, n)
+                                                        : typed(std::integral_constant<int, GGUFMM_BF16>{}, n));
+  };
+  if (whole(8)) return sized(std::integral_constant<int, 8>{});
+  if (whole(4)) return sized(std::integral_constant<int, 4>{});
+  return sized(std::integral_constant<int, 1>{});
 }
