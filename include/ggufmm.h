@@ -383,7 +383,8 @@ int ggufmm_mul_mat(const void* q, int qtype, int64_t n, int64_t k,
 /* ---- what lies between a layer's projections ------------------------------------------
  * Norm, rotary positions, key-value cache and attention. The reference runs them as
  * separate WGSL dispatches with f16 buffers between them
- * (vllm_webgpu/models/llama.py:239-367).
+ * (vllm_webgpu/models/llama.py:239-367). Arguments come in structs of 8-byte fields, read
+ * before the call returns; every pointer in them is a device pointer.
  */
 
 /*
@@ -399,18 +400,25 @@ int ggufmm_mul_mat(const void* q, int qtype, int64_t n, int64_t k,
  * does nothing; n is at most GGUFMM_NORM_MAX_N.
  */
 #define GGUFMM_NORM_MAX_N 65536
-int ggufmm_rms_norm(const void* x, int x_dtype, int64_t m, int64_t n, int64_t ldx,
-                    const void* resid, int r_dtype, int64_t ldr, void* resid_out, int64_t ldro,
-                    const void* w, int w_dtype, float w_add, float eps,
-                    void* y, int y_dtype, int64_t ldy, void* stream);
+typedef struct ggufmm_norm_args {
+  const void* x;
+  const void* resid;
+  void* resid_out;
+  const void* w;
+  void* y;
+  int64_t ldx, ldr, ldro, ldy; /* row strides, elements */
+  int64_t m, n, x_dtype, r_dtype, w_dtype, y_dtype;
+  double w_add, eps;
+} ggufmm_norm_args;
+
+int ggufmm_rms_norm(const ggufmm_norm_args* args, void* stream);
 
 /*
  * The paged key-value cache of the calls below: k and v, each [num_pages, kv_heads,
  * page_size, head_dim] of f16 or bf16 values. Strides are in elements, multiples of 8,
  * the innermost 1, pointers 16-byte aligned; head_dim is a multiple of 8 up to
  * GGUFMM_MAX_HEAD_DIM and page_size a multiple of 8. Slot s is offset s % page_size of
- * page s / page_size. The structs hold 8-byte fields only; every pointer but the struct's
- * own is a device pointer.
+ * page s / page_size.
  */
 #define GGUFMM_MAX_HEAD_DIM 256
 

@@ -115,7 +115,8 @@ def test_packed_arguments_match_the_header():
     from vllm_webgpu_b200 import ops
     text = open(os.path.join(ROOT, "include", "ggufmm.h")).read()
     text = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
-    for name, fmt in (("ggufmm_rope_args", ops._ROPE_ARGS), ("ggufmm_attention_args", ops._ATTENTION_ARGS)):
+    for name, fmt in (("ggufmm_norm_args", ops._NORM_ARGS), ("ggufmm_rope_args", ops._ROPE_ARGS),
+                      ("ggufmm_attention_args", ops._ATTENTION_ARGS)):
         body = re.search(r"typedef struct %s \{(.*?)\}" % name, text, flags=re.S).group(1)
         kinds = ""
         for decl in body.split(";"):
@@ -174,7 +175,9 @@ def test_norm_and_rope_refuse_on_the_host():
     lib, p = L.lib(), 1 << 20
 
     def norm(x=p, xt=2, m=1, n=64, ldx=64, r=p, rt=2, ldr=64, ro=p, ldro=64, w=p, wt=0, add=0.0, eps=1e-5, y=p, yt=2, ldy=64):
-        return lib.ggufmm_rms_norm(x, xt, m, n, ldx, r, rt, ldr, ro, ldro, w, wt, add, eps, y, yt, ldy, None)
+        return lib.ggufmm_rms_norm(ops._NORM_ARGS.pack(x or 0, r or 0, ro, w, y or 0, ldx, ldr, ldro, ldy, m, n, xt, rt, wt, yt,
+                                                       add, eps), None)
+    assert lib.ggufmm_rms_norm(None, None) == L.ERR_ARG
     assert norm(m=0) == L.OK
     assert norm(x=None) == L.ERR_ARG and norm(y=None) == L.ERR_ARG and norm(r=None) == L.ERR_ARG
     assert norm(eps=-1.0) == L.ERR_ARG and norm(eps=float("nan")) == L.ERR_ARG

@@ -270,7 +270,7 @@ cudaError_t launch_norm(const NormArgs& a, cudaStream_t st) {
   return x4 ? launch_any<4, 2>(a, st) : launch_any<2, 2>(a, st);
 }
 
-int elem(int dtype) { return dtype == GGUFMM_F32 ? 4 : dtype == GGUFMM_F16 || dtype == GGUFMM_BF16 ? 2 : 0; }
+int elem(int64_t dtype) { return dtype == GGUFMM_F32 ? 4 : dtype == GGUFMM_F16 || dtype == GGUFMM_BF16 ? 2 : 0; }
 bool al(const void* p, int a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
 }  // namespace
@@ -279,22 +279,39 @@ bool al(const void* p, int a) { return reinterpret_cast<uintptr_t>(p) % a == 0; 
 
 using namespace ggufmm;
 
-extern "C" int ggufmm_rms_norm(const void* x, int x_dtype, int64_t m, int64_t n, int64_t ldx, const void* resid,
-                               int r_dtype, int64_t ldr, void* resid_out, int64_t ldro, const void* w, int w_dtype,
-                               float w_add, float eps, void* y, int y_dtype, int64_t ldy, void* stream) {
-  const int xe = elem(x_dtype), ye = elem(y_dtype), we = w ? elem(w_dtype) : 1, re = resid ? elem(r_dtype) : 1;
+extern "C" int ggufmm_rms_norm(const ggufmm_norm_args* args, void* stream) {
+  if (!args) return GGUFMM_ERR_ARG;
+  const ggufmm_norm_args& p = *args;
+  const int xe = elem(p.x_dtype), ye = elem(p.y_dtype), we = p.w ? elem(p.w_dtype) : 1, re = p.resid ? elem(p.r_dtype) : 1;
   if (!xe || !ye || !we || !re) return GGUFMM_ERR_DTYPE;
-  if (m < 0 || m > (int64_t(1) << 31) - 1 || n <= 0 || n > GGUFMM_NORM_MAX_N || ldx < n || ldy < n ||
-      (resid && ldr < n) || (resid_out && ldro < n))
+  if (p.m < 0 || p.m > (int64_t(1) << 31) - 1 || p.n <= 0 || p.n > GGUFMM_NORM_MAX_N || p.ldx < p.n || p.ldy < p.n ||
+      (p.resid && p.ldr < p.n) || (p.resid_out && p.ldro < p.n))
     return GGUFMM_ERR_SHAPE;
-  if (resid_out && !resid) return GGUFMM_ERR_ARG;
-  if (!(eps >= 0.f)) return GGUFMM_ERR_ARG;
-  if (m == 0) return GGUFMM_OK;
-  if (!x || !y) return GGUFMM_ERR_ARG;
-  if (!al(x, xe) || !al(y, ye) || !al(w, we) || !al(resid, re) || !al(resid_out, re)) return GGUFMM_ERR_ALIGN;
+  if (p.resid_out && !p.resid) return GGUFMM_ERR_ARG;
+  if (!(p.eps >= 0.)) return GGUFMM_ERR_ARG;
+  if (p.m == 0) return GGUFMM_OK;
+  if (!p.x || !p.y) return GGUFMM_ERR_ARG;
+  if (!al(p.x, xe) || !al(p.y, ye) || !al(p.w, we) || !al(p.resid, re) || !al(p.resid_out, re)) return GGUFMM_ERR_ALIGN;
   const int s = check_device();
   if (s) return s;
-  const NormArgs a{x,   resid, resid_out, w,       y,       ldx,     ldr,   ldro, ldy, static_cast<int>(m), static_cast<int>(n),
-                   x_dtype, r_dtype, w_dtype, y_dtype, w_add, eps,  1.f / static_cast<float>(n)};
+  NormArgs a;
+  a.x = p.x;
+  a.r = p.resid;
+  a.ro = p.resid_out;
+  a.w = p.w;
+  a.y = p.y;
+  a.ldx = p.ldx;
+  a.ldr = p.ldr;
+  a.ldro = p.ldro;
+  a.ldy = p.ldy;
+  a.m = static_cast<int>(p.m);
+  a.n = static_cast<int>(p.n);
+  a.xt = static_cast<int>(p.x_dtype);
+  a.rt = static_cast<int>(p.r_dtype);
+  a.wt = static_cast<int>(p.w_dtype);
+  a.yt = static_cast<int>(p.y_dtype);
+  a.c = static_cast<float>(p.w_add);
+  a.eps = static_cast<float>(p.eps);
+  a.inv_n = 1.f / static_cast<float>(a.n);
   return record_cuda_status(launch_norm(a, static_cast<cudaStream_t>(stream)));
 }

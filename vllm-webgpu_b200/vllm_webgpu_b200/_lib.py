@@ -61,8 +61,7 @@ SIGNATURES = {
     "ggufmm_ffn_epilogue": (_I, [_VP, _I64, _I64, _I, _VP, _I64, _VP, _I, _I64, _VP]),
     "ggufmm_gemm_swiglu": (_I, [_VP, _VP, _I, _I64, _I64, _VP, _I, _I64, _I64, _VP, _I, _I64, _VP, _SZ, _VP]),
     "ggufmm_gemm_residual": (_I, [_VP, _I, _I64, _I64, _VP, _I, _I64, _I64, _VP, _I, _I64, _VP, _I64, _VP, _SZ, _VP]),
-    "ggufmm_rms_norm": (_I, [_VP, _I, _I64, _I64, _I64, _VP, _I, _I64, _VP, _I64, _VP, _I, ctypes.c_float,
-                             ctypes.c_float, _VP, _I, _I64, _VP]),
+    "ggufmm_rms_norm": (_I, [ctypes.c_char_p, _VP]),  # a packed ggufmm_norm_args
     "ggufmm_rope_append": (_I, [ctypes.c_char_p, _VP]),  # a packed ggufmm_rope_args
     "ggufmm_paged_attention_workspace_size": (_SZ, [_I64, _I64, _I64, _I64]),
     "ggufmm_paged_attention": (_I, [ctypes.c_char_p, _VP, _SZ, _VP]),  # a packed ggufmm_attention_args

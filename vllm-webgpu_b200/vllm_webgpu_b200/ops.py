@@ -619,33 +619,31 @@ def mul_mat(x: torch.Tensor, w: GGUFQuantTensor, out: torch.Tensor | None = None
 # what lies between a layer's projections: norm, rotary positions, key-value cache, attention
 # (the reference's shaders of vllm_webgpu/models/llama.py:239-367)
 # ---------------------------------------------------------------------------------------------
-# These calls are short next to their launch, so their wrappers keep to few tensor attributes.
+# These calls are short next to their launch, so their wrappers keep to few tensor attributes,
+# look each up once and pass the arguments as one packed struct.
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_native: dict = {}
 
 
-def _call(index: int, what: str, fn, *args) -> None:
-    """fn(*args, stream) with CUDA device ``index`` current, its status checked."""
+def _call(index: int, name: str, *args) -> None:
+    """The library's ``name``(*args, stream) with CUDA device ``index`` current, its status checked."""
+    fn = _native.get(name)
+    if fn is None:
+        fn = _native[name] = getattr(_lib.lib(), name)
     if torch.cuda.current_device() == index:
         st = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
             st = fn(*args, _raw_stream(index))
     if st:
-        _lib.check(st, what)
+        _lib.check(st, name)
 
 
-def _new(shape, dtype: torch.dtype, like: torch.Tensor) -> torch.Tensor:
-    """An uninitialised contiguous tensor beside ``like`` (quickest where like has its form)."""
-    if like.dtype is dtype and like.shape == shape and like.is_contiguous():
-        return torch.empty_like(like)
-    return torch.empty(shape, dtype=dtype, device=like.device)
-
-
-def _norm_rows(t: torch.Tensor, x: torch.Tensor, n: int, m: int, what: str | None) -> tuple[torch.Tensor, int]:
+def _norm_rows(t: torch.Tensor, shape, index: int, n: int, m: int, what: str | None) -> tuple[torch.Tensor, int]:
     """t as rows of n values, and the stride of a row: an input (what None: copied where its
     layout allows no rows) or an output."""
-    if t.shape != x.shape or t.get_device() != x.get_device():
-        raise ValueError(f"{what or 'residual'} must be a {tuple(x.shape)} tensor on {x.device}")
+    if t.shape != shape or t.get_device() != index:
+        raise ValueError(f"{what or 'residual'} must be a {tuple(shape)} tensor on cuda:{index}")
     if t.is_contiguous():
         return t, n
     if t.dim() == 2 and t.stride(1) == 1:
@@ -653,6 +651,9 @@ def _norm_rows(t: torch.Tensor, x: torch.Tensor, n: int, m: int, what: str | Non
     if what is not None:
         raise ValueError(f"{what} must be contiguous, or two-dimensional with contiguous rows")
     return t.contiguous(), n
+
+
+_NORM_ARGS = struct.Struct("5Q10q2d")
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-5,
@@ -666,40 +667,51 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1
     different dtypes. ``residual_out`` may be ``residual`` and ``out`` may be ``x`` (in
     place). Replaces the reference's add and rms_norm dispatches
     (vllm_webgpu/models/llama.py:262-270, 335-341)."""
-    if not x.is_cuda:
+    shape, index = x.shape, x.get_device()
+    if index < 0:
         _require_cuda(x)
-    shape = x.shape
-    if not shape or not shape[-1]:
+    count = x.numel()
+    n = shape[-1] if shape else 0
+    if n == 0:
         raise ValueError("rms_norm needs at least one value in a row")
-    n, index = shape[-1], x.get_device()
-    m = x.numel() // n
-    x2, ldx = _norm_rows(x, x, n, m, None)
-    r2, r_ptr, r_code, ldr, ro_ptr, ldro = None, None, 0, 0, None, 0
-    if residual is not None:
-        r2, ldr = _norm_rows(residual, x, n, m, None)
-        r_ptr, r_code = r2.data_ptr(), _code(r2.dtype)
-        if residual_out is None:
-            residual_out, ldro = _new(shape, residual.dtype, r2), n
+    m = count // n
+    x2, ldx = (x, n) if x.is_contiguous() else _norm_rows(x, shape, index, n, m, None)
+    r_ptr = r_code = ldr = ro_ptr = ldro = w_ptr = w_code = 0
+    like = x2
+    try:
+        if residual is not None:
+            r2, ldr = _norm_rows(residual, shape, index, n, m, None)
+            r_dtype = r2.dtype
+            r_ptr, r_code = r2.data_ptr(), _DTYPE_CODE[r_dtype]
+            if residual_out is None:
+                residual_out, ldro = torch.empty_like(r2, memory_format=torch.contiguous_format), n
+                like = residual_out
+            else:
+                if residual_out.dtype is not r_dtype:
+                    raise ValueError("residual_out must have the residual's dtype")
+                _, ldro = _norm_rows(residual_out, shape, index, n, m, "residual_out")
+            ro_ptr = residual_out.data_ptr()
+        elif residual_out is not None:
+            raise ValueError("residual_out needs a residual")
+        if out is None:
+            dtype = out_dtype or x2.dtype
+            if like.is_contiguous():
+                out = torch.empty_like(like) if like.dtype is dtype else torch.empty_like(like, dtype=dtype)
+            else:
+                out = torch.empty(shape, dtype=dtype, device=like.device)
+            ldy = n
         else:
-            if residual_out.dtype is not residual.dtype:
-                raise ValueError("residual_out must have the residual's dtype")
-            _, ldro = _norm_rows(residual_out, x, n, m, "residual_out")
-        ro_ptr = residual_out.data_ptr()
-    elif residual_out is not None:
-        raise ValueError("residual_out needs a residual")
-    if out is None:
-        dtype = out_dtype or x.dtype
-        out, ldy = _new(shape, dtype, r2 if r2 is not None and r2.dtype is dtype else x2), n
-    else:
-        _, ldy = _norm_rows(out, x, n, m, "out")
-        dtype = out.dtype
-    w_ptr = w_code = 0
-    if weight is not None:
-        if weight.dim() != 1 or weight.numel() != n or weight.get_device() != index or not weight.is_contiguous():
-            raise ValueError(f"weight must be a contiguous [{n}] tensor on {x.device}")
-        w_ptr, w_code = weight.data_ptr(), _code(weight.dtype)
-    _call(index, "ggufmm_rms_norm", _lib.lib().ggufmm_rms_norm, x2.data_ptr(), _code(x2.dtype), m, n, ldx, r_ptr, r_code,
-          ldr, ro_ptr, ldro, w_ptr, w_code, weight_add, eps, out.data_ptr(), _code(dtype), ldy)
+            _, ldy = _norm_rows(out, shape, index, n, m, "out")
+            dtype = out.dtype
+        if weight is not None:
+            if weight.numel() != n or weight.dim() != 1 or weight.get_device() != index or not weight.is_contiguous():
+                raise ValueError(f"weight must be a contiguous [{n}] tensor on {x.device}")
+            w_ptr, w_code = weight.data_ptr(), _DTYPE_CODE[weight.dtype]
+        args = _NORM_ARGS.pack(x2.data_ptr(), r_ptr, ro_ptr, w_ptr, out.data_ptr(), ldx, ldr, ldro, ldy, m, n,
+                               _DTYPE_CODE[x2.dtype], r_code, w_code, _DTYPE_CODE[dtype], weight_add, eps)
+    except KeyError as e:
+        raise ValueError(f"unsupported dtype {e.args[0]}; expected float32, float16 or bfloat16") from None
+    _call(index, "ggufmm_rms_norm", args)
     return out if residual is None else (out, residual_out)
 
 
@@ -759,23 +771,29 @@ def rope_steps(rot_dim: int, theta: float = 10000.0, scaling: dict | None = None
     return torch.from_numpy(steps.copy()).to(device if device is not None else "cuda"), factor
 
 
-def _heads(t: torch.Tensor, what: str, index: int) -> torch.Tensor:
-    """t as [tokens, heads, head_dim] with a unit stride in the last dimension, on device ``index``."""
-    if t.dim() != 3 or t.get_device() != index:
+def _heads(t: torch.Tensor, what: str, index: int) -> tuple[torch.Tensor, tuple, tuple]:
+    """t as [tokens, heads, head_dim] with a unit stride in the last dimension, on device
+    ``index``; its shape and strides."""
+    shape = t.shape
+    if len(shape) != 3 or t.get_device() != index:
         raise ValueError(f"{what} must be a [tokens, heads, head_dim] tensor on cuda:{index}")
-    return t if t.stride(2) == 1 else t.contiguous()
+    st = t.stride()
+    if st[2] != 1:
+        t = t.contiguous()
+        st = t.stride()
+    return t, shape, st
 
 
 def _index(t: torch.Tensor, dtype: torch.dtype, length: int, what: str, index: int) -> torch.Tensor:
-    if t.dim() != 1 or t.numel() != length or t.get_device() != index:
+    if t.numel() != length or t.dim() != 1 or t.get_device() != index:
         raise ValueError(f"{what} must be a [{length}] tensor on cuda:{index}")
     return t if t.dtype is dtype and t.is_contiguous() else t.to(dtype).contiguous()
 
 
 def _cache_strides(k_cache: torch.Tensor, v_cache: torch.Tensor, index: int) -> tuple:
-    """(shape, strides of page, head and slot of k, of v) of caches [pages, kv heads, page size, head_dim]."""
-    shape = k_cache.shape
-    if len(shape) != 4 or shape != v_cache.shape or k_cache.dtype is not v_cache.dtype:
+    """(shape, dtype, strides of k, of v) of caches [pages, kv heads, page size, head_dim]."""
+    shape, dtype = k_cache.shape, k_cache.dtype
+    if len(shape) != 4 or shape != v_cache.shape or dtype is not v_cache.dtype:
         raise ValueError("k_cache and v_cache must be [pages, kv heads, page size, head_dim] tensors of one shape and dtype")
     if k_cache.get_device() != index or v_cache.get_device() != index:
         raise ValueError(f"the cache must lie on cuda:{index}")
@@ -785,46 +803,49 @@ def _cache_strides(k_cache: torch.Tensor, v_cache: torch.Tensor, index: int) -> 
     if 1 in shape:  # the stride of a dimension of one says nothing: any valid one does
         d = shape[3]
         ks, vs = ([d if shape[i] == 1 else st[i] for i in range(3)] for st in (ks, vs))
-    return shape, ks[:3], vs[:3]
+    return shape, dtype, ks, vs
 
 
 _ROPE_ARGS = struct.Struct("Q2qQ2qQ2qQ2qQ3qQ3q3Q11qd")
 
 
 def _rope(q, k, v, positions, steps, slots, k_cache, v_cache, interleaved, factor, q_out):
-    if not q.is_cuda:
-        _require_cuda(q)
     index = q.get_device()
-    q = _heads(q, "q", index)
-    t, hq, d = q.shape
+    if index < 0:
+        _require_cuda(q)
+    q, shape, qs = _heads(q, "q", index)
+    t, hq, d = shape
     dtype = q.dtype
     if q_out is None:
-        q_out = _new(q.shape, dtype, q)
-    elif q_out.shape != q.shape or q_out.get_device() != index or q_out.stride(2) != 1:
-        raise ValueError(f"q_out must be a {tuple(q.shape)} tensor with unit stride in its last dimension")
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif q_out.shape != shape or q_out.get_device() != index or q_out.stride(2) != 1:
+        raise ValueError(f"q_out must be a {tuple(shape)} tensor with unit stride in its last dimension")
     positions = _index(positions, torch.int64, t, "positions", index)
     if steps.get_device() != index or steps.dtype is not torch.int64 or steps.dim() != 1 or not steps.is_contiguous():
         raise ValueError(f"steps must be the int64 tensor of rope_steps on cuda:{index}")
-    qs, os = q.stride(), q_out.stride()
-    if k is None:
-        kv = (0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
-        hkv, cache_dtype, page, pages, slot_ptr = 0, 0, 0, 0, 0
-    else:
-        k, v = _heads(k, "k", index), _heads(v, "v", index)
-        hkv = k.shape[1]
-        if k.shape != (t, hkv, d) or v.shape != k.shape or k.dtype is not dtype or v.dtype is not dtype:
-            raise ValueError(f"k and v must be [{t}, kv heads, {d}] tensors of q's dtype")
-        (pages, heads, page, dk), kst, vst = _cache_strides(k_cache, v_cache, index)
-        if heads != hkv or dk != d:
-            raise ValueError(f"the cache holds {heads} heads of {dk}, k has {hkv} of {d}")
-        slots = _index(slots, torch.int64, t, "slots", index)
-        slot_ptr, cache_dtype = slots.data_ptr(), _code(k_cache.dtype)
-        s, u = k.stride(), v.stride()
-        kv = (k.data_ptr(), s[0], s[1], v.data_ptr(), u[0], u[1], k_cache.data_ptr(), *kst, v_cache.data_ptr(), *vst)
-    args = _ROPE_ARGS.pack(q.data_ptr(), qs[0], qs[1], q_out.data_ptr(), os[0], os[1], *kv, positions.data_ptr(), slot_ptr,
-                           steps.data_ptr(), t, hq, hkv, d, 2 * steps.shape[0], 1 if interleaved else 0, _code(dtype),
-                           _code(q_out.dtype), cache_dtype, page, pages, factor)
-    _call(index, "ggufmm_rope_append", _lib.lib().ggufmm_rope_append, args)
+    os = q_out.stride()
+    try:
+        if k is None:
+            kv = (0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+            hkv, cache_code, page, pages, slot_ptr = 0, 0, 0, 0, 0
+        else:
+            (k, k_shape, s), (v, v_shape, u) = _heads(k, "k", index), _heads(v, "v", index)
+            hkv = k_shape[1]
+            if k_shape[0] != t or k_shape[2] != d or v_shape != k_shape or k.dtype is not dtype or v.dtype is not dtype:
+                raise ValueError(f"k and v must be [{t}, kv heads, {d}] tensors of q's dtype")
+            (pages, heads, page, dk), cache_dtype, ks, vs = _cache_strides(k_cache, v_cache, index)
+            if heads != hkv or dk != d:
+                raise ValueError(f"the cache holds {heads} heads of {dk}, k has {hkv} of {d}")
+            slots = _index(slots, torch.int64, t, "slots", index)
+            slot_ptr, cache_code = slots.data_ptr(), _DTYPE_CODE[cache_dtype]
+            kv = (k.data_ptr(), s[0], s[1], v.data_ptr(), u[0], u[1], k_cache.data_ptr(), ks[0], ks[1], ks[2],
+                  v_cache.data_ptr(), vs[0], vs[1], vs[2])
+        args = _ROPE_ARGS.pack(q.data_ptr(), qs[0], qs[1], q_out.data_ptr(), os[0], os[1], *kv, positions.data_ptr(),
+                               slot_ptr, steps.data_ptr(), t, hq, hkv, d, 2 * steps.numel(), 1 if interleaved else 0,
+                               _DTYPE_CODE[dtype], _DTYPE_CODE[q_out.dtype], cache_code, page, pages, factor)
+    except KeyError as e:
+        raise ValueError(f"unsupported dtype {e.args[0]}; expected float32, float16 or bfloat16") from None
+    _call(index, "ggufmm_rope_append", args)
     return q_out
 
 
@@ -887,21 +908,24 @@ def _attention_workspace(batch: int, hq: int, hkv: int, d: int, index: int) -> t
 
 def _attention_args(q, k_cache, v_cache, tables, lens, scale, window, out, q_starts, max_q):
     """(device index, packed arguments, out, sizes, the tensors the arguments point to)."""
-    if not q.is_cuda:
-        _require_cuda(q)
     index = q.get_device()
-    q = _heads(q, "q", index)
-    t, hq, d = q.shape
-    (pages, hkv, page, dk), ks, vs = _cache_strides(k_cache, v_cache, index)
+    if index < 0:
+        _require_cuda(q)
+    q, shape, qs = _heads(q, "q", index)
+    t, hq, d = shape
+    (pages, hkv, page, dk), cache_dtype, ks, vs = _cache_strides(k_cache, v_cache, index)
     dtype = q.dtype
-    if dk != d or k_cache.dtype is not dtype:
-        raise ValueError(f"q and the cache must share head_dim and dtype: {d} {dtype}, {dk} {k_cache.dtype}")
+    if dk != d or cache_dtype is not dtype:
+        raise ValueError(f"q and the cache must share head_dim and dtype: {d} {dtype}, {dk} {cache_dtype}")
     if hkv == 0 or hq % hkv:
         raise ValueError(f"{hq} query heads are no multiple of {hkv} kv heads")
     if out is None:
-        out = _new(q.shape, dtype, q)
-    elif out.shape != q.shape or out.dtype is not dtype or out.get_device() != index or out.stride(2) != 1:
-        raise ValueError(f"out must be a {tuple(q.shape)} {dtype} tensor with unit stride in its last dimension")
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        os = (hq * d, d)
+    else:
+        if out.shape != shape or out.dtype is not dtype or out.get_device() != index or out.stride(2) != 1:
+            raise ValueError(f"out must be a {tuple(shape)} {dtype} tensor with unit stride in its last dimension")
+        os = out.stride()
     if tables.dim() != 2 or tables.get_device() != index:
         raise ValueError(f"block_tables must be a [batch, pages] tensor on cuda:{index}")
     b, width = tables.shape
@@ -914,13 +938,13 @@ def _attention_args(q, k_cache, v_cache, tables, lens, scale, window, out, q_sta
         starts = q_starts.data_ptr()
     elif t != b:
         raise ValueError(f"q holds {t} tokens for {b} sequences")
-    qs, os = q.stride(), out.stride()
     if t == 1 or hq == 1:  # the stride of a dimension of one says nothing: any valid one does
         qs, os = ((st[0] if t > 1 else hq * d, st[1] if hq > 1 else d) for st in (qs, os))
+    code = _DTYPE_CODE.get(dtype, -1)  # the library refuses what the cache cannot hold
     args = _ATTENTION_ARGS.pack(
-        q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], k_cache.data_ptr(), *ks, v_cache.data_ptr(), *vs,
-        tables.data_ptr(), tables.stride(0) if b > 1 else width, width, lens.data_ptr(), starts, b, t, max_q, hq, hkv, d,
-        page, pages, _code(dtype), window, d ** -0.5 if scale is None else scale)
+        q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], k_cache.data_ptr(), ks[0], ks[1], ks[2],
+        v_cache.data_ptr(), vs[0], vs[1], vs[2], tables.data_ptr(), tables.stride(0) if b > 1 else width, width,
+        lens.data_ptr(), starts, b, t, max_q, hq, hkv, d, page, pages, code, window, d ** -0.5 if scale is None else scale)
     return index, args, out, (b, hq, hkv, d), (q, tables, lens, q_starts)
 
 
@@ -939,7 +963,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         workspace = _attention_workspace(*sizes, index)
     elif workspace.get_device() != index:
         raise ValueError(f"workspace must lie on cuda:{index}")
-    _call(index, "ggufmm_paged_attention", _lib.lib().ggufmm_paged_attention, args, workspace.data_ptr(), workspace.numel())
+    _call(index, "ggufmm_paged_attention", args, workspace.data_ptr(), workspace.numel())
     return out
 
 
@@ -954,5 +978,5 @@ def paged_prompt_attention(q: torch.Tensor, q_starts: torch.Tensor, max_q: int, 
     reference feeds a prompt token by token (run_inference.py:323-350)."""
     index, args, out, _, keep = _attention_args(q, k_cache, v_cache, block_tables, lens, scale, window, out, q_starts,
                                                 max_q)
-    _call(index, "ggufmm_paged_prompt_attention", _lib.lib().ggufmm_paged_prompt_attention, args)
+    _call(index, "ggufmm_paged_prompt_attention", args)
     return out
