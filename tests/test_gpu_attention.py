@@ -142,6 +142,34 @@ def test_decode_peaked_and_flat_scores(cuda):
     _decode(c, q=q)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("kind", ["single", "prompt"])
+def test_a_long_tail_of_small_weights(cuda, dtype, kind):
+    """One weight of 1 and 60000 of 2^-24.5, below the smallest 16-bit float: together 0.25%."""
+    from vllm_webgpu_b200 import ops
+    n = 60001
+    c = Case([n], 4, 1, 64, dtype, 64, seed=13)
+    top = 24.5 * 0.6931471805599453
+    c.kc.zero_()
+    c.vc.fill_(1.0)
+    page, at = int(c.table[0, 700]), 33
+    c.kc[page, 0, at, 0] = 1.0
+    c.vc[page, 0, at] = 0.0
+    q = torch.zeros(1, 4, 64, dtype=dtype, device="cuda")
+    q[..., 0] = 17.0
+    scale = top / 17.0
+    if kind == "single":
+        got = ops.paged_attention(q, c.kc, c.vc, c.table, c.device_lens(), scale=scale)
+    else:
+        got = ops.paged_prompt_attention(q, torch.tensor([0, 1], dtype=torch.int32, device="cuda"), 1, c.kc, c.vc, c.table,
+                                         c.device_lens(), scale=scale)
+    tail = (n - 1) * 2.0 ** -24.5
+    want = torch.full((1, 4, 64), tail / (1 + tail), dtype=torch.float64)
+    # the bound of _check, with A = the result itself (v is not negative); the prompt's running
+    # maximum may stand 2^8 below, which the weights' range takes up
+    _check(got, want, want, dtype)
+
+
 def test_decode_strides_and_scale(cuda):
     from vllm_webgpu_b200 import ops
     c = Case([33, 260], 8, 2, 128, BF16, 16, seed=7, slots_first=True)

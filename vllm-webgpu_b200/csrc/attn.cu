@@ -73,6 +73,7 @@ extern "C" int ggufmm_paged_prompt_attention(const ggufmm_attention_args* args, 
   const ggufmm_attention_args& p = *args;
   int s = check_attention(p, true);
   if (s || p.batch == 0 || p.total_q == 0 || p.max_q == 0) return s;
+  if (p.max_q > kI32Max / (p.batch * p.kv_heads)) return GGUFMM_ERR_SHAPE;  // tiles of the grid
   s = check_device();
   if (s) return s;
   return record_cuda_status(launch_paged_prompt(p, static_cast<cudaStream_t>(stream)));

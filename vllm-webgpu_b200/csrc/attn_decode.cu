@@ -189,6 +189,9 @@ __global__ void __launch_bounds__(Shape<DP>::W * 32, 1) paged_decode_kernel(cons
   // a stage: K, then V, 16 tokens each: row r, 128-byte column block c at (r / 8) * 1024 +
   // c * 2048 + (r % 8) * 128, its 16-byte chunks in the order chunk ^ (r % 8)
   constexpr int HS = 1024, BS = 2048;
+  // 16-bit floats underflow early (2^-24), and a long tail of small weights can add up: theirs
+  // are kept 2^14 larger, the sum too
+  constexpr float kUp = DT == GGUFMM_F16 ? 14.f : 0.f;
   extern __shared__ __align__(1024) uint8_t ring[];
   float* join = reinterpret_cast<float*>(ring + C::JOIN);
   float* ml = reinterpret_cast<float*>(ring + C::ML);
@@ -415,7 +418,7 @@ __global__ void __launch_bounds__(Shape<DP>::W * 32, 1) paged_decode_kernel(cons
             o[i][3] *= f1;
           }
         }
-        const float z0 = m0 == -INFINITY ? 0.f : m0, z1 = m1 == -INFINITY ? 0.f : m1;
+        const float z0 = (m0 == -INFINITY ? 0.f : m0) - kUp, z1 = (m1 == -INFINITY ? 0.f : m1) - kUp;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
           s[n][0] = exp2_fast(s[n][0] - z0);
@@ -425,7 +428,7 @@ __global__ void __launch_bounds__(Shape<DP>::W * 32, 1) paged_decode_kernel(cons
           l0 += s[n][0] + s[n][1];
           l1 += s[n][2] + s[n][3];
         }
-        // the weights, in [0, 1], rounded to the cache's type for the product with v: a
+        // the weights, at most 1 (2^kUp), rounded to the cache's type for the product with v: a
         // relative 2^-9 (2^-12) each, below the rounding of the output; their sum is not rounded
         const uint32_t p[4] = {pack16<DT>(s[0][0], s[0][1]), pack16<DT>(s[0][2], s[0][3]), pack16<DT>(s[1][0], s[1][1]),
                                pack16<DT>(s[1][2], s[1][3])};

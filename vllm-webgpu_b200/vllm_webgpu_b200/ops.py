@@ -622,6 +622,7 @@ def mul_mat(x: torch.Tensor, w: GGUFQuantTensor, out: torch.Tensor | None = None
 # These calls are short next to their launch, so their wrappers keep to few tensor attributes,
 # look each up once and pass the arguments as one packed struct.
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice  # the callers' tensors are on a GPU: CUDA is up
 _native: dict = {}
 
 
@@ -630,7 +631,7 @@ def _call(index: int, name: str, *args) -> None:
     fn = _native.get(name)
     if fn is None:
         fn = _native[name] = getattr(_lib.lib(), name)
-    if torch.cuda.current_device() == index:
+    if _current_device() == index:
         st = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
