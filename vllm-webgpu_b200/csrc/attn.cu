@@ -3,7 +3,7 @@
 // ggufmm_paged_prompt_attention (ragged causal prompts, attn_prompt.cu), and their checks.
 //
 // The reference runs a score, a softmax and an output shader over one sequence
-// (vllm_webgpu/models/llama.py:314-326; shaders/generic/{attn_score,softmax,attn_output}.wgsl).
+// (vllm_webgpu/models/llama.py:239-367; shaders/generic/{attn_score,softmax,attn_output}.wgsl).
 #include <cmath>
 
 #include "paged.cuh"

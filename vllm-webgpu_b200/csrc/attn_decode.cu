@@ -13,8 +13,7 @@
 // tokens; an item counts as one block more, for what it costs to begin and to end one. Every
 // CTA (one per SM) takes an equal run of consecutive blocks, whatever sequences they belong
 // to, so ragged lengths leave no SM idle; it finds its run by a sum over the lengths on the
-// device. An item inside one run is written directly. An item that
-// crosses runs leaves fp32 partials (m, sum, o) in the workspace, and the last of its CTAs
+// device. An item inside one run is written directly. An item that crosses runs leaves fp32 partials (m, sum, o) in the workspace, and the last of its CTAs
 // to finish (a counter) adds them in the order of the CTAs, so the result does not depend
 // on which was last. (Handing part of the work out in short runs as CTAs finish was measured:
 // 196 to 208 us for 64 sequences up to 8192 tokens against 195, 124 to 152 us for one of 131035
@@ -25,6 +24,11 @@
 // except where an item ends, and the ring keeps streaming over that too. (TMA boxes of whole
 // 16-token pages did as well at head width 128, but the unit takes about 134 clocks for every
 // request: pages of 8 or 24 tokens, or heads that are no multiple of 64 wide, got 2.4 TB/s.)
+//
+// 32 / 8 heads of 128, bf16, pages of 16: 64 sequences up to 8192 tokens (1.155 GB) 184 us, 6.27
+// TB/s, 97% of the measured copy rate; 16 around 1300 (90 MB) 25 us; one of 513 9.1 us. 64 / 8 heads,
+// f16, one sequence of 131035 (537 MB) 94 us, 5.7 TB/s. HBM bound when long; when short the time is
+// a chain of waits: lengths, page table, first copies (4 us), join in the CTA (0.8), join of CTAs (1.5).
 #include <algorithm>
 #include <atomic>
 #include <cmath>

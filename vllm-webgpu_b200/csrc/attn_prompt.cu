@@ -26,11 +26,11 @@
 // than 2^8 since its last rescaling (the weights then reach at most 2^8, harmless in 32-bit
 // sums).
 //
-// 8192 tokens of 32 / 8 heads of 128: 447 us, 1231 TFLOP/s, 74% of the measured bf16 burst (called
-// for a second on end, under the power limit, 515 us, 75% of the sustained rate). Per 256 x 128
-// scores the tensor core is busy for about 2050 of 3280 clocks and the exponentials for 2050;
-// what is left is each tile's chain of load, maximum, exponentials and hand-over (2650). A
-// quarter of the exponentials as polynomials on the FMA units took 460 us.
+// 8192 tokens of 32 / 8 heads of 128: 425 us, 1294 TFLOP/s, 78% of the measured bf16 burst (called
+// for a second on end, under the power limit, 500 us, 77% of the sustained rate). Per 256 x 128
+// scores the tensor core and the exponentials are each busy for about 2050 of 3100 clocks; what
+// is left is each tile's chain of load, maximum, exponentials and hand-over (2500). A
+// quarter of the exponentials as polynomials on the FMA units took 3% longer.
 //
 // Warps: 4 softmax warps per query tile, one that loads queries and values, one that issues
 // the products, two that load keys.
@@ -563,9 +563,8 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
       for (int h = 0; h < 2; ++h) {
         uint32_t p[BN / 4];
         const float* v = s + h * (BN / 2);
-        weights<DT, BN / 4>(v, s2, z, p, sum);
+        weights<DT, BN / 2>(v, s2, z, p, sum);
         if (h) handed(0);  // its store has had time to finish
-        weights<DT, BN / 4>(v + BN / 4, s2, z, p + BN / 8, sum);
 #pragma unroll
         for (int c = 0; c < BN / 4; c += 16) tmem_st16(pc + h * (BN / 4) + c, p + c);
       }

@@ -4,9 +4,14 @@
 //   s = x + r,  y = s * rsqrt(mean(s^2) + eps) * (w + c),  r' = s
 //
 // The reference runs its add shader and its rms_norm shader as two dispatches
-// (vllm_webgpu/models/llama.py:262-270, :335-341; shaders/generic/{add,rms_norm}.wgsl),
+// (vllm_webgpu/models/llama.py:239-367; shaders/generic/{add,rms_norm}.wgsl),
 // with the stream rounded to f16 between them. Here the sum stays in 32 bits: it is
 // rounded once into r' and, after the norm, once into y.
+//
+// HBM bound: a row is read once, held in registers over the sum of its squares, and written.
+// 8192 rows of 4096, x in 32 bits, r, r' and y in bf16 (336 MB): 51.5 us, 6.5 TB/s, the measured
+// copy rate. One row takes 2.2 us, a launch and two memory latencies. Rows that do not start on
+// 16 bytes go value by value: 8192 rows of 4095 take 94 us.
 #include "mma16.cuh"
 
 namespace ggufmm {

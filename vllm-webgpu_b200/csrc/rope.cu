@@ -5,7 +5,7 @@
 //   a' = factor * (a cos phi - b sin phi),  b' = factor * (a sin phi + b cos phi)
 // with (a, b) = (i, i + rot_dim/2) or, interleaved, (2i, 2i + 1). The reference runs this
 // as its rope shader on q and on k and its kv_cache_store shader on k and on v
-// (vllm_webgpu/models/llama.py:286-312; shaders/generic/{rope,kv_cache_store}.wgsl).
+// (vllm_webgpu/models/llama.py:239-367; shaders/generic/{rope,kv_cache_store}.wgsl).
 //
 // The frequencies come as turns per position in units of 2^-64 (a 64-bit integer), so the
 // product with the position, reduced modulo one turn by the integer's own overflow, is

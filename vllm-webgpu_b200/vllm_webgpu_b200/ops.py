@@ -667,7 +667,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1
     computed in 32 bits and rounded once each; x, residual, weight and out may have
     different dtypes. ``residual_out`` may be ``residual`` and ``out`` may be ``x`` (in
     place). Replaces the reference's add and rms_norm dispatches
-    (vllm_webgpu/models/llama.py:262-270, 335-341)."""
+    (vllm_webgpu/models/llama.py:239-367)."""
     shape, index = x.shape, x.get_device()
     if index < 0:
         _require_cuda(x)
@@ -856,7 +856,7 @@ def rope(x: torch.Tensor, positions: torch.Tensor, steps: torch.Tensor, interlea
     each head turn in pairs (i, i + half) or, ``interleaved`` (as GGUF files of the Llama
     family order them), (2i, 2i + 1), by positions[t] times the step of ``rope_steps``;
     the rest passes. ``out`` may be x. Replaces the reference's rope dispatch
-    (vllm_webgpu/models/llama.py:286-298)."""
+    (vllm_webgpu/models/llama.py:239-367)."""
     return _rope(x, None, None, positions, steps, None, None, None, interleaved, factor, out)
 
 
@@ -869,7 +869,7 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     page s // page size) of ``k_cache`` / ``v_cache`` [pages, kv heads, page size,
     head_dim], f16 or bf16. A negative slot stores nothing; one past the last page too, and
     sets bit 2 of the device status word. Replaces the reference's rope and kv_cache_store
-    dispatches (vllm_webgpu/models/llama.py:286-312)."""
+    dispatches (vllm_webgpu/models/llama.py:239-367)."""
     if k is None or v is None or slots is None or k_cache is None or v_cache is None:
         raise ValueError("rope_append needs k, v, slots and the caches (rope turns q alone)")
     return _rope(q, k, v, positions, steps, slots, k_cache, v_cache, interleaved, factor, q_out)
@@ -958,7 +958,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     token included). ``scale`` defaults to head_dim^-1/2; ``window`` > 0 lets a token see
     the last ``window`` positions only. A sequence of length 0 gives zeros. ``workspace``
     (``attention_workspace``) defaults to one kept per stream. Replaces the reference's
-    score, softmax and output dispatches (vllm_webgpu/models/llama.py:314-326)."""
+    score, softmax and output dispatches (vllm_webgpu/models/llama.py:239-367)."""
     index, args, out, sizes, keep = _attention_args(q, k_cache, v_cache, block_tables, lens, scale, window, out, None, 0)
     if workspace is None:
         workspace = _attention_workspace(*sizes, index)
