@@ -466,7 +466,9 @@ int ggufmm_rope_append(const ggufmm_rope_args* args, void* stream);
  * length with its new tokens, whose keys and values are in the cache already. A query at
  * position i sees j <= i and, when window > 0, j > i - window; one that sees nothing gives
  * zeros. A page outside the cache reads as zeros and a length past the table is cut to it;
- * both set bit 2 of the device status word.
+ * both set bit 2 of the device status word. Slots past a sequence's length, and whole pages
+ * before every query's window, may hold anything; the values of tokens that some query of a
+ * prompt sees must be finite, since they meet the other queries' weights of 0 in one product.
  *
  * ggufmm_paged_attention: one new token per sequence, total_q == batch (q_starts and max_q
  * are not read), at position lens[b] - 1; a length <= 0 gives zeros. The cache's length is
@@ -477,7 +479,9 @@ int ggufmm_rope_append(const ggufmm_rope_args* args, void* stream);
  * ggufmm_paged_prompt_attention: sequence b's new tokens are rows q_starts[b] to
  * q_starts[b + 1] of q, the last lens[b]-positions of the sequence; max_q is at least the
  * longest of them (rows past it are not computed, and set bit 2). Rows that belong to no
- * sequence are not written.
+ * sequence are not written. `workspace` (ggufmm_paged_prompt_attention_workspace_size bytes,
+ * 256-byte aligned, any content) lets a few new tokens on a long cache share its keys out over
+ * the SMs; 0 bytes where the new tokens fill them, and NULL or less works without sharing.
  */
 #define GGUFMM_MAX_GROUP 64
 typedef struct ggufmm_attention_args {
@@ -499,7 +503,9 @@ typedef struct ggufmm_attention_args {
 
 size_t ggufmm_paged_attention_workspace_size(int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_dim);
 int ggufmm_paged_attention(const ggufmm_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
-int ggufmm_paged_prompt_attention(const ggufmm_attention_args* args, void* stream);
+size_t ggufmm_paged_prompt_attention_workspace_size(const ggufmm_attention_args* args);
+int ggufmm_paged_prompt_attention(const ggufmm_attention_args* args, void* workspace, size_t workspace_bytes,
+                                  void* stream);
 
 #ifdef __cplusplus
 }

@@ -272,6 +272,24 @@ def test_prompt_lengths(cuda, new, lens):
     _prompt(Case(lens, 8, 2, 128, BF16, 16, seed=len(new)), new, extra_max=3)
 
 
+@pytest.mark.parametrize("hq,hkv,d,dtype", [(8, 2, 128, BF16), (3, 1, 64, F16), (4, 1, 256, BF16), (5, 1, 96, F16)])
+@pytest.mark.parametrize("new,lens,window", [([3], [5000], 0), ([1, 40, 7], [4100, 40, 0], 0), ([2, 2], [9000, 3000], 2500),
+                                             ([130], [3000], 0)])
+def test_prompt_keys_shared_out(cuda, hq, hkv, d, dtype, new, lens, window):
+    """A few new tokens on a long cache: several CTAs take shares of the keys, some of them none."""
+    from vllm_webgpu_b200 import ops
+    c = Case(lens, hq, hkv, d, dtype, 16, seed=sum(new))
+    wide = torch.full((len(lens), 2000), -1, dtype=torch.int32, device="cuda")  # a table for long texts
+    wide[:, :c.table.shape[1]] = c.table
+    c.table = wide
+    first = _prompt(c, new, window)
+    q = c.q(sum(new))
+    starts = torch.tensor([sum(new[:i]) for i in range(len(new) + 1)], dtype=torch.int32, device="cuda")
+    a, b = (ops.paged_prompt_attention(q, starts, max(new), c.kc, c.vc, c.table, c.device_lens(), window=window)
+            for _ in range(2))
+    assert torch.equal(a, b) and first.shape == a.shape
+
+
 def test_prompt_masked_out_rows(cuda):
     """More new tokens than the length holds: the queries before position 0 see nothing."""
     from vllm_webgpu_b200 import ops

@@ -141,7 +141,7 @@ def _attention(**other):
     f.update(other)
     args = ops._ATTENTION_ARGS.pack(*f.values())
     lib = _lib.lib()
-    return (lib.ggufmm_paged_attention(args, p, 1 << 40, None), lib.ggufmm_paged_prompt_attention(args, None))
+    return (lib.ggufmm_paged_attention(args, p, 1 << 40, None), lib.ggufmm_paged_prompt_attention(args, None, 0, None))
 
 
 def test_attention_refuses_on_the_host():
@@ -164,7 +164,7 @@ def test_attention_refuses_on_the_host():
     assert _attention(q_heads=8 * 65) == (L.ERR_SHAPE, L.ERR_SHAPE)
     lib = L.lib()
     assert lib.ggufmm_paged_attention(None, None, 0, None) == L.ERR_ARG
-    assert lib.ggufmm_paged_prompt_attention(None, None) == L.ERR_ARG
+    assert lib.ggufmm_paged_prompt_attention(None, None, 0, None) == L.ERR_ARG
     assert lib.ggufmm_paged_attention_workspace_size(0, 8, 8, 128) == 0
     assert lib.ggufmm_paged_attention_workspace_size(2, 8, 8, 128) > 0
 

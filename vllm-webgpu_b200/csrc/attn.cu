@@ -12,7 +12,14 @@ namespace ggufmm {
 
 size_t paged_decode_workspace(int64_t group, int64_t head_dim);  // attn_decode.cu
 cudaError_t launch_paged_decode(const ggufmm_attention_args& p, void* workspace, cudaStream_t st);
-cudaError_t launch_paged_prompt(const ggufmm_attention_args& p, cudaStream_t st);  // attn_prompt.cu
+size_t paged_prompt_workspace(const ggufmm_attention_args& p, int sms);  // attn_prompt.cu
+cudaError_t launch_paged_prompt(const ggufmm_attention_args& p, int sms, void* workspace, size_t workspace_bytes,
+                                cudaStream_t st);
+struct DevInfo {
+  int sms = 0;
+  int smem_optin = 0;
+};
+DevInfo device_info(int dev);  // capi.cu
 
 namespace {
 
@@ -68,13 +75,27 @@ extern "C" int ggufmm_paged_attention(const ggufmm_attention_args* args, void* w
   return record_cuda_status(launch_paged_decode(p, workspace, static_cast<cudaStream_t>(stream)));
 }
 
-extern "C" int ggufmm_paged_prompt_attention(const ggufmm_attention_args* args, void* stream) {
+extern "C" size_t ggufmm_paged_prompt_attention_workspace_size(const ggufmm_attention_args* args) {
+  int dev = 0;
+  if (!args || check_attention(*args, true) || args->batch == 0 || args->max_q == 0 || check_device() ||
+      cudaGetDevice(&dev) != cudaSuccess || args->max_q > kI32Max / (args->batch * args->kv_heads))
+    return 0;
+  return paged_prompt_workspace(*args, device_info(dev).sms);
+}
+
+extern "C" int ggufmm_paged_prompt_attention(const ggufmm_attention_args* args, void* workspace, size_t workspace_bytes,
+                                             void* stream) {
   if (!args) return GGUFMM_ERR_ARG;
   const ggufmm_attention_args& p = *args;
   int s = check_attention(p, true);
   if (s || p.batch == 0 || p.total_q == 0 || p.max_q == 0) return s;
   if (p.max_q > kI32Max / (p.batch * p.kv_heads)) return GGUFMM_ERR_SHAPE;  // tiles of the grid
+  if (!aligned_to(workspace, 256)) return GGUFMM_ERR_ALIGN;
   s = check_device();
   if (s) return s;
-  return record_cuda_status(launch_paged_prompt(p, static_cast<cudaStream_t>(stream)));
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return record_cuda_status(e);
+  return record_cuda_status(
+      launch_paged_prompt(p, device_info(dev).sms, workspace, workspace_bytes, static_cast<cudaStream_t>(stream)));
 }

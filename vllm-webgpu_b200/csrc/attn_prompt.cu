@@ -32,6 +32,10 @@
 // is left is each tile's chain of load, maximum, exponentials and hand-over (2500). A
 // quarter of the exponentials as polynomials on the FMA units took 3% longer.
 //
+// Where the query tiles are fewer than the SMs and the cache may be long (a few new tokens on a
+// long text), several CTAs take shares of a tile's keys, leave fp32 partials (maximum, sum,
+// output) in the workspace, and a second kernel adds them in order, a warp a row.
+//
 // Warps: 4 softmax warps per query tile, one that loads queries and values, one that issues
 // the products, two that load keys.
 #include <algorithm>
@@ -63,6 +67,7 @@ struct PShape {
   static constexpr int THREADS = NQ * 128 + 128;
 };
 
+constexpr int kMinShare = 8;      // key tiles of a CTA where the keys are shared out
 constexpr int kLaunchRegs = 168;  // a thread's at launch, where warps shift registers: (208 + 208 + 88) / 3
 
 struct PromptArgs {
@@ -73,7 +78,8 @@ struct PromptArgs {
   const int32_t* lens;
   const int32_t* starts;
   int64_t o_row, o_head, table_row, room, total_q;
-  int batch, hkv, group, toks, tiles, d, page_size, num_pages, window, max_q;
+  float* part;  // splits > 1: [units][splits][rows][DP] outputs, then [units][splits][rows][2] (max, sum)
+  int batch, hkv, group, toks, tiles, d, page_size, num_pages, window, max_q, splits, units;
   int box;      // rows of a K / V box
   int one_box;  // a V box holds all column blocks of its rows
   float s2;  // scale * log2(e)
@@ -240,10 +246,20 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
   const int first = len - n_all + t0;                                    // its position
   const int end = len - n_all + min(n, t0 + NQ * a.toks);                 // one past the last query's
   const int lo = a.window > 0 ? max(0, first - a.window + 1) : 0;
-  const int j0 = lo / BN;
-  const int nt = end > 0 ? (end + BN - 1) / BN - j0 : 0;  // key tiles
+  const int all = end > 0 ? (end + BN - 1) / BN - lo / BN : 0;  // key tiles
+  // this CTA's share of them
+  const int share = max((all + a.splits - 1) / a.splits, kMinShare), split = static_cast<int>(blockIdx.y);
+  const int j0 = lo / BN + (a.splits > 1 ? split * share : 0);
+  const int nt = a.splits > 1 ? min(share, all - split * share) : all;
 
   uint16_t* outp = static_cast<uint16_t*>(a.out) + static_cast<int64_t>(head) * a.group * a.o_head;
+  const int64_t rows0 = (static_cast<int64_t>(blockIdx.x) * a.splits + split) * (NQ * 128);  // in the partials
+  float* const part_ml = a.part + static_cast<int64_t>(a.units) * a.splits * (NQ * 128) * DP;
+  if (nt <= 0 && a.splits > 1) {  // nothing of it is left for this CTA
+    for (int i = threadIdx.x; i < NQ * 128; i += C::THREADS)
+      *reinterpret_cast<float2*>(part_ml + (rows0 + i) * 2) = make_float2(-INFINITY, 0.f);
+    return;
+  }
   if (nt <= 0) {  // every query lies before position 0
     const int c8 = a.d / 8, cnt = min(NQ * a.toks, n - t0) * a.group * c8;
     for (int i = threadIdx.x; i < cnt; i += C::THREADS) {
@@ -523,7 +539,8 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
       static_assert((BN - 12) % 8 == 4, "the last four");
       mx[0] = max3(mx[0], s[BN - 4], s[BN - 3]);
       mx[1] = max3(mx[1], s[BN - 2], s[BN - 1]);
-      const float top = max3(fmaxf_nan(mx[0], mx[1]), mx[2], mx[3]) * s2;
+      // a row of no token of this sequence holds anything, and has no say in rescaling
+      const float top = live ? max3(fmaxf_nan(mx[0], mx[1]), mx[2], mx[3]) * s2 : -INFINITY;
       // rescale when the maximum has grown by more than kGrow (or is the first; a NaN stays one)
       float f = 1.f;
       if (!(top <= m + kGrow)) {
@@ -580,12 +597,20 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
       const float inv = l == 0.f ? 0.f : 1.f / l;
       uint16_t* dst = outp + static_cast<int64_t>(q0 + tok) * a.o_row + g * a.o_head;
       const uint32_t oc = lanes + C::OCOL + i * DP;
+      float* po = a.part + (rows0 + i * 128 + r) * DP;
+      if (a.splits > 1) *reinterpret_cast<float2*>(part_ml + (rows0 + i * 128 + r) * 2) = make_float2(m, l);
 #pragma unroll 1
       for (int c = 0; c < DP; c += 32) {
         uint32_t o[32];
         tmem_ld32(oc + c, o);
         tmem_wait_ld();
-        if (live) {
+        if (a.splits > 1) {
+          if (live) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<uint4*>(po + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          }
+        } else if (live) {
 #pragma unroll
           for (int e = 0; e < 32; e += 8) {
             if (c + e >= a.d) break;
@@ -613,6 +638,72 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
   }
 }
 
+// Adds the splits' partials of a row, in their order: one warp a row.
+template <int DP, int DT>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ PromptArgs a) {
+  using C = PShape<DP>;
+  constexpr int R = C::NQ * 128, V = DP / 32;  // rows of a unit, values of a lane
+  pdl_wait();
+  pdl_trigger();
+  const int lane = threadIdx.x & 31, r = static_cast<int>(blockIdx.y) * 8 + (threadIdx.x >> 5);
+  const int per = a.hkv * a.batch, bh = static_cast<int>(blockIdx.x) % per, b = bh / a.hkv, head = bh % a.hkv;
+  const int tile = a.tiles - 1 - static_cast<int>(blockIdx.x) / per;
+  const int q0 = a.starts[b], n_all = a.starts[b + 1] - q0;
+  const int n = q0 < 0 || q0 > a.total_q ? 0 : static_cast<int>(min(static_cast<int64_t>(min(n_all, a.max_q)), a.total_q - q0));
+  const int in = r % 128, tok = (tile * C::NQ + r / 128) * a.toks + in / a.group, g = in % a.group;
+  if (in >= a.toks * a.group || tok >= n) return;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.splits * R + r;
+  const float* ml = a.part + static_cast<int64_t>(a.units) * a.splits * R * DP;
+  float m = -INFINITY;
+  for (int s = lane; s < a.splits; s += 32) m = fmaxf(m, ml[(row0 + static_cast<int64_t>(s) * R) * 2]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+  const float z = m == -INFINITY ? 0.f : m;
+  float l = 0.f, acc[V] = {};
+#pragma unroll 4
+  for (int s = 0; s < a.splits; ++s) {
+    const int64_t row = row0 + static_cast<int64_t>(s) * R;
+    const float2 w = *reinterpret_cast<const float2*>(ml + row * 2);
+    if (w.x == -INFINITY) continue;  // it saw nothing, and wrote no output
+    const float f = exp2_fast(w.x - z);
+    l += w.y * f;
+#pragma unroll
+    for (int c = 0; c < V; c += 2) {
+      const float2 v = *reinterpret_cast<const float2*>(a.part + row * DP + (c / 2) * 64 + lane * 2);
+      acc[c] += v.x * f;
+      acc[c + 1] += v.y * f;
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint16_t* dst = static_cast<uint16_t*>(a.out) + static_cast<int64_t>(q0 + tok) * a.o_row +
+                  (static_cast<int64_t>(head) * a.group + g) * a.o_head;
+#pragma unroll
+  for (int c = 0; c < V; c += 2) {
+    const int col = (c / 2) * 64 + lane * 2;
+    if (col < a.d) *reinterpret_cast<uint32_t*>(dst + col) = pack16<DT>(l == 0.f ? 0.f : acc[c] * inv, l == 0.f ? 0.f : acc[c + 1] * inv);
+  }
+}
+
+// How the work of a call is cut: query tiles per sequence, CTAs for them, and, where those
+// leave SMs idle and the cache may be long, shares of the keys for several CTAs each.
+struct Cut {
+  int tiles, units, splits, rows, dp;
+  size_t bytes() const { return splits > 1 ? static_cast<size_t>(units) * splits * rows * (dp + 2) * 4 : 0; }
+};
+Cut cut_of(const ggufmm_attention_args& p, int sms) {
+  Cut c;
+  c.dp = p.head_dim <= 64 ? 64 : p.head_dim <= 128 ? 128 : 256;
+  const int nq = c.dp == 256 ? PShape<256>::NQ : PShape<128>::NQ, bn = c.dp == 256 ? PShape<256>::BN : PShape<128>::BN;
+  const int64_t toks = nq * (128 / (p.q_heads / p.kv_heads));
+  const int64_t tiles = (p.max_q + toks - 1) / toks, units = tiles * p.kv_heads * p.batch;
+  c.tiles = static_cast<int>(tiles);
+  c.units = static_cast<int>(units);
+  c.rows = nq * 128;
+  const int64_t longest = (p.table_width * p.page_size + bn - 1) / bn;
+  c.splits = units >= sms ? 1 : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sms / units, longest / kMinShare)));
+  return c;
+}
+
 bool encode(CUtensorMap* map, int64_t dtype, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
             const cuuint32_t* box) {
   PFN_encodeTiled enc = get_encode_fn();
@@ -625,7 +716,7 @@ bool encode(CUtensorMap* map, int64_t dtype, const void* base, int rank, const c
 }
 
 template <int DP, int DT>
-cudaError_t launch(const ggufmm_attention_args& p, cudaStream_t st) {
+cudaError_t launch(const ggufmm_attention_args& p, const Cut& cut, void* workspace, cudaStream_t st) {
   using C = PShape<DP>;
   const cuuint64_t d = static_cast<cuuint64_t>(p.head_dim), g = static_cast<cuuint64_t>(p.q_heads / p.kv_heads);
   PromptArgs a;
@@ -647,7 +738,10 @@ cudaError_t launch(const ggufmm_attention_args& p, cudaStream_t st) {
   a.group = static_cast<int>(g);
   a.toks = 128 / a.group;
   a.max_q = static_cast<int>(p.max_q);
-  a.tiles = (a.max_q + C::NQ * a.toks - 1) / (C::NQ * a.toks);
+  a.tiles = cut.tiles;
+  a.units = cut.units;
+  a.splits = cut.splits;
+  a.part = static_cast<float*>(workspace);
   a.d = static_cast<int>(p.head_dim);
   a.page_size = static_cast<int>(p.page_size);
   a.num_pages = static_cast<int>(p.num_pages);
@@ -655,8 +749,6 @@ cudaError_t launch(const ggufmm_attention_args& p, cudaStream_t st) {
   a.s2 = static_cast<float>(p.scale * 1.4426950408889634);
   a.box = 8;  // the largest run of rows up to a tile that divides a page
   while (a.box < C::BN && p.page_size % (2 * a.box) == 0) a.box *= 2;
-  const int64_t ctas = static_cast<int64_t>(a.tiles) * a.hkv * a.batch;
-  if (ctas > kI32Max) return cudaErrorInvalidConfiguration;
   CUtensorMap qm, vm;
   const cuuint64_t qd[4] = {d, g, static_cast<cuuint64_t>(p.kv_heads), static_cast<cuuint64_t>(p.total_q)};
   const cuuint64_t qs[3] = {static_cast<cuuint64_t>(p.q_head) * 2, static_cast<cuuint64_t>(p.q_head) * g * 2,
@@ -689,16 +781,25 @@ cudaError_t launch(const ggufmm_attention_args& p, cudaStream_t st) {
     if (C::NQ == 2 && fa.numRegs < kLaunchRegs) return cudaErrorInvalidKernelImage;
     ready.fetch_or(uint64_t(1) << (dev & 63), std::memory_order_release);
   }
-  return pdl_launch(fn, dim3(static_cast<unsigned>(ctas)), dim3(C::THREADS), C::SMEM, st, qm, vm, a);
+  e = pdl_launch(fn, dim3(static_cast<unsigned>(a.units), static_cast<unsigned>(a.splits)), dim3(C::THREADS), C::SMEM, st, qm,
+                 vm, a);
+  if (e != cudaSuccess || a.splits == 1) return e;
+  return pdl_launch(join_kernel<DP, DT>, dim3(static_cast<unsigned>(a.units), C::NQ * 16), dim3(256), 0, st, a);
 }
 
 }  // namespace
 
-cudaError_t launch_paged_prompt(const ggufmm_attention_args& p, cudaStream_t st) {
+size_t paged_prompt_workspace(const ggufmm_attention_args& p, int sms) { return cut_of(p, sms).bytes(); }
+
+cudaError_t launch_paged_prompt(const ggufmm_attention_args& p, int sms, void* workspace, size_t workspace_bytes,
+                                cudaStream_t st) {
+  Cut cut = cut_of(p, sms);
+  if (!workspace || workspace_bytes < cut.bytes()) cut.splits = 1;
   const bool f16 = p.dtype == GGUFMM_F16;
-  if (p.head_dim <= 64) return f16 ? launch<64, GGUFMM_F16>(p, st) : launch<64, GGUFMM_BF16>(p, st);
-  if (p.head_dim <= 128) return f16 ? launch<128, GGUFMM_F16>(p, st) : launch<128, GGUFMM_BF16>(p, st);
-  return f16 ? launch<256, GGUFMM_F16>(p, st) : launch<256, GGUFMM_BF16>(p, st);
+  if (cut.dp == 64) return f16 ? launch<64, GGUFMM_F16>(p, cut, workspace, st) : launch<64, GGUFMM_BF16>(p, cut, workspace, st);
+  if (cut.dp == 128)
+    return f16 ? launch<128, GGUFMM_F16>(p, cut, workspace, st) : launch<128, GGUFMM_BF16>(p, cut, workspace, st);
+  return f16 ? launch<256, GGUFMM_F16>(p, cut, workspace, st) : launch<256, GGUFMM_BF16>(p, cut, workspace, st);
 }
 
 cudaError_t attn_prompt_device_error(int* v, int clear, cudaStream_t st) { return tu_device_error(v, clear, st); }

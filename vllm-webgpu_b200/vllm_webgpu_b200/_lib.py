@@ -65,7 +65,8 @@ SIGNATURES = {
     "ggufmm_rope_append": (_I, [ctypes.c_char_p, _VP]),  # a packed ggufmm_rope_args
     "ggufmm_paged_attention_workspace_size": (_SZ, [_I64, _I64, _I64, _I64]),
     "ggufmm_paged_attention": (_I, [ctypes.c_char_p, _VP, _SZ, _VP]),  # a packed ggufmm_attention_args
-    "ggufmm_paged_prompt_attention": (_I, [ctypes.c_char_p, _VP]),
+    "ggufmm_paged_prompt_attention_workspace_size": (_SZ, [ctypes.c_char_p]),
+    "ggufmm_paged_prompt_attention": (_I, [ctypes.c_char_p, _VP, _SZ, _VP]),
     "ggufmm_gemm_noalloc": (_I, [_VP, _I, _I64, _I64, _VP, _I, _I64, _I64, _VP, _I, _I64, _VP]),
 }
 
