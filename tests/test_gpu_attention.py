@@ -302,6 +302,16 @@ def test_prompt_masked_out_rows(cuda):
     assert int(got[:5].count_nonzero()) == 0 and int(got[15:].count_nonzero()) == 0
 
 
+def test_prompt_widest_window(cuda):
+    """A window past every length hides nothing, at positions before 0 either."""
+    from vllm_webgpu_b200 import ops
+    c = Case([10, 300], 4, 1, 64, F16, 16, seed=5)
+    q = c.q(30)
+    starts = torch.tensor([0, 15, 30], dtype=torch.int32, device="cuda")
+    a, b = (ops.paged_prompt_attention(q, starts, 15, c.kc, c.vc, c.table, c.device_lens(), window=w) for w in (0, 2 ** 31 - 1))
+    assert torch.equal(a, b) and int(a[5:].count_nonzero()) > 0
+
+
 def test_prompt_agrees_with_single_tokens(cuda):
     from vllm_webgpu_b200 import ops
     c = Case([300], 8, 2, 128, F16, 16, seed=4)

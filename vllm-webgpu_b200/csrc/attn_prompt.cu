@@ -34,7 +34,11 @@
 //
 // Where the query tiles are fewer than the SMs and the cache may be long (a few new tokens on a
 // long text), several CTAs take shares of a tile's keys, leave fp32 partials (maximum, sum,
-// output) in the workspace, and a second kernel adds them in order, a warp a row.
+// output) in the workspace, and a second kernel adds them in order, a warp a row. How long the
+// texts are is known on the device alone, so a CTA takes at least kMinShare key tiles, and one
+// that gets them all writes the output itself. 32 / 8 heads of 128, shared out or not: 64 new
+// tokens on 32768 53 or 414 us, 4 on 131072 119 or 1629, 512 on 32768 226 or 416, 100 on 2000
+// 27 or 32; under 8 tiles the second launch costs 2 us of 14 for nothing.
 //
 // Warps: 4 softmax warps per query tile, one that loads queries and values, one that issues
 // the products, two that load keys.
@@ -84,6 +88,34 @@ struct PromptArgs {
   int one_box;  // a V box holds all column blocks of its rows
   float s2;  // scale * log2(e)
 };
+
+// What the CTAs of blockIdx.x work on: heads fastest, the longest (latest) tiles first.
+struct Unit {
+  int tile, b, head, q0, n, n_all, len;  // n: new tokens that there is room for, of n_all
+  int t0, first, end, lo;                // first token; its position, one past the last query's, first visible
+  int all, share;                        // key tiles, and those of a CTA
+};
+template <int DP>
+__device__ __forceinline__ Unit unit_of(const PromptArgs& a) {
+  using C = PShape<DP>;
+  Unit u;
+  const int per = a.hkv * a.batch, bh = static_cast<int>(blockIdx.x) % per;
+  u.tile = a.tiles - 1 - static_cast<int>(blockIdx.x) / per;
+  u.b = bh / a.hkv;
+  u.head = bh % a.hkv;
+  u.q0 = a.starts[u.b];
+  u.n_all = a.starts[u.b + 1] - u.q0;
+  u.n = u.q0 < 0 || u.q0 > a.total_q ? 0 : static_cast<int>(min(static_cast<int64_t>(min(u.n_all, a.max_q)), a.total_q - u.q0));
+  const int64_t len = a.lens[u.b];
+  u.len = static_cast<int>(len < 0 ? 0 : len > a.room ? a.room : len);
+  u.t0 = u.tile * C::NQ * a.toks;
+  u.first = u.len - u.n_all + u.t0;
+  u.end = u.len - u.n_all + min(u.n, u.t0 + C::NQ * a.toks);
+  u.lo = a.window > 0 ? max(0, u.first - a.window + 1) : 0;
+  u.all = u.end > 0 ? (u.end + C::BN - 1) / C::BN - u.lo / C::BN : 0;
+  u.share = a.splits > 1 ? max((u.all + a.splits - 1) / a.splits, kMinShare) : max(u.all, 1);
+  return u;
+}
 
 // A [tokens][64 columns] block of 128-byte rows read with the columns as the long (N)
 // dimension: 64-column blocks `block` bytes apart, groups of 8 tokens `group` apart.
@@ -231,31 +263,21 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
   const int warp = __shfl_sync(0xFFFFFFFFu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   pdl_wait();
 
-  // ---- what this CTA works on: heads fastest, the longest (latest) tiles first -----------
-  const int per = a.hkv * a.batch;
-  const int tile = a.tiles - 1 - static_cast<int>(blockIdx.x) / per;
-  const int bh = static_cast<int>(blockIdx.x) % per, b = bh / a.hkv, head = bh % a.hkv;
-  const int q0 = a.starts[b], n_all = a.starts[b + 1] - q0;
-  const int n = q0 < 0 || q0 > a.total_q ? 0 : static_cast<int>(min(static_cast<int64_t>(min(n_all, a.max_q)), a.total_q - q0));
-  const int64_t len64 = a.lens[b];
-  const int len = static_cast<int>(len64 < 0 ? 0 : len64 > a.room ? a.room : len64);
-  if (tile == 0 && head == 0 && threadIdx.x == 0 && (n < n_all || n_all < 0 || len < len64))
+  const Unit un = unit_of<DP>(a);
+  const int b = un.b, head = un.head, q0 = un.q0, n = un.n, n_all = un.n_all, len = un.len, t0 = un.t0, lo = un.lo;
+  if (un.tile == 0 && head == 0 && blockIdx.y == 0 && threadIdx.x == 0 && (n < n_all || n_all < 0 || len < a.lens[b]))
     atomicOr(&g_device_error, kErrIndex);
-  const int t0 = tile * NQ * a.toks;  // first token of the CTA
   if (t0 >= n) return;
-  const int first = len - n_all + t0;                                    // its position
-  const int end = len - n_all + min(n, t0 + NQ * a.toks);                 // one past the last query's
-  const int lo = a.window > 0 ? max(0, first - a.window + 1) : 0;
-  const int all = end > 0 ? (end + BN - 1) / BN - lo / BN : 0;  // key tiles
-  // this CTA's share of them
-  const int share = max((all + a.splits - 1) / a.splits, kMinShare), split = static_cast<int>(blockIdx.y);
-  const int j0 = lo / BN + (a.splits > 1 ? split * share : 0);
-  const int nt = a.splits > 1 ? min(share, all - split * share) : all;
+  // this CTA's share of the key tiles
+  const int split = static_cast<int>(blockIdx.y);
+  const int j0 = lo / BN + split * un.share, nt = min(un.share, un.all - split * un.share);
+  const bool parts = un.all > un.share;  // there are others
+  if (!parts && split > 0) return;
 
   uint16_t* outp = static_cast<uint16_t*>(a.out) + static_cast<int64_t>(head) * a.group * a.o_head;
   const int64_t rows0 = (static_cast<int64_t>(blockIdx.x) * a.splits + split) * (NQ * 128);  // in the partials
   float* const part_ml = a.part + static_cast<int64_t>(a.units) * a.splits * (NQ * 128) * DP;
-  if (nt <= 0 && a.splits > 1) {  // nothing of it is left for this CTA
+  if (nt <= 0 && parts) {  // nothing is left for this CTA
     for (int i = threadIdx.x; i < NQ * 128; i += C::THREADS)
       *reinterpret_cast<float2*>(part_ml + (rows0 + i) * 2) = make_float2(-INFINITY, 0.f);
     return;
@@ -598,13 +620,13 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
       uint16_t* dst = outp + static_cast<int64_t>(q0 + tok) * a.o_row + g * a.o_head;
       const uint32_t oc = lanes + C::OCOL + i * DP;
       float* po = a.part + (rows0 + i * 128 + r) * DP;
-      if (a.splits > 1) *reinterpret_cast<float2*>(part_ml + (rows0 + i * 128 + r) * 2) = make_float2(m, l);
+      if (parts) *reinterpret_cast<float2*>(part_ml + (rows0 + i * 128 + r) * 2) = make_float2(m, l);
 #pragma unroll 1
       for (int c = 0; c < DP; c += 32) {
         uint32_t o[32];
         tmem_ld32(oc + c, o);
         tmem_wait_ld();
-        if (a.splits > 1) {
+        if (parts) {
           if (live) {
 #pragma unroll
             for (int e = 0; e < 32; e += 4)
@@ -646,12 +668,10 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Promp
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31, r = static_cast<int>(blockIdx.y) * 8 + (threadIdx.x >> 5);
-  const int per = a.hkv * a.batch, bh = static_cast<int>(blockIdx.x) % per, b = bh / a.hkv, head = bh % a.hkv;
-  const int tile = a.tiles - 1 - static_cast<int>(blockIdx.x) / per;
-  const int q0 = a.starts[b], n_all = a.starts[b + 1] - q0;
-  const int n = q0 < 0 || q0 > a.total_q ? 0 : static_cast<int>(min(static_cast<int64_t>(min(n_all, a.max_q)), a.total_q - q0));
-  const int in = r % 128, tok = (tile * C::NQ + r / 128) * a.toks + in / a.group, g = in % a.group;
-  if (in >= a.toks * a.group || tok >= n) return;
+  const Unit un = unit_of<DP>(a);
+  if (un.t0 >= un.n || un.all <= un.share) return;  // nothing, or written by one CTA
+  const int in = r % 128, tok = un.t0 + r / 128 * a.toks + in / a.group, g = in % a.group;
+  if (in >= a.toks * a.group || tok >= un.n) return;
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.splits * R + r;
   const float* ml = a.part + static_cast<int64_t>(a.units) * a.splits * R * DP;
   float m = -INFINITY;
@@ -675,8 +695,8 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Promp
     }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  uint16_t* dst = static_cast<uint16_t*>(a.out) + static_cast<int64_t>(q0 + tok) * a.o_row +
-                  (static_cast<int64_t>(head) * a.group + g) * a.o_head;
+  uint16_t* dst = static_cast<uint16_t*>(a.out) + static_cast<int64_t>(un.q0 + tok) * a.o_row +
+                  (static_cast<int64_t>(un.head) * a.group + g) * a.o_head;
 #pragma unroll
   for (int c = 0; c < V; c += 2) {
     const int col = (c / 2) * 64 + lane * 2;
@@ -699,7 +719,8 @@ Cut cut_of(const ggufmm_attention_args& p, int sms) {
   c.tiles = static_cast<int>(tiles);
   c.units = static_cast<int>(units);
   c.rows = nq * 128;
-  const int64_t longest = (p.table_width * p.page_size + bn - 1) / bn;
+  int64_t longest = (p.table_width * p.page_size + bn - 1) / bn;
+  if (p.window > 0) longest = std::min<int64_t>(longest, (p.window + toks + bn - 1) / bn + 1);
   c.splits = units >= sms ? 1 : static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sms / units, longest / kMinShare)));
   return c;
 }
@@ -745,7 +766,7 @@ cudaError_t launch(const ggufmm_attention_args& p, const Cut& cut, void* workspa
   a.d = static_cast<int>(p.head_dim);
   a.page_size = static_cast<int>(p.page_size);
   a.num_pages = static_cast<int>(p.num_pages);
-  a.window = static_cast<int>(p.window);
+  a.window = p.window < a.room ? static_cast<int>(p.window) : 0;  // one as wide as the table hides nothing
   a.s2 = static_cast<float>(p.scale * 1.4426950408889634);
   a.box = 8;  // the largest run of rows up to a tile that divides a page
   while (a.box < C::BN && p.page_size % (2 * a.box) == 0) a.box *= 2;

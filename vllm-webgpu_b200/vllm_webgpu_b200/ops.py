@@ -979,12 +979,9 @@ def paged_prompt_attention(q: torch.Tensor, q_starts: torch.Tensor, max_q: int, 
     reference feeds a prompt token by token (run_inference.py:323-350)."""
     index, args, out, _, keep = _attention_args(q, k_cache, v_cache, block_tables, lens, scale, window, out, q_starts,
                                                 max_q)
-    ws = None
-    if max_q < 2048:  # few new tokens may share the keys of a long cache out: scratch for this call alone
-        with torch.cuda.device(index):
-            need = int(_lib.lib().ggufmm_paged_prompt_attention_workspace_size(args))
-        if need:
-            ws = torch.empty(need, dtype=torch.uint8, device=out.device)
+    with torch.cuda.device(index):  # few new tokens may share the keys of a long cache out: scratch for this call alone
+        need = int(_lib.lib().ggufmm_paged_prompt_attention_workspace_size(args))
+    ws = torch.empty(need, dtype=torch.uint8, device=out.device) if need else None
     _call(index, "ggufmm_paged_prompt_attention", args, None if ws is None else ws.data_ptr(),
           0 if ws is None else ws.numel())
     return out
