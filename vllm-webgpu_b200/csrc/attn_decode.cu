@@ -13,9 +13,9 @@
 // tokens; an item counts as one block more, for what it costs to begin and to end one. Every
 // CTA (one per SM) takes an equal run of consecutive blocks, whatever sequences they belong
 // to, so ragged lengths leave no SM idle; it finds its run by a sum over the lengths on the
-// device. An item inside one run is written directly. An item that crosses runs leaves fp32 partials (m, sum, o) in the workspace, and the last of its CTAs
-// to finish (a counter) adds them in the order of the CTAs, so the result does not depend
-// on which was last. (Handing part of the work out in short runs as CTAs finish was measured:
+// device. An item inside one run is written directly. An item that crosses runs leaves fp32
+// partials (m, sum, o) in the workspace, and the last of its CTAs to finish (a counter) adds
+// them in the order of the CTAs, so the result does not depend on which was last. (Handing part of the work out in short runs as CTAs finish was measured:
 // 196 to 208 us for 64 sequences up to 8192 tokens against 195, 124 to 152 us for one of 131035
 // against 105, since every run costs a join.)
 //

@@ -12,7 +12,7 @@ On the matmul path Gemma 4 differs from Llama in two ways, both kept here:
 The reference's FFN activation shader for Gemma is the same gelu_mul
 (silu(gate) * up, shaders/generic/gelu_mul.wgsl:14-20) as Llama's, so the fused
 SwiGLU paths apply unchanged. The per-head norms, PLE block and logit softcap
-are outside the quantized-matmul path.
+are not built, so ``forward`` refuses.
 """
 from __future__ import annotations
 
