@@ -69,6 +69,29 @@ def test_in_place_and_strided(cuda, n):
     assert torch.equal(rw[:, :1], rw0[:, :1]) and torch.equal(rw[:, 1 + n:], rw0[:, 1 + n:])
 
 
+@pytest.mark.parametrize("n", [1, 2, 3, 5, 9, 15, 17, 250, 254, 1006, 1009, 1010, 1011, 1023, 4095, 16367, 16369, 16371])
+@pytest.mark.parametrize("xt,rt,yt,wt", [(F32, BF16, BF16, F32), (F16, None, F16, F16), (BF16, F32, F32, BF16)])
+def test_packed_rows_of_odd_width(cuda, n, xt, rt, yt, wt):
+    """Rows without a gap that begin anywhere between 16-byte boundaries, in place; what lies
+    behind the last row stays."""
+    from vllm_webgpu_b200 import ops
+    m = 11
+    store = _make(1, m * n + 64, xt, 8)[0]
+    x, behind = store[:m * n].view(m, n), store[m * n:].clone()
+    r = _make(m, n, rt, 9, 2.0) if rt is not None else None
+    w = (1 + _make(1, n, F32, 3, 0.1)[0]).to(wt)
+    s, y = _ref(x, w, 1e-5, r, 0.0)
+    want_ro = None if r is None else (x.float() + r.float()).to(rt)
+    same = xt == yt
+    got = ops.rms_norm(x, w, 1e-5, r, out=x if same else None, out_dtype=None if same else yt, residual_out=r)
+    if r is not None:
+        got, ro = got
+        assert torch.equal(ro, want_ro)
+    assert (got.data_ptr() == x.data_ptr()) == same
+    _check(got, y, n, yt)
+    assert torch.equal(store[m * n:], behind)
+
+
 def test_same_bits_on_every_call_and_row(cuda):
     """A row's result depends on that row alone, and not on the number of rows beside it."""
     from vllm_webgpu_b200 import ops

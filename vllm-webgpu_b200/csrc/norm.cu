@@ -10,8 +10,9 @@
 //
 // HBM bound: a row is read once, held in registers over the sum of its squares, and written.
 // 8192 rows of 4096, x in 32 bits, r, r' and y in bf16 (336 MB): 51.5 us, 6.5 TB/s, the measured
-// copy rate. One row takes 2.2 us, a launch and two memory latencies. Rows that do not start on
-// 16 bytes go value by value: 8192 rows of 4095 take 94 us.
+// copy rate. One row takes 2.2 us, a launch and two memory latencies. Rows of odd width start
+// between 16-byte boundaries: without gaps they are read by the tensor's aligned groups (8192 rows
+// of 4095: 59 us, 5.7 TB/s; 94 value by value, as rows with odd gaps still go).
 #include "mma16.cuh"
 
 namespace ggufmm {
@@ -103,30 +104,91 @@ __device__ __forceinline__ void store8(void* p, int t, int64_t i, const float* f
   }
 }
 
-// Rows of whole 16-byte groups. A row is held in the registers of WARP ? one warp : one
-// CTA, V groups of eight values a thread; XS, RS: bytes of a value of x and of r (0: none).
-template <int XS, int RS, int V, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : 1024) rms_norm_vec_kernel(const __grid_constant__ NormArgs a) {
+// The same of the tensor's last group, which ends behind it.
+template <int ES>
+__device__ __forceinline__ void raw_load_last(Raw8<ES>& d, const void* p, int64_t row, int i, int n) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(d.v);
+#pragma unroll
+  for (int e = 0; e < 2 * ES; ++e) u[e] = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if (i + e < 0 || i + e >= n) continue;
+    if (ES == 4) u[e] = static_cast<const uint32_t*>(p)[row + i + e];
+    else u[e / 2] |= static_cast<uint32_t>(static_cast<const uint16_t*>(p)[row + i + e]) << (e % 2 * 16);
+  }
+}
+
+__device__ __forceinline__ void store8_edge(void* p, int t, int64_t row, int i, int n, const float* f) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (i + e >= 0 && i + e < n) store_y_rt(p, t, row + i + e, f[e]);
+}
+
+__device__ __forceinline__ void weights8(const void* p, int t, int i, float* w) {
+  if (t == GGUFMM_F32) {
+    Raw8<4> q;
+    raw_load(q, p, i);
+    raw_float(q, t, w);
+  } else {
+    Raw8<2> q;
+    raw_load(q, p, i);
+    raw_float(q, t, w);
+  }
+}
+
+// Eight weights from i = 8 g - shift on, out of the two aligned groups that hold them (shift is
+// the same for a whole row). What lies outside the row is anything.
+__device__ __forceinline__ void weights8_shifted(const void* p, int t, int i, int shift, int n, float* w) {
+  const int at = i + shift;
+  float v[16], a[12], b[10];
+  weights8(p, t, at ? at - 8 : 0, v);
+  if (at + 8 <= n) {
+    weights8(p, t, at, v + 8);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[8 + e] = at + e < n ? load_y_rt(p, t, at + e) : 0.f;
+  }
+#pragma unroll
+  for (int e = 0; e < 12; ++e) a[e] = shift & 4 ? v[e] : v[e + 4];
+#pragma unroll
+  for (int e = 0; e < 10; ++e) b[e] = shift & 2 ? a[e] : a[e + 2];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w[e] = shift & 1 ? b[e + 1] : b[e + 2];
+}
+
+// A row is held in the registers of WARP ? one warp : one CTA, V groups of eight values a
+// thread; XS, RS: bytes of a value of x and of r (0: none). Rows of whole 16-byte groups, or,
+// SHIFT, rows of any width from 8 without a gap: the groups are then those of the whole tensor,
+// each on 16 bytes; what a row's first and last hold of its neighbours is read and dropped. (A
+// row's squares are then added in an order that depends on where it begins.)
+template <int XS, int RS, int V, bool WARP, bool SHIFT>
+__global__ void __launch_bounds__(WARP ? 256 : SHIFT ? 512 : 1024, SHIFT && V == 1 ? 3 : 1) rms_norm_vec_kernel(const __grid_constant__ NormArgs a) {
   __shared__ float part[32];
   pdl_wait();
   pdl_trigger();
   const int64_t row = WARP ? static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5) : blockIdx.x;
   if (row >= a.m) return;  // whole warps
   const int tid = WARP ? threadIdx.x & 31 : threadIdx.x, nt = WARP ? 32 : blockDim.x;
+  const int shift = SHIFT ? static_cast<int>(row * a.n & 7) : 0;
+  auto inside = [&](int i) { return !SHIFT || (i >= 0 && i + 8 <= a.n); };
   Raw8<XS> xr[V];
   Raw8<RS> rr[V];
 #pragma unroll
   for (int k = 0; k < V; ++k) {
-    const int i = (tid + k * nt) * 8;
-    if (i < a.n) {
+    const int i = (tid + k * nt) * 8 - shift;
+    if (i >= a.n) continue;
+    if (!SHIFT || row + 1 < a.m || i + 8 <= a.n) {
       raw_load(xr[k], a.x, row * a.ldx + i);
       if constexpr (RS != 0) raw_load(rr[k], a.r, row * a.ldr + i);
+    } else {
+      raw_load_last(xr[k], a.x, row * a.ldx, i, a.n);
+      if constexpr (RS != 0) raw_load_last(rr[k], a.r, row * a.ldr, i, a.n);
     }
   }
   float s[V][8], ss = 0.f;
 #pragma unroll
   for (int k = 0; k < V; ++k) {
-    const int i = (tid + k * nt) * 8;
+    const int i = (tid + k * nt) * 8 - shift;
     if (i < a.n) {
       raw_float(xr[k], a.xt, s[k]);
       if constexpr (RS != 0) {
@@ -134,36 +196,39 @@ __global__ void __launch_bounds__(WARP ? 256 : 1024) rms_norm_vec_kernel(const _
         raw_float(rr[k], a.rt, r);
 #pragma unroll
         for (int e = 0; e < 8; ++e) s[k][e] += r[e];
-        if (a.ro) store8(a.ro, a.rt, row * a.ldro + i, s[k]);
+        if (a.ro) {
+          if (inside(i)) store8(a.ro, a.rt, row * a.ldro + i, s[k]);
+          else store8_edge(a.ro, a.rt, row * a.ldro, i, a.n, s[k]);
+        }
       }
+      if (inside(i)) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(s[k][e], s[k][e], ss);
+        for (int e = 0; e < 8; ++e) ss = fmaf(s[k][e], s[k][e], ss);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (i + e >= 0 && i + e < a.n) ss = fmaf(s[k][e], s[k][e], ss);
+      }
     }
   }
   ss = WARP ? warp_sum(ss) : cta_sum(ss, part);
   const float inv = rsqrtf(fmaf(ss, a.inv_n, a.eps));
 #pragma unroll
   for (int k = 0; k < V; ++k) {
-    const int i = (tid + k * nt) * 8;
+    const int i = (tid + k * nt) * 8 - shift;
     if (i < a.n) {
       float w[8];
       if (a.w) {
-        if (a.wt == GGUFMM_F32) {
-          Raw8<4> q;
-          raw_load(q, a.w, i);
-          raw_float(q, a.wt, w);
-        } else {
-          Raw8<2> q;
-          raw_load(q, a.w, i);
-          raw_float(q, a.wt, w);
-        }
+        if (SHIFT) weights8_shifted(a.w, a.wt, i, shift, a.n, w);
+        else weights8(a.w, a.wt, i, w);
 #pragma unroll
         for (int e = 0; e < 8; ++e) w[e] = s[k][e] * inv * (w[e] + a.c);
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) w[e] = s[k][e] * inv;
       }
-      store8(a.y, a.yt, row * a.ldy + i, w);
+      if (inside(i)) store8(a.y, a.yt, row * a.ldy + i, w);
+      else store8_edge(a.y, a.yt, row * a.ldy, i, a.n, w);
     }
   }
 }
@@ -249,13 +314,28 @@ cudaError_t launch_vec(const NormArgs& a, cudaStream_t st) {
   const int groups = a.n / 8;
   const dim3 rows8(static_cast<unsigned>((static_cast<int64_t>(a.m) + 7) / 8)), rows(static_cast<unsigned>(a.m));
   // a warp per row up to 1024 values, above it a CTA with two (up to 16384) or four groups
-  if (groups <= 32) return pdl_launch(rms_norm_vec_kernel<XS, RS, 1, true>, rows8, dim3(256), 0, st, a);
-  if (groups <= 64) return pdl_launch(rms_norm_vec_kernel<XS, RS, 2, true>, rows8, dim3(256), 0, st, a);
-  if (groups <= 128) return pdl_launch(rms_norm_vec_kernel<XS, RS, 4, true>, rows8, dim3(256), 0, st, a);
+  if (groups <= 32) return pdl_launch(rms_norm_vec_kernel<XS, RS, 1, true, false>, rows8, dim3(256), 0, st, a);
+  if (groups <= 64) return pdl_launch(rms_norm_vec_kernel<XS, RS, 2, true, false>, rows8, dim3(256), 0, st, a);
+  if (groups <= 128) return pdl_launch(rms_norm_vec_kernel<XS, RS, 4, true, false>, rows8, dim3(256), 0, st, a);
   const int v = groups <= 2048 ? 2 : 4;
   const dim3 block(static_cast<unsigned>(((groups + v - 1) / v + 31) / 32 * 32));
-  if (v == 2) return pdl_launch(rms_norm_vec_kernel<XS, RS, 2, false>, rows, block, 0, st, a);
-  return pdl_launch(rms_norm_vec_kernel<XS, RS, 4, false>, rows, block, 0, st, a);
+  if (v == 2) return pdl_launch(rms_norm_vec_kernel<XS, RS, 2, false, false>, rows, block, 0, st, a);
+  return pdl_launch(rms_norm_vec_kernel<XS, RS, 4, false, false>, rows, block, 0, st, a);
+}
+
+// One group a thread where that makes a CTA of up to 512: 38 registers, so that three of them hide
+// each other's loads, sums and weights (8192 bf16 rows of 4095 without r 45 us; two groups 54).
+template <int XS, int RS>
+cudaError_t launch_shift(const NormArgs& a, cudaStream_t st) {
+  const int groups = (a.n + 14) / 8;  // at the largest shift
+  if (groups <= 128)
+    return pdl_launch(rms_norm_vec_kernel<XS, RS, 4, true, true>, dim3(static_cast<unsigned>((static_cast<int64_t>(a.m) + 7) / 8)),
+                      dim3(256), 0, st, a);
+  const int v = groups <= 512 ? 1 : groups <= 1024 ? 2 : 4;
+  const dim3 rows(static_cast<unsigned>(a.m)), block(static_cast<unsigned>(((groups + v - 1) / v + 31) / 32 * 32));
+  if (v == 1) return pdl_launch(rms_norm_vec_kernel<XS, RS, 1, false, true>, rows, block, 0, st, a);
+  if (v == 2) return pdl_launch(rms_norm_vec_kernel<XS, RS, 2, false, true>, rows, block, 0, st, a);
+  return pdl_launch(rms_norm_vec_kernel<XS, RS, 4, false, true>, rows, block, 0, st, a);
 }
 
 cudaError_t launch_norm(const NormArgs& a, cudaStream_t st) {
@@ -270,6 +350,15 @@ cudaError_t launch_norm(const NormArgs& a, cudaStream_t st) {
     return x4 ? launch_vec<4, 2>(a, st) : launch_vec<2, 2>(a, st);
   }
   const bool x4 = a.xt == GGUFMM_F32;
+  auto packed = [&](const void* p, int64_t ld) {  // null, or on 16 bytes and without a gap
+    return !p || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld == a.n);
+  };
+  if (a.n >= 8 && a.n <= 16368 && packed(a.x, a.ldx) && packed(a.r, a.ldr) && packed(a.ro, a.ldro) && packed(a.w, a.n) &&
+      packed(a.y, a.ldy)) {
+    if (!a.r) return x4 ? launch_shift<4, 0>(a, st) : launch_shift<2, 0>(a, st);
+    if (a.rt == GGUFMM_F32) return x4 ? launch_shift<4, 4>(a, st) : launch_shift<2, 4>(a, st);
+    return x4 ? launch_shift<4, 2>(a, st) : launch_shift<2, 2>(a, st);
+  }
   if (!a.r) return x4 ? launch_any<4, 0>(a, st) : launch_any<2, 0>(a, st);
   if (a.rt == GGUFMM_F32) return x4 ? launch_any<4, 4>(a, st) : launch_any<2, 4>(a, st);
   return x4 ? launch_any<4, 2>(a, st) : launch_any<2, 2>(a, st);
