@@ -290,6 +290,27 @@ def test_prompt_keys_shared_out(cuda, hq, hkv, d, dtype, new, lens, window):
     assert torch.equal(a, b) and first.shape == a.shape
 
 
+@pytest.mark.parametrize("batch", [3, 40, 70])
+def test_prompt_mixed_lengths(cuda, batch):
+    """One long run of new tokens beside many short and empty ones, more work than SMs."""
+    new = [700 if b == batch // 2 else b % 4 for b in range(batch)]
+    lens = [n + (b * 37) % 300 for b, n in enumerate(new)]
+    _prompt(Case(lens, 8, 8, 64, BF16, 16, seed=batch), new, extra_max=5)
+
+
+def test_prompt_many_units_for_each_sm(cuda):
+    """Every CTA takes several pieces of work: a repeat gives the same bits."""
+    from vllm_webgpu_b200 import ops
+    n, b = 260, 48
+    c = Case([n] * b, 8, 4, 128, BF16, 16, seed=11)
+    new = [n] * b
+    first = _prompt(c, new)
+    q = c.q(n * b)
+    starts = torch.arange(0, n * b + 1, n, dtype=torch.int32, device="cuda")
+    x, y = (ops.paged_prompt_attention(q, starts, n, c.kc, c.vc, c.table, c.device_lens()) for _ in range(2))
+    assert torch.equal(x, y) and first.shape == x.shape
+
+
 def test_prompt_masked_out_rows(cuda):
     """More new tokens than the length holds: the queries before position 0 see nothing."""
     from vllm_webgpu_b200 import ops

@@ -26,8 +26,16 @@
 // than 2^8 since its last rescaling (the weights then reach at most 2^8, harmless in 32-bit
 // sums).
 //
-// 8192 tokens of 32 / 8 heads of 128: 425 us, 1294 TFLOP/s, 78% of the measured bf16 burst (called
-// for a second on end, under the power limit, 500 us, 77% of the sustained rate). Per 256 x 128
+// A CTA stays and takes one unit of work (a pair of query tiles) after another: when the loads of
+// one are under way its loading warp asks the hardware for a unit that no CTA has begun, so that
+// the loads and first scores of the next run under the last softmax and the output of this one.
+// One CTA per unit, or this: 2048 tokens 40.9 or 38.5 us, 8 prompts of 512 47 or 36, 32 of 128 38 or
+// 28, 8192 with a window of 1024 190 or 142; one short prompt, where a CTA has one unit, 0.3 us more.
+// Units are those of the sequences' own lengths, found on the device: 2048 new tokens beside 63
+// single ones take 112 us, 235 with units for the longest in every sequence.
+//
+// 8192 tokens of 32 / 8 heads of 128: 416 us, 1321 TFLOP/s, 79% of the measured bf16 burst (called
+// for a second on end, under the power limit, 485 us, 79% of the sustained rate). Per 256 x 128
 // scores the tensor core and the exponentials are each busy for about 2050 of 3100 clocks; what
 // is left is each tile's chain of load, maximum, exponentials and hand-over (2500). A
 // quarter of the exponentials as polynomials on the FMA units took 3% longer.
@@ -37,11 +45,13 @@
 // output) in the workspace, and a second kernel adds them in order, a warp a row. How long the
 // texts are is known on the device alone, so a CTA takes at least kMinShare key tiles, and one
 // that gets them all writes the output itself. 32 / 8 heads of 128, shared out or not: 64 new
-// tokens on 32768 53 or 414 us, 4 on 131072 119 or 1629, 512 on 32768 226 or 416, 100 on 2000
-// 27 or 32; under 8 tiles the second launch costs 2 us of 14 for nothing.
+// tokens on 32768 53 or 420 us, 4 on 131072 118 or 1650, 256 on 4096 32 or 56, 100 on 2000 28 or
+// 33; with less than 8 tiles in truth the second launch costs 4 us of 13 for nothing.
 //
 // Warps: 4 softmax warps per query tile, one that loads queries and values, one that issues
 // the products, two that load keys.
+#include <cuda/ptx>
+
 #include <algorithm>
 #include <atomic>
 
@@ -61,8 +71,9 @@ struct PShape {
   static constexpr int QB = 128 * DP * 2, KB = BN * DP * 2;
   static constexpr int SLOTS = DP == 64 ? 10 : 5;  // tiles of keys or values in flight
   static constexpr int BARS = NQ * QB + SLOTS * KB;
-  static constexpr int NBARS = 1 + 2 * SLOTS + 2 + 4 * NQ;
-  static constexpr int SMEM = BARS + NBARS * 8 + 16;
+  static constexpr int NBARS = 7 + 2 * SLOTS + 5 * NQ;
+  static constexpr int PLAN = (BARS + NBARS * 8 + 15) / 16 * 16;  // Plan, a 16-byte answer, a word
+  static constexpr int SMEM = PLAN + 64 + 16 + 16;
   static_assert(SMEM <= 232448, "a CTA's shared memory");
   // TMEM columns: one score buffer for all query tiles, their weights, their outputs
   static constexpr int PCOL = BN, OCOL = PCOL + NQ * BN / 2, COLS = 512;
@@ -89,33 +100,85 @@ struct PromptArgs {
   float s2;  // scale * log2(e)
 };
 
-// What the CTAs of blockIdx.x work on: heads fastest, the longest (latest) tiles first.
+// One unit of work: a pair (one) of query tiles of a sequence and kv head.
 struct Unit {
-  int tile, b, head, q0, n, n_all, len;  // n: new tokens that there is room for, of n_all
-  int t0, first, end, lo;                // first token; its position, one past the last query's, first visible
-  int all, share;                        // key tiles, and those of a CTA
+  int b, head, q0, n, base, len;  // n: new tokens that there is room for; base: position of the first
+  int t0, lo;                     // first token, first visible position
+  int all, share;                 // key tiles, and those of a CTA
 };
-template <int DP>
-__device__ __forceinline__ Unit unit_of(const PromptArgs& a) {
-  using C = PShape<DP>;
-  Unit u;
-  const int per = a.hkv * a.batch, bh = static_cast<int>(blockIdx.x) % per;
-  u.tile = a.tiles - 1 - static_cast<int>(blockIdx.x) / per;
-  u.b = bh / a.hkv;
-  u.head = bh % a.hkv;
-  u.q0 = a.starts[u.b];
-  u.n_all = a.starts[u.b + 1] - u.q0;
-  u.n = u.q0 < 0 || u.q0 > a.total_q ? 0 : static_cast<int>(min(static_cast<int64_t>(min(u.n_all, a.max_q)), a.total_q - u.q0));
-  const int64_t len = a.lens[u.b];
-  u.len = static_cast<int>(len < 0 ? 0 : len > a.room ? a.room : len);
-  u.t0 = u.tile * C::NQ * a.toks;
-  u.first = u.len - u.n_all + u.t0;
-  u.end = u.len - u.n_all + min(u.n, u.t0 + C::NQ * a.toks);
-  u.lo = a.window > 0 ? max(0, u.first - a.window + 1) : 0;
-  u.all = u.end > 0 ? (u.end + C::BN - 1) / C::BN - u.lo / C::BN : 0;
-  u.share = a.splits > 1 ? max((u.all + a.splits - 1) / a.splits, kMinShare) : max(u.all, 1);
-  return u;
+
+// The new tokens from q0 on that there is room for, of the n that the caller gives a sequence.
+__device__ __forceinline__ int new_tokens(const PromptArgs& a, int q0, int n) {
+  const int room = q0 < 0 || q0 > a.total_q ? 0 : static_cast<int>(min(static_cast<int64_t>(a.max_q), a.total_q - q0));
+  return max(min(n, room), 0);
 }
+
+// Unit x, by a warp: heads fastest, then the sequences that have a tile as late as this one, the
+// latest tiles (the longest) first. Sequences with few new tokens beside others with many take no
+// more units than they have tiles. False past the last one.
+template <int DP>
+__device__ __forceinline__ bool unit_of(const PromptArgs& a, int x, Unit& u) {
+  using C = PShape<DP>;
+  const int lane = threadIdx.x & 31, per = C::NQ * a.toks;
+  auto tiles_of = [&](int b) {
+    if (b >= a.batch) return 0;
+    const int q0 = a.starts[b];
+    return (new_tokens(a, q0, a.starts[b + 1] - q0) + per - 1) / per;
+  };
+  // the first 32 sequences stay in registers: one wait for memory, not three
+  const bool there = lane < a.batch;
+  const int start = there ? a.starts[lane] : 0, given = there ? a.starts[lane + 1] - start : 0, held = there ? a.lens[lane] : 0;
+  const int first = (new_tokens(a, start, given) + per - 1) / per;
+  auto count = [&](int tile) {  // of tiles from `tile` on, of all sequences
+    int c = max(first - tile, 0);
+    for (int b = 32 + lane; b < a.batch; b += 32) c += max(tiles_of(b) - tile, 0);
+    return __reduce_add_sync(0xFFFFFFFFu, c);
+  };
+  int at = x / a.hkv, tile = 0, after = 0;  // after: tiles behind `tile`
+  u.head = x % a.hkv;
+  if (at >= count(0)) return false;
+  for (int end = a.tiles; end - tile > 1;) {
+    const int mid = (tile + end) / 2, c = count(mid);
+    if (c > at) tile = mid;
+    else end = mid, after = c;
+  }
+  at -= after;
+  u.b = -1;
+  for (int b0 = 0; b0 < a.batch; b0 += 32) {
+    const bool has = (b0 ? tiles_of(b0 + lane) : first) > tile;
+    const uint32_t m = __ballot_sync(0xFFFFFFFFu, has);
+    const uint32_t me = __ballot_sync(0xFFFFFFFFu, has && __popc(m & ((1u << lane) - 1)) == at);
+    if (me) {
+      u.b = b0 + __ffs(me) - 1;
+      break;
+    }
+    at -= __popc(m);
+  }
+  if (u.b < 0) return false;
+  const bool early = u.b < 32;
+  u.q0 = early ? __shfl_sync(0xFFFFFFFFu, start, u.b & 31) : a.starts[u.b];
+  const int n = early ? __shfl_sync(0xFFFFFFFFu, given, u.b & 31) : a.starts[u.b + 1] - u.q0;
+  const int64_t len = early ? __shfl_sync(0xFFFFFFFFu, held, u.b & 31) : a.lens[u.b];
+  u.n = new_tokens(a, u.q0, n);
+  u.t0 = tile * per;
+  if (u.t0 >= u.n) return false;  // the lengths changed under the kernel
+  u.len = static_cast<int>(len < 0 ? 0 : len > a.room ? a.room : len);
+  u.base = u.len - n;
+  const int end = u.base + min(u.n, u.t0 + per);  // one past the last query's position
+  u.lo = a.window > 0 ? max(0, u.base + u.t0 - a.window + 1) : 0;
+  u.all = end > 0 ? (end + C::BN - 1) / C::BN - u.lo / C::BN : 0;
+  u.share = a.splits > 1 ? max((u.all + a.splits - 1) / a.splits, kMinShare) : max(u.all, 1);
+  return true;
+}
+
+// What the warp that loads tells the others of the CTA's next work.
+struct alignas(16) Plan {
+  int more;                        // 0: there is none
+  int rows, b, head, q0, n, base;  // rows: first of the partials; the rest as in Unit
+  int len, t0, lo, j0, nt, parts;  // key tiles j0 to j0 + nt; parts: others have more of them
+  int pad[3];
+};
+static_assert(sizeof(Plan) == 64, "of shared memory");
 
 // A [tokens][64 columns] block of 128-byte rows read with the columns as the long (N)
 // dimension: 64-column blocks `block` bytes apart, groups of 8 tokens `group` apart.
@@ -241,70 +304,65 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
+__device__ __forceinline__ void store32(void* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
+struct alignas(16) Answer {
+  long long x, y;
+};
+
 template <int DP, int DT>
 __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
-    paged_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ PromptArgs a) {
+    paged_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap vmap,
+                        const __grid_constant__ PromptArgs a) {
   using C = PShape<DP>;
   constexpr int NQ = C::NQ, BN = C::BN, NB = C::NB, SLOTS = C::SLOTS, OW = C::OW;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* sq = smem;
   uint8_t* ring = sq + NQ * C::QB;  // K(0), V(0), K(1), V(1), ... in turn
   uint64_t* qfull = reinterpret_cast<uint64_t*>(smem + C::BARS);
-  uint64_t* full = qfull + 1;
+  uint64_t* qfree = qfull + 1;    // the queries have been multiplied
+  uint64_t* full = qfree + 1;
   uint64_t* empty = full + SLOTS;
   uint64_t* vfix = empty + SLOTS;
   uint64_t* sfree = vfix + 1;     // the score buffer's content is in registers
-  uint64_t* sfull = sfree + 1;    // [NQ] a query tile's scores are in the buffer
+  uint64_t* told = sfree + 1;     // the plan is there
+  uint64_t* heard = told + 1;     // it has been read
+  uint64_t* next = heard + 1;     // the answer to the question for another unit
+  uint64_t* sfull = next + 1;     // [NQ] a query tile's scores are in the buffer
   uint64_t* odone = sfull + NQ;   // [NQ] a query tile's product with the values is done
-  uint64_t* pready = odone + NQ;  // [NQ][2] half of a query tile's weights
-  uint32_t* slot = reinterpret_cast<uint32_t*>(pready + 2 * NQ);
-  static_assert(3 + 2 * SLOTS + 4 * NQ == C::NBARS, "the barriers above");
+  uint64_t* ofree = odone + NQ;   // [NQ] a query tile's output has been read
+  uint64_t* pready = ofree + NQ;  // [NQ][2] half of a query tile's weights
+  static_assert(7 + 2 * SLOTS + 5 * NQ == C::NBARS, "the barriers above");
+  Plan* plan = reinterpret_cast<Plan*>(smem + C::PLAN);
+  uint4* answer = reinterpret_cast<uint4*>(plan + 1);
+  uint32_t* slot = reinterpret_cast<uint32_t*>(answer + 1);
   // the same in all lanes, and known to be: the products' operands then live in uniform registers
   const int warp = __shfl_sync(0xFFFFFFFFu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
-  pdl_wait();
-
-  const Unit un = unit_of<DP>(a);
-  const int b = un.b, head = un.head, q0 = un.q0, n = un.n, n_all = un.n_all, len = un.len, t0 = un.t0, lo = un.lo;
-  if (un.tile == 0 && head == 0 && blockIdx.y == 0 && threadIdx.x == 0 && (n < n_all || n_all < 0 || len < a.lens[b]))
-    atomicOr(&g_device_error, kErrIndex);
-  if (t0 >= n) return;
-  // this CTA's share of the key tiles
-  const int split = static_cast<int>(blockIdx.y);
-  const int j0 = lo / BN + split * un.share, nt = min(un.share, un.all - split * un.share);
-  const bool parts = un.all > un.share;  // there are others
-  if (!parts && split > 0) return;
-
-  uint16_t* outp = static_cast<uint16_t*>(a.out) + static_cast<int64_t>(head) * a.group * a.o_head;
-  const int64_t rows0 = (static_cast<int64_t>(blockIdx.x) * a.splits + split) * (NQ * 128);  // in the partials
-  float* const part_ml = a.part + static_cast<int64_t>(a.units) * a.splits * (NQ * 128) * DP;
-  if (nt <= 0 && parts) {  // nothing is left for this CTA
-    for (int i = threadIdx.x; i < NQ * 128; i += C::THREADS)
-      *reinterpret_cast<float2*>(part_ml + (rows0 + i) * 2) = make_float2(-INFINITY, 0.f);
-    return;
-  }
-  if (nt <= 0) {  // every query lies before position 0
-    const int c8 = a.d / 8, cnt = min(NQ * a.toks, n - t0) * a.group * c8;
-    for (int i = threadIdx.x; i < cnt; i += C::THREADS) {
-      const int c = i % c8, g = i / c8 % a.group, t = i / c8 / a.group;
-      *reinterpret_cast<uint4*>(outp + static_cast<int64_t>(q0 + t0 + t) * a.o_row + g * a.o_head + c * 8) =
-          make_uint4(0, 0, 0, 0);
-    }
-    return;
-  }
-
   if (smem_u32(smem) & 1023) {  // the swizzled tiles need it, and a CTA's memory starts so
     if (threadIdx.x == 0) atomicOr(&g_device_error, kErrIndex);
     return;
   }
   if (threadIdx.x == 0) {
     mbar_init(qfull, 1);
+    mbar_init(qfree, 1);
     for (int i = 0; i < SLOTS; ++i) mbar_init(full + i, 1), mbar_init(empty + i, 1);
     mbar_init(vfix, 1);
     mbar_init(sfree, 4);
-    for (int i = 0; i < NQ; ++i) mbar_init(sfull + i, 1), mbar_init(odone + i, 1);
+    mbar_init(told, 1);
+    mbar_init(heard, 3 + 4 * NQ);
+    mbar_init(next, 1);
+    for (int i = 0; i < NQ; ++i) mbar_init(sfull + i, 1), mbar_init(odone + i, 1), mbar_init(ofree + i, 4);
     for (int i = 0; i < 2 * NQ; ++i) mbar_init(pready + i, 4);
     fence_mbar_init();
   }
+  pdl_wait();
+  Unit u;
+  bool some = false;
+  if (warp == OW) some = unit_of<DP>(a, static_cast<int>(blockIdx.x), u);
   if (warp == OW + 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)),
                  "r"(static_cast<uint32_t>(C::COLS))
@@ -319,115 +377,191 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
   // grid must find that all of this grid's CTAs have theirs
   pdl_trigger();
 
+  // every other warp: the next plan; false where a wait ran out
+  auto hear = [&](Plan& p, int count) {
+    const bool ok = mbar_wait(told, count & 1);
+    if (!__all_sync(0xFFFFFFFFu, ok)) return false;
+    p = *plan;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(heard);
+    return true;
+  };
+
   // the softmax warps hold a row's scores in registers: they take what the others leave
   // (208 + 208 + 88 = 3 x 168, the launch's share)
   if (warp >= OW) {
-    const int32_t* row = a.tables + b * a.table_row;
     if (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp == OW) {
-      // ---- queries and values, by TMA ----------------------------------------------------
-      bool ok = true;
-      if (lane == 0) mbar_arrive_expect_tx(qfull, NQ * NB * a.toks * a.group * 128);
-      __syncwarp();
-      if (lane < NQ * NB) {
-        const int i = lane / NB, c = lane % NB;
-        tma_load_4d(sq + i * C::QB + c * (128 * 128), &qmap, c * 64, 0, head, q0 + t0 + i * a.toks, qfull);
-      }
+      // ---- what to do next; queries and values, by TMA ---------------------------------------
       // a lane's box of a tile: all column blocks of box rows, or one of them; and its page
       const int cols = a.one_box ? 1 : NB, boxes = cols * (BN / a.box), rb = lane / cols, cb = lane % cols;
-      auto page_of = [&](int j) {
-        const int tok = j * BN + rb * a.box;
-        if (lane >= boxes || tok >= len || tok + a.box <= lo) return a.num_pages;  // the box is filled with zeros
-        const int p = row[tok / a.page_size];
-        if (p >= 0 && p < a.num_pages) return p;
-        atomicOr(&g_device_error, kErrIndex);
-        return a.num_pages;
-      };
-      auto load = [&](uint8_t* dst, int j, int page, uint64_t* bar) {
-        if (lane == 0) mbar_arrive_expect_tx(bar, C::KB);
-        __syncwarp();
-        if (lane < boxes)
-          tma_load_5d(dst + (a.one_box ? rb * (a.box * NB * 128) : cb * (BN * 128) + rb * (a.box * 128)), &vmap, cb * 64,
-                      (j * BN + rb * a.box) % a.page_size, 0, head, page, bar);
-      };
-      int page = page_of(j0), sl = 1, last = -1;  // the values have every other tile of the ring
-      uint32_t par = 1;
-      for (int t = 0; t < nt; ++t) {
-        const int j = j0 + t, next = t + 1 < nt ? page_of(j + 1) : 0;
-        ok = mbar_wait(empty + sl, par);
-        if (!__all_sync(0xFFFFFFFFu, ok)) break;
-        uint8_t* dst = ring + sl * C::KB;
-        // tokens past the length that share a box with some before it may hold anything, NaN
-        // too, and a weight of 0 must meet 0: that tile's values are cleared there by hand
-        if ((j + 1) * BN > len && len % a.box) {
-          load(dst, j, page, vfix);
-          ok = mbar_wait(vfix, 0);  // at most once: it is the last tile of the sequence
-          if (!__all_sync(0xFFFFFFFFu, ok)) break;
-          const int r0 = len - j * BN, rows = (r0 + a.box - 1) / a.box * a.box - r0;
-          for (int x = lane; x < rows * NB * 8; x += 32) {
-            const int c = x / 8 % NB, r = r0 + x / 8 / NB;
-            const int at = a.one_box ? (r / a.box * NB + c) * (a.box * 128) + r % a.box * 128 : c * (BN * 128) + r * 128;
-            *reinterpret_cast<uint4*>(dst + at + x % 8 * 16) = make_uint4(0, 0, 0, 0);
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) mbar_arrive(full + sl);
-        } else {
-          load(dst, j, page, full + sl);
+      bool ok = true;
+      int x = static_cast<int>(blockIdx.x), split = static_cast<int>(blockIdx.y);
+      int plans = 0, works = 0, tiles = 0, fixes = 0, sl = 1;  // plans told, with key tiles; tiles loaded in all
+      uint32_t par = 1, asked = 0;
+      auto tell = [&](const Plan& p) {
+        if (plans) ok = mbar_wait(heard, (plans - 1) & 1);
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (!ok) return;
+        if (lane == 0) {
+          *plan = p;
+          mbar_arrive(told);
         }
-        page = next;
-        last = t;
-        sl += 2;
-        if (sl >= SLOTS) sl -= SLOTS, par ^= 1;
+        __syncwarp();
+        ++plans;
+      };
+      for (;;) {
+        Plan p;
+        if (some) {
+          p = {1,     a.splits > 1 ? (x * a.splits + split) * (NQ * 128) : 0, u.b, u.head, u.q0, u.n, u.base, u.len, u.t0, u.lo,
+               u.lo / BN + split * u.share, min(u.share, u.all - split * u.share), u.all > u.share, {}};
+          some = p.parts || split == 0;
+        }
+        if (some) tell(p);
+        if (some && ok && p.nt > 0) {
+          if (works) ok = mbar_wait(qfree, (works - 1) & 1);
+          if (!__all_sync(0xFFFFFFFFu, ok)) break;
+          if (lane == 0) mbar_arrive_expect_tx(qfull, NQ * NB * a.toks * a.group * 128);
+          __syncwarp();
+          if (lane < NQ * NB) {
+            const int i = lane / NB, c = lane % NB;
+            tma_load_4d(sq + i * C::QB + c * (128 * 128), &qmap, c * 64, 0, p.head, p.q0 + p.t0 + i * a.toks, qfull);
+          }
+          ++works;
+          const int32_t* row = a.tables + p.b * a.table_row;
+          auto page_of = [&](int j) {
+            const int tok = j * BN + rb * a.box;
+            if (lane >= boxes || tok >= p.len || tok + a.box <= p.lo) return a.num_pages;  // the box is filled with zeros
+            const int pg = row[tok / a.page_size];
+            if (pg >= 0 && pg < a.num_pages) return pg;
+            atomicOr(&g_device_error, kErrIndex);
+            return a.num_pages;
+          };
+          auto load = [&](uint8_t* dst, int j, int page, uint64_t* bar) {
+            if (lane == 0) mbar_arrive_expect_tx(bar, C::KB);
+            __syncwarp();
+            if (lane < boxes)
+              tma_load_5d(dst + (a.one_box ? rb * (a.box * NB * 128) : cb * (BN * 128) + rb * (a.box * 128)), &vmap, cb * 64,
+                          (j * BN + rb * a.box) % a.page_size, 0, p.head, page, bar);
+          };
+          int page = page_of(p.j0);  // the values have every other tile of the ring
+          for (int t = 0; t < p.nt; ++t) {
+            const int j = p.j0 + t, later = t + 1 < p.nt ? page_of(j + 1) : 0;
+            ok = mbar_wait(empty + sl, par);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (!ok) break;
+            uint8_t* dst = ring + sl * C::KB;
+            // tokens past the length that share a box with some before it may hold anything, NaN
+            // too, and a weight of 0 must meet 0: that tile's values are cleared there by hand
+            if ((j + 1) * BN > p.len && p.len % a.box) {
+              load(dst, j, page, vfix);
+              ok = mbar_wait(vfix, fixes++ & 1);
+              ok = __all_sync(0xFFFFFFFFu, ok);
+              if (!ok) break;
+              const int r0 = p.len - j * BN, rows = (r0 + a.box - 1) / a.box * a.box - r0;
+              for (int x8 = lane; x8 < rows * NB * 8; x8 += 32) {
+                const int c = x8 / 8 % NB, r = r0 + x8 / 8 / NB;
+                const int at = a.one_box ? (r / a.box * NB + c) * (a.box * 128) + r % a.box * 128 : c * (BN * 128) + r * 128;
+                *reinterpret_cast<uint4*>(dst + at + x8 % 8 * 16) = make_uint4(0, 0, 0, 0);
+              }
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              __syncwarp();
+              if (lane == 0) mbar_arrive(full + sl);
+            } else {
+              load(dst, j, page, full + sl);
+            }
+            page = later;
+            ++tiles;
+            sl += 2;
+            if (sl >= SLOTS) sl -= SLOTS, par ^= 1;
+          }
+        }
+        if (!ok) break;
+        // another unit, one that no CTA has begun; not earlier, since a free CTA would begin it sooner
+        if (lane == 0) {
+          mbar_arrive_expect_tx(next, 16);
+          cuda::ptx::clusterlaunchcontrol_try_cancel(answer, next);
+        }
+        __syncwarp();
+        ok = mbar_wait(next, asked++ & 1);
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (!ok) break;
+        const longlong2 got = *reinterpret_cast<const longlong2*>(answer);
+        const Answer ans{got.x, got.y};
+        if (!cuda::ptx::clusterlaunchcontrol_query_cancel_is_canceled(ans)) {
+          p = {};
+          tell(p);
+          break;
+        }
+        x = cuda::ptx::clusterlaunchcontrol_query_cancel_get_first_ctaid_x<int>(ans);
+        split = cuda::ptx::clusterlaunchcontrol_query_cancel_get_first_ctaid_y<int>(ans);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // read before it is written again
+        __syncwarp();
+        some = unit_of<DP>(a, x, u);
       }
-      if (!__all_sync(0xFFFFFFFFu, ok)) {  // a wait ran out: the copies still in flight
-        mbar_wait(qfull, 0);
-        for (int t = max(0, last - SLOTS / 2); t <= last; ++t)
+      if (blockIdx.x == 0 && blockIdx.y == 0)  // lengths that do not fit
+        for (int b = lane; b < a.batch; b += 32) {
+          const int q0 = a.starts[b], n = a.starts[b + 1] - q0;
+          if (n < 0 || n > new_tokens(a, q0, n) || a.lens[b] > a.room) atomicOr(&g_device_error, kErrIndex);
+        }
+      if (!ok) {  // a wait ran out: the copies still in flight
+        if (works) mbar_wait(qfull, (works - 1) & 1);
+        for (int t = max(0, tiles - 1 - SLOTS / 2); t < tiles; ++t)
           mbar_wait(full + (2 * t + 1) % SLOTS, (2 * t + 1) / SLOTS & 1);
       }
     } else if (warp >= OW + 2) {
-      // ---- keys, two warps in turn, by 16-byte copies: a TMA box of one 64-column block of a 16-token page is a
-      // request of 2 KB, and the unit takes about 134 clocks for each
+      // ---- keys, two warps in turn, by 16-byte copies: a TMA box of one 64-column block of a
+      // 16-token page is a request of 2 KB, and the unit takes about 134 clocks for each
       constexpr int CH = DP / 8, RPI = 32 / CH;  // 16-byte chunks of a row, rows of a warp's copy
       const int ch = lane % CH, sub = lane / CH;
       const bool col = ch * 8 < a.d;
-      const uint16_t* base = a.k + head * a.k_head + (col ? ch * 8 : 0);
-      // lane x: where tokens 8 x .. 8 x + 7 of a tile lie, negative where they are not read
-      auto place_of = [&](int j) -> int64_t {
-        const int tok = j * BN + lane * 8;
-        if (lane >= BN / 8 || tok >= len || tok + 8 <= lo) return -1;
-        const int p = row[tok / a.page_size];
-        if (p < 0 || p >= a.num_pages) return -1;  // reads as zeros; the values' warp reports it
-        return p * a.k_page + tok % a.page_size * a.k_slot;
-      };
       const uint32_t dst0 = smem_u32(ring) + (ch >> 3) * (BN * 128);
-      int64_t place = place_of(j0 + warp - OW - 2);
-      for (int t = warp - OW - 2; t < nt; t += 2) {
-        const int64_t next = t + 2 < nt ? place_of(j0 + t + 2) : 0;
-        const int sl = 2 * t % SLOTS;  // the keys have every other tile of the ring
-        if (!__all_sync(0xFFFFFFFFu, mbar_wait(empty + sl, (2 * t / SLOTS & 1) ^ 1))) break;
-        const uint32_t dst = dst0 + sl * C::KB;
+      Plan p;
+      bool ok = true;
+      for (int plans = 0, tiles = 0; ok && hear(p, plans) && p.more; ++plans) {
+        if (p.nt <= 0) continue;
+        const int32_t* row = a.tables + p.b * a.table_row;
+        const uint16_t* base = a.k + p.head * a.k_head + (col ? ch * 8 : 0);
+        // lane x: where tokens 8 x .. 8 x + 7 of a tile lie, negative where they are not read
+        auto place_of = [&](int j) -> int64_t {
+          const int tok = j * BN + lane * 8;
+          if (lane >= BN / 8 || tok >= p.len || tok + 8 <= p.lo) return -1;
+          const int pg = row[tok / a.page_size];
+          if (pg < 0 || pg >= a.num_pages) return -1;  // reads as zeros; the values' warp reports it
+          return pg * a.k_page + tok % a.page_size * a.k_slot;
+        };
+        int t = (warp - OW - 2) ^ (tiles & 1);
+        int64_t place = place_of(p.j0 + t);
+        for (; t < p.nt; t += 2) {
+          const int64_t later = t + 2 < p.nt ? place_of(p.j0 + t + 2) : 0;
+          const int at2 = 2 * (tiles + t), sl = at2 % SLOTS;  // the keys have every other tile of the ring
+          ok = mbar_wait(empty + sl, (at2 / SLOTS & 1) ^ 1);
+          ok = __all_sync(0xFFFFFFFFu, ok);
+          if (!ok) break;
+          const uint32_t dst = dst0 + sl * C::KB;
 #pragma unroll 4
-        for (int g = 0; g < BN / 8; ++g) {
-          const int64_t at = __shfl_sync(0xFFFFFFFFu, place, g);
-          const bool in = at >= 0 && col;
-          const uint16_t* src = in ? base + at : a.k;
-          const int64_t step = in ? a.k_slot : 0;
-          const uint32_t bytes = in ? 16 : 0;  // the rest of the 16 is filled with zeros
+          for (int g = 0; g < BN / 8; ++g) {
+            const int64_t at = __shfl_sync(0xFFFFFFFFu, place, g);
+            const bool in = at >= 0 && col;
+            const uint16_t* src = in ? base + at : a.k;
+            const int64_t step = in ? a.k_slot : 0;
+            const uint32_t bytes = in ? 16 : 0;  // the rest of the 16 is filled with zeros
 #pragma unroll
-          for (int x = 0; x < 8; x += RPI) {
-            const int r = x + sub;
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + (g * 8 + r) * 128 +
-                                                                              (((ch & 7) ^ r) << 4)),
-                         "l"(src + r * step), "r"(bytes)
-                         : "memory");
+            for (int x = 0; x < 8; x += RPI) {
+              const int r = x + sub;
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + (g * 8 + r) * 128 +
+                                                                                (((ch & 7) ^ r) << 4)),
+                           "l"(src + r * step), "r"(bytes)
+                           : "memory");
+            }
           }
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(full + sl);
+          place = later;
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(full + sl);
-        place = next;
+        tiles += p.nt;
       }
     } else if (warp == OW + 1) {
       // ---- products --------------------------------------------------------------------
@@ -444,8 +578,9 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
 #pragma unroll
       for (int k = 0; k < BN / 16; ++k)
         v_at[k] = ((16u * k >> vlog) * vbox + (16u * k & ((1u << vlog) - 1)) * 128) >> 4;
+      int tiles = 0, works = 0;              // key tiles of the units before, and those units
       auto qk = [&](int i, int t, int sl) {  // scores of query tile i, key tile t
-        const int use = t * NQ + i;  // of the score buffer: the one before must be in registers
+        const int use = (tiles + t) * NQ + i;  // of the score buffer: the one before must be in registers
         if (use && !mbar_wait(sfree, (use - 1) & 1)) return false;
         fence_after();
         const uint64_t qd = q_desc + i * (C::QB >> 4), kd = k_desc + static_cast<uint32_t>(sl * (C::KB >> 4));
@@ -464,9 +599,10 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
       // multiplied while the second is still being made
       auto pv = [&](int i, int t, int sl) {
         const uint64_t vd = v_desc + static_cast<uint32_t>(sl * (C::KB >> 4));
+        if (t == 0 && works && !mbar_wait(ofree + i, (works - 1) & 1)) return false;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          if (!mbar_wait(pready + i * 2 + h, t & 1)) return false;
+          if (!mbar_wait(pready + i * 2 + h, (tiles + t) & 1)) return false;
           fence_after();
           if (elect_one()) {
 #pragma unroll
@@ -491,162 +627,209 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
         if (elect_one()) umma_commit(empty + at);
         __syncwarp();
       };
-      int ks = 0, vs = 0;
-      bool ok = mbar_wait(qfull, 0) && wait_tile(ks);
-      for (int i = 0; i < NQ; ++i) ok = ok && qk(i, 0, ks);
-      if (ok) release(ks);
-      for (int t = 0; t < nt && ok; ++t) {
-        const bool more = t + 1 < nt;
-        ok = wait_tile(vs);
-        if (ok && more) ok = wait_tile(ks);
+      Plan p;
+      bool ok = true;
+      for (int plans = 0; ok && hear(p, plans) && p.more; ++plans) {
+        const int nt = p.nt;
+        if (nt <= 0) continue;
+        int ks = 0, vs = 0;
+        auto queries_done = [&]() {
+          if (elect_one()) umma_commit(qfree);
+          __syncwarp();
+        };
+        ok = mbar_wait(qfull, works & 1) && wait_tile(ks);
+        for (int i = 0; i < NQ; ++i) ok = ok && qk(i, 0, ks);
+        if (ok) release(ks);
+        if (ok && nt == 1) queries_done();
+        for (int t = 0; t < nt && ok; ++t) {
+          const bool more = t + 1 < nt;
+          ok = wait_tile(vs);
+          if (ok && more) ok = wait_tile(ks);
 #pragma unroll
-        for (int i = 0; i < NQ; ++i) {
-          if (more) {
-            ok = ok && qk(i, t + 1, ks);
-            if (ok && i == NQ - 1) release(ks);
+          for (int i = 0; i < NQ; ++i) {
+            if (more) {
+              ok = ok && qk(i, t + 1, ks);
+              if (ok && i == NQ - 1) {
+                release(ks);
+                if (t + 2 == nt) queries_done();
+              }
+            }
+            ok = ok && pv(i, t, vs);
           }
-          ok = ok && pv(i, t, vs);
+          if (ok) release(vs);
         }
-        if (ok) release(vs);
+        tiles += nt;
+        ++works;
       }
     }
   } else {
     if (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ---- softmax: thread r of a warpgroup has row r of its query tile ---------------------
     const int i = warp >> 2, r = (warp & 3) * 32 + lane;
-    const int tok = t0 + i * a.toks + r / a.group, g = r % a.group;
-    const bool live = r < a.toks * a.group && tok < n;
-    const int pos = len - n_all + tok;  // this row's position
-    const int pos_a = len - n_all + t0 + i * a.toks, pos_b = pos_a + a.toks - 1;  // the tile's first and last
     const uint32_t lanes = tmem + (static_cast<uint32_t>(warp & 3) << 21);
     // 16-bit floats underflow early (2^-24), and a long tail of small weights can add up: theirs
     // are kept 2^11 larger, the sum too, and rescaled when the maximum has grown by 2^4
     constexpr float kUp = DT == GGUFMM_F16 ? 11.f : 0.f, kGrow = DT == GGUFMM_F16 ? 4.f : 8.f;
     const bool odd_scale = a.s2 <= 0.f;
     const float s2 = odd_scale ? 1.f : a.s2;
-    float m = -INFINITY, l = 0.f;
+    float* const part_ml = a.part + static_cast<int64_t>(a.units) * a.splits * (NQ * 128) * DP;
+    const int mine = i * a.toks + r / a.group, g = r % a.group;  // token and head
+    // whole sectors, where the rows begin on them: half the requests, which bound the output's writing
+    const bool wide = (a.o_row | a.o_head | a.d) % 16 == 0 && reinterpret_cast<uintptr_t>(a.out) % 32 == 0;
     bool ok = true;
-    for (int t = 0; t < nt; ++t) {
-      ok = mbar_wait(sfull + i, t & 1);
-      ok = __all_sync(0xFFFFFFFFu, ok);
-      if (!ok) break;
-      fence_after();
-      uint32_t sr[BN];
-#pragma unroll
-      for (int c = 0; c < BN; c += 32) tmem_ld32(lanes + c, sr + c);
-      tmem_wait_ld();
-      fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(sfree);
-      float* s = reinterpret_cast<float*>(sr);
-      if (odd_scale) {
-#pragma unroll
-        for (int c = 0; c < BN; ++c) s[c] *= a.s2;
+    Plan p;
+    for (int plans = 0, tiles = 0; ok && hear(p, plans) && p.more; ++plans) {
+      uint16_t* const outp = static_cast<uint16_t*>(a.out) + static_cast<int64_t>(p.head) * a.group * a.o_head;
+      const int nt = p.nt;
+      if (nt <= 0 && p.parts) {  // nothing of the unit is left for this CTA
+        *reinterpret_cast<float2*>(part_ml + (static_cast<int64_t>(p.rows) + i * 128 + r) * 2) = make_float2(-INFINITY, 0.f);
+        continue;
       }
-      const int jb = (j0 + t) * BN;
-      const bool edge = jb + BN - 1 > pos_a || (a.window > 0 && jb <= pos_b - a.window);
-      if (edge) {
-        const int up = pos - jb, dn = a.window > 0 ? pos - a.window - jb : -1;  // visible: dn < c <= up
-#pragma unroll
-        for (int c = 0; c < BN; ++c)
-          if (c > up || c <= dn) s[c] = -INFINITY;
+      if (nt <= 0) {  // every query lies before position 0
+        const int c8 = a.d / 8, cnt = min(NQ * a.toks, p.n - p.t0) * a.group * c8;
+        for (int e = threadIdx.x; e < cnt; e += NQ * 128) {
+          const int c = e % c8, h = e / c8 % a.group, t = e / c8 / a.group;
+          *reinterpret_cast<uint4*>(outp + static_cast<int64_t>(p.q0 + p.t0 + t) * a.o_row + h * a.o_head + c * 8) =
+              make_uint4(0, 0, 0, 0);
+        }
+        continue;
       }
-      float mx[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) mx[e] = max3(s[e], s[4 + e], s[8 + e]);
-#pragma unroll
-      for (int c = 12; c + 8 <= BN; c += 8)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[c + e], s[c + 4 + e]);
-      static_assert((BN - 12) % 8 == 4, "the last four");
-      mx[0] = max3(mx[0], s[BN - 4], s[BN - 3]);
-      mx[1] = max3(mx[1], s[BN - 2], s[BN - 1]);
-      // a row of no token of this sequence holds anything, and has no say in rescaling
-      const float top = live ? max3(fmaxf_nan(mx[0], mx[1]), mx[2], mx[3]) * s2 : -INFINITY;
-      // rescale when the maximum has grown by more than kGrow (or is the first; a NaN stays one)
-      float f = 1.f;
-      if (!(top <= m + kGrow)) {
-        f = exp2_fast(m - top);  // 0 for the first
-        m = top == INFINITY ? __int_as_float(0x7FFFFFFF) : top;  // inf - inf
-        l *= f;
-      }
-      if (t > 0) {  // the product that reads the last weights, and adds to the output
-        ok = mbar_wait(odone + i, (t - 1) & 1);
+      const int tok = p.t0 + mine;
+      const bool live = r < a.toks * a.group && tok < p.n;
+      const int pos = p.base + tok;  // this row's position
+      const int pos_a = p.base + p.t0 + i * a.toks, pos_b = pos_a + a.toks - 1;  // the tile's first and last
+      const int j0 = p.j0;
+      float m = -INFINITY, l = 0.f;
+      for (int t = 0; t < nt; ++t) {
+        ok = mbar_wait(sfull + i, (tiles + t) & 1);
         ok = __all_sync(0xFFFFFFFFu, ok);
         if (!ok) break;
         fence_after();
+        uint32_t sr[BN];
+#pragma unroll
+        for (int c = 0; c < BN; c += 32) tmem_ld32(lanes + c, sr + c);
+        tmem_wait_ld();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(sfree);
+        float* s = reinterpret_cast<float*>(sr);
+        if (odd_scale) {
+#pragma unroll
+          for (int c = 0; c < BN; ++c) s[c] *= a.s2;
+        }
+        const int jb = (j0 + t) * BN;
+        const bool edge = jb + BN - 1 > pos_a || (a.window > 0 && jb <= pos_b - a.window);
+        if (edge) {
+          const int up = pos - jb, dn = a.window > 0 ? pos - a.window - jb : -1;  // visible: dn < c <= up
+#pragma unroll
+          for (int c = 0; c < BN; ++c)
+            if (c > up || c <= dn) s[c] = -INFINITY;
+        }
+        float mx[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx[e] = max3(s[e], s[4 + e], s[8 + e]);
+#pragma unroll
+        for (int c = 12; c + 8 <= BN; c += 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[c + e], s[c + 4 + e]);
+        static_assert((BN - 12) % 8 == 4, "the last four");
+        mx[0] = max3(mx[0], s[BN - 4], s[BN - 3]);
+        mx[1] = max3(mx[1], s[BN - 2], s[BN - 1]);
+        // a row of no token of this sequence holds anything, and has no say in rescaling
+        const float top = live ? max3(fmaxf_nan(mx[0], mx[1]), mx[2], mx[3]) * s2 : -INFINITY;
+        // rescale when the maximum has grown by more than kGrow (or is the first; a NaN stays one)
+        float f = 1.f;
+        if (!(top <= m + kGrow)) {
+          f = exp2_fast(m - top);  // 0 for the first
+          m = top == INFINITY ? __int_as_float(0x7FFFFFFF) : top;  // inf - inf
+          l *= f;
+        }
+        if (t > 0) {  // the product that reads the last weights, and adds to the output
+          ok = mbar_wait(odone + i, (tiles + t - 1) & 1);
+          ok = __all_sync(0xFFFFFFFFu, ok);
+          if (!ok) break;
+          fence_after();
+        }
+        if (t > 0 && __any_sync(0xFFFFFFFFu, f != 1.f)) {
+          const uint32_t oc = lanes + C::OCOL + i * DP;
+#pragma unroll 1
+          for (int c = 0; c < DP; c += 32) {
+            uint32_t o[32];
+            tmem_ld32(oc + c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tmem_st16(oc + c, o);
+            tmem_st16(oc + c + 16, o + 16);
+          }
+        }
+        const float z = (m == -INFINITY ? 0.f : m) - kUp;
+        uint64_t sum[2] = {0, 0};
+        auto handed = [&](int h) {  // half h of the weights is in tensor memory
+          tmem_wait_st();
+          fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(pready + i * 2 + h);
+        };
+        const uint32_t pc = lanes + C::PCOL + i * (BN / 2);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t w[BN / 4];
+          const float* v = s + h * (BN / 2);
+          weights<DT, BN / 2>(v, s2, z, w, sum);
+          if (h) handed(0);  // its store has had time to finish
+#pragma unroll
+          for (int c = 0; c < BN / 4; c += 16) tmem_st16(pc + h * (BN / 4) + c, w + c);
+        }
+        handed(1);
+        float a0, a1;
+        unpair(add2(sum[0], sum[1]), a0, a1);
+        l += a0 + a1;
       }
-      if (t > 0 && __any_sync(0xFFFFFFFFu, f != 1.f)) {
+      tiles += nt;
+      if (ok) ok = mbar_wait(odone + i, (tiles - 1) & 1);
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      if (ok) {
+        fence_after();
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        uint16_t* dst = outp + static_cast<int64_t>(p.q0 + tok) * a.o_row + g * a.o_head;
         const uint32_t oc = lanes + C::OCOL + i * DP;
+        const int64_t pr = static_cast<int64_t>(p.rows) + i * 128 + r;
+        float* po = a.part + pr * DP;
+        if (p.parts) *reinterpret_cast<float2*>(part_ml + pr * 2) = make_float2(m, l);
 #pragma unroll 1
         for (int c = 0; c < DP; c += 32) {
           uint32_t o[32];
           tmem_ld32(oc + c, o);
           tmem_wait_ld();
+          if (p.parts) {
+            if (live) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-          tmem_st16(oc + c, o);
-          tmem_st16(oc + c + 16, o + 16);
+              for (int e = 0; e < 32; e += 8) store32(po + c + e, o + e);
+            }
+          } else if (live) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 16) {
+              if (c + e >= a.d) break;
+              uint32_t w[8];
+#pragma unroll
+              for (int x = 0; x < 8; ++x) {
+                const float v0 = l == 0.f ? 0.f : __uint_as_float(o[e + 2 * x]) * inv;
+                const float v1 = l == 0.f ? 0.f : __uint_as_float(o[e + 2 * x + 1]) * inv;
+                w[x] = pack16<DT>(v0, v1);
+              }
+              if (wide) {
+                store32(dst + c + e, w);
+              } else {
+                *reinterpret_cast<uint4*>(dst + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                if (c + e + 8 < a.d) *reinterpret_cast<uint4*>(dst + c + e + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+              }
+            }
+          }
         }
-      }
-      const float z = (m == -INFINITY ? 0.f : m) - kUp;
-      uint64_t sum[2] = {0, 0};
-      auto handed = [&](int h) {  // half h of the weights is in tensor memory
-        tmem_wait_st();
         fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(pready + i * 2 + h);
-      };
-      const uint32_t pc = lanes + C::PCOL + i * (BN / 2);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t p[BN / 4];
-        const float* v = s + h * (BN / 2);
-        weights<DT, BN / 2>(v, s2, z, p, sum);
-        if (h) handed(0);  // its store has had time to finish
-#pragma unroll
-        for (int c = 0; c < BN / 4; c += 16) tmem_st16(pc + h * (BN / 4) + c, p + c);
-      }
-      handed(1);
-      float a0, a1;
-      unpair(add2(sum[0], sum[1]), a0, a1);
-      l += a0 + a1;
-    }
-    if (ok) ok = mbar_wait(odone + i, (nt - 1) & 1);
-    ok = __all_sync(0xFFFFFFFFu, ok);
-    if (ok) {
-      fence_after();
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      uint16_t* dst = outp + static_cast<int64_t>(q0 + tok) * a.o_row + g * a.o_head;
-      const uint32_t oc = lanes + C::OCOL + i * DP;
-      float* po = a.part + (rows0 + i * 128 + r) * DP;
-      if (parts) *reinterpret_cast<float2*>(part_ml + (rows0 + i * 128 + r) * 2) = make_float2(m, l);
-#pragma unroll 1
-      for (int c = 0; c < DP; c += 32) {
-        uint32_t o[32];
-        tmem_ld32(oc + c, o);
-        tmem_wait_ld();
-        if (parts) {
-          if (live) {
-#pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<uint4*>(po + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-          }
-        } else if (live) {
-#pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            if (c + e >= a.d) break;
-            uint4 v;
-            uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const float p = l == 0.f ? 0.f : __uint_as_float(o[e + 2 * x]) * inv;
-              const float q = l == 0.f ? 0.f : __uint_as_float(o[e + 2 * x + 1]) * inv;
-              w[x] = pack16<DT>(p, q);
-            }
-            *reinterpret_cast<uint4*>(dst + c + e) = v;
-          }
-        }
+        if (lane == 0) mbar_arrive(ofree + i);
       }
     }
     fence_before();
@@ -665,11 +848,21 @@ template <int DP, int DT>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ PromptArgs a) {
   using C = PShape<DP>;
   constexpr int R = C::NQ * 128, V = DP / 32;  // rows of a unit, values of a lane
+  __shared__ Unit un;
+  __shared__ int parts;
   pdl_wait();
   pdl_trigger();
   const int lane = threadIdx.x & 31, r = static_cast<int>(blockIdx.y) * 8 + (threadIdx.x >> 5);
-  const Unit un = unit_of<DP>(a);
-  if (un.t0 >= un.n || un.all <= un.share) return;  // nothing, or written by one CTA
+  if (threadIdx.x < 32) {
+    Unit u;
+    const bool some = unit_of<DP>(a, static_cast<int>(blockIdx.x), u);
+    if (lane == 0) {
+      if (some) un = u;
+      parts = some && u.all > u.share;
+    }
+  }
+  __syncthreads();
+  if (!parts) return;  // nothing, or written by one CTA
   const int in = r % 128, tok = un.t0 + r / 128 * a.toks + in / a.group, g = in % a.group;
   if (in >= a.toks * a.group || tok >= un.n) return;
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.splits * R + r;
@@ -700,7 +893,9 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Promp
 #pragma unroll
   for (int c = 0; c < V; c += 2) {
     const int col = (c / 2) * 64 + lane * 2;
-    if (col < a.d) *reinterpret_cast<uint32_t*>(dst + col) = pack16<DT>(l == 0.f ? 0.f : acc[c] * inv, l == 0.f ? 0.f : acc[c + 1] * inv);
+    if (col < a.d)
+      *reinterpret_cast<uint32_t*>(dst + col) =
+          pack16<DT>(l == 0.f ? 0.f : acc[c] * inv, l == 0.f ? 0.f : acc[c + 1] * inv);
   }
 }
 
@@ -715,7 +910,8 @@ Cut cut_of(const ggufmm_attention_args& p, int sms) {
   c.dp = p.head_dim <= 64 ? 64 : p.head_dim <= 128 ? 128 : 256;
   const int nq = c.dp == 256 ? PShape<256>::NQ : PShape<128>::NQ, bn = c.dp == 256 ? PShape<256>::BN : PShape<128>::BN;
   const int64_t toks = nq * (128 / (p.q_heads / p.kv_heads));
-  const int64_t tiles = (p.max_q + toks - 1) / toks, units = tiles * p.kv_heads * p.batch;
+  const int64_t tiles = (p.max_q + toks - 1) / toks;
+  const int64_t units = std::min(tiles * p.batch, (p.total_q + p.batch * (toks - 1)) / toks) * p.kv_heads;  // at most
   c.tiles = static_cast<int>(tiles);
   c.units = static_cast<int>(units);
   c.rows = nq * 128;
