@@ -12,7 +12,8 @@
 // Tiles: the G query heads of a kv head and floor(128 / G) consecutive tokens are the 128
 // rows of one query tile (row = token * G + head), so short prompts fill tiles and every key
 // is loaded once for the whole group. A CTA holds two query tiles (one for heads wider than
-// 128) and walks the keys 128 (64) at a time. Keys and values come page by page into swizzled
+// 128, or where no sequence has more new tokens than one holds: 4 on 131072 take 97 us with one,
+// 122 with two, 4 each of 32 on 2000 52 or 69) and walks the keys 128 (64) at a time. Keys and values come page by page into swizzled
 // tiles of one ring in shared memory; q k^T goes to TMEM, thread r of a softmax warpgroup
 // takes row r into registers, writes the weights to TMEM as 16-bit values, and the second
 // product reads them from there. Tensor memory holds two outputs of 128 columns, two sets of
@@ -45,7 +46,7 @@
 // output) in the workspace, and a second kernel adds them in order, a warp a row. How long the
 // texts are is known on the device alone, so a CTA takes at least kMinShare key tiles, and one
 // that gets them all writes the output itself. 32 / 8 heads of 128, shared out or not: 64 new
-// tokens on 32768 53 or 420 us, 4 on 131072 118 or 1650, 256 on 4096 32 or 56, 100 on 2000 28 or
+// tokens on 32768 53 or 420 us, 4 on 131072 97 or 1650, 256 on 4096 32 or 56, 100 on 2000 28 or
 // 33; with less than 8 tiles in truth the second launch costs 4 us of 13 for nothing.
 //
 // Warps: 4 softmax warps per query tile, one that loads queries and values, one that issues
@@ -54,6 +55,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "mma16.cuh"
 #include "paged.cuh"
@@ -63,13 +65,14 @@ namespace ggufmm {
 
 namespace {
 
-template <int DP>
+template <int DP, int QT>  // QT: query tiles of a CTA
 struct PShape {
-  static constexpr int NQ = DP == 256 ? 1 : 2;     // query tiles
+  static_assert(QT == 1 || (QT == 2 && DP < 256), "two outputs of 256 columns leave no room for scores");
+  static constexpr int NQ = QT;
   static constexpr int BN = DP == 256 ? 64 : 128;  // keys of a tile
   static constexpr int NB = DP / 64;               // 128-byte column blocks of a row
   static constexpr int QB = 128 * DP * 2, KB = BN * DP * 2;
-  static constexpr int SLOTS = DP == 64 ? 10 : 5;  // tiles of keys or values in flight
+  static constexpr int SLOTS = DP == 64 ? 10 : DP == 128 && QT == 1 ? 6 : 5;  // tiles of keys or values in flight
   static constexpr int BARS = NQ * QB + SLOTS * KB;
   static constexpr int NBARS = 7 + 2 * SLOTS + 5 * NQ;
   static constexpr int PLAN = (BARS + NBARS * 8 + 15) / 16 * 16;  // Plan, a 16-byte answer, a word
@@ -116,9 +119,9 @@ __device__ __forceinline__ int new_tokens(const PromptArgs& a, int q0, int n) {
 // Unit x, by a warp: heads fastest, then the sequences that have a tile as late as this one, the
 // latest tiles (the longest) first. Sequences with few new tokens beside others with many take no
 // more units than they have tiles. False past the last one.
-template <int DP>
+template <int DP, int QT>
 __device__ __forceinline__ bool unit_of(const PromptArgs& a, int x, Unit& u) {
-  using C = PShape<DP>;
+  using C = PShape<DP, QT>;
   const int lane = threadIdx.x & 31, per = C::NQ * a.toks;
   auto tiles_of = [&](int b) {
     if (b >= a.batch) return 0;
@@ -314,11 +317,11 @@ struct alignas(16) Answer {
   long long x, y;
 };
 
-template <int DP, int DT>
-__global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
+template <int DP, int QT, int DT>
+__global__ void __launch_bounds__(PShape<DP, QT>::THREADS, 1)
     paged_prompt_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap vmap,
                         const __grid_constant__ PromptArgs a) {
-  using C = PShape<DP>;
+  using C = PShape<DP, QT>;
   constexpr int NQ = C::NQ, BN = C::BN, NB = C::NB, SLOTS = C::SLOTS, OW = C::OW;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* sq = smem;
@@ -362,7 +365,7 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
   pdl_wait();
   Unit u;
   bool some = false;
-  if (warp == OW) some = unit_of<DP>(a, static_cast<int>(blockIdx.x), u);
+  if (warp == OW) some = unit_of<DP, QT>(a, static_cast<int>(blockIdx.x), u);
   if (warp == OW + 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)),
                  "r"(static_cast<uint32_t>(C::COLS))
@@ -497,7 +500,7 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
         split = cuda::ptx::clusterlaunchcontrol_query_cancel_get_first_ctaid_y<int>(ans);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // read before it is written again
         __syncwarp();
-        some = unit_of<DP>(a, x, u);
+        some = unit_of<DP, QT>(a, x, u);
       }
       if (blockIdx.x == 0 && blockIdx.y == 0)  // lengths that do not fit
         for (int b = lane; b < a.batch; b += 32) {
@@ -844,9 +847,9 @@ __global__ void __launch_bounds__(PShape<DP>::THREADS, 1)
 }
 
 // Adds the splits' partials of a row, in their order: one warp a row.
-template <int DP, int DT>
+template <int DP, int QT, int DT>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ PromptArgs a) {
-  using C = PShape<DP>;
+  using C = PShape<DP, QT>;
   constexpr int R = C::NQ * 128, V = DP / 32;  // rows of a unit, values of a lane
   __shared__ Unit un;
   __shared__ int parts;
@@ -855,7 +858,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Promp
   const int lane = threadIdx.x & 31, r = static_cast<int>(blockIdx.y) * 8 + (threadIdx.x >> 5);
   if (threadIdx.x < 32) {
     Unit u;
-    const bool some = unit_of<DP>(a, static_cast<int>(blockIdx.x), u);
+    const bool some = unit_of<DP, QT>(a, static_cast<int>(blockIdx.x), u);
     if (lane == 0) {
       if (some) un = u;
       parts = some && u.all > u.share;
@@ -902,14 +905,16 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Promp
 // How the work of a call is cut: query tiles per sequence, CTAs for them, and, where those
 // leave SMs idle and the cache may be long, shares of the keys for several CTAs each.
 struct Cut {
-  int tiles, units, splits, rows, dp;
+  int nq, tiles, units, splits, rows, dp;
   size_t bytes() const { return splits > 1 ? static_cast<size_t>(units) * splits * rows * (dp + 2) * 4 : 0; }
 };
 Cut cut_of(const ggufmm_attention_args& p, int sms) {
   Cut c;
   c.dp = p.head_dim <= 64 ? 64 : p.head_dim <= 128 ? 128 : 256;
-  const int nq = c.dp == 256 ? PShape<256>::NQ : PShape<128>::NQ, bn = c.dp == 256 ? PShape<256>::BN : PShape<128>::BN;
-  const int64_t toks = nq * (128 / (p.q_heads / p.kv_heads));
+  const int64_t one = 128 / (p.q_heads / p.kv_heads);
+  c.nq = c.dp == 256 || p.max_q <= one ? 1 : 2;
+  const int nq = c.nq, bn = c.dp == 256 ? PShape<256, 1>::BN : PShape<128, 2>::BN;
+  const int64_t toks = nq * one;
   const int64_t tiles = (p.max_q + toks - 1) / toks;
   const int64_t units = std::min(tiles * p.batch, (p.total_q + p.batch * (toks - 1)) / toks) * p.kv_heads;  // at most
   c.tiles = static_cast<int>(tiles);
@@ -932,9 +937,9 @@ bool encode(CUtensorMap* map, int64_t dtype, const void* base, int rank, const c
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int DP, int DT>
+template <int DP, int QT, int DT>
 cudaError_t launch(const ggufmm_attention_args& p, const Cut& cut, void* workspace, cudaStream_t st) {
-  using C = PShape<DP>;
+  using C = PShape<DP, QT>;
   const cuuint64_t d = static_cast<cuuint64_t>(p.head_dim), g = static_cast<cuuint64_t>(p.q_heads / p.kv_heads);
   PromptArgs a;
   a.out = p.out;
@@ -982,7 +987,7 @@ cudaError_t launch(const ggufmm_attention_args& p, const Cut& cut, void* workspa
                             static_cast<cuuint64_t>(p.v_page) * 2};
   const cuuint32_t vb[5] = {64, static_cast<cuuint32_t>(a.box), static_cast<cuuint32_t>(blocks), 1, 1};
   if (!encode(&qm, p.dtype, p.q, 4, qd, qs, qb) || !encode(&vm, p.dtype, p.v, 5, vd, vs, vb)) return cudaErrorInvalidValue;
-  auto fn = paged_prompt_kernel<DP, DT>;
+  auto fn = paged_prompt_kernel<DP, QT, DT>;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
@@ -1001,7 +1006,7 @@ cudaError_t launch(const ggufmm_attention_args& p, const Cut& cut, void* workspa
   e = pdl_launch(fn, dim3(static_cast<unsigned>(a.units), static_cast<unsigned>(a.splits)), dim3(C::THREADS), C::SMEM, st, qm,
                  vm, a);
   if (e != cudaSuccess || a.splits == 1) return e;
-  return pdl_launch(join_kernel<DP, DT>, dim3(static_cast<unsigned>(a.units), C::NQ * 16), dim3(256), 0, st, a);
+  return pdl_launch(join_kernel<DP, QT, DT>, dim3(static_cast<unsigned>(a.units), C::NQ * 16), dim3(256), 0, st, a);
 }
 
 }  // namespace
@@ -1013,10 +1018,16 @@ cudaError_t launch_paged_prompt(const ggufmm_attention_args& p, int sms, void* w
   Cut cut = cut_of(p, sms);
   if (!workspace || workspace_bytes < cut.bytes()) cut.splits = 1;
   const bool f16 = p.dtype == GGUFMM_F16;
-  if (cut.dp == 64) return f16 ? launch<64, GGUFMM_F16>(p, cut, workspace, st) : launch<64, GGUFMM_BF16>(p, cut, workspace, st);
+  auto sized = [&](auto dp, auto qt) {
+    constexpr int DP = decltype(dp)::value, QT = decltype(qt)::value;
+    return f16 ? launch<DP, QT, GGUFMM_F16>(p, cut, workspace, st) : launch<DP, QT, GGUFMM_BF16>(p, cut, workspace, st);
+  };
+  constexpr std::integral_constant<int, 1> one{};
+  constexpr std::integral_constant<int, 2> two{};
+  if (cut.dp == 64) return cut.nq == 1 ? sized(std::integral_constant<int, 64>{}, one) : sized(std::integral_constant<int, 64>{}, two);
   if (cut.dp == 128)
-    return f16 ? launch<128, GGUFMM_F16>(p, cut, workspace, st) : launch<128, GGUFMM_BF16>(p, cut, workspace, st);
-  return f16 ? launch<256, GGUFMM_F16>(p, cut, workspace, st) : launch<256, GGUFMM_BF16>(p, cut, workspace, st);
+    return cut.nq == 1 ? sized(std::integral_constant<int, 128>{}, one) : sized(std::integral_constant<int, 128>{}, two);
+  return sized(std::integral_constant<int, 256>{}, one);
 }
 
 cudaError_t attn_prompt_device_error(int* v, int clear, cudaStream_t st) { return tu_device_error(v, clear, st); }
