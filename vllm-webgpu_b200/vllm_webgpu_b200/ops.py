@@ -626,16 +626,20 @@ _current_device = torch._C._cuda_getDevice  # the callers' tensors are on a GPU:
 _native: dict = {}
 
 
-def _call(index: int, name: str, *args) -> None:
-    """The library's ``name``(*args, stream) with CUDA device ``index`` current, its status checked."""
+def _on_device(index: int, name: str, *args) -> int:
+    """The library's ``name``(*args) with CUDA device ``index`` current."""
     fn = _native.get(name)
     if fn is None:
         fn = _native[name] = getattr(_lib.lib(), name)
     if _current_device() == index:
-        st = fn(*args, _raw_stream(index))
-    else:
-        with torch.cuda.device(index):
-            st = fn(*args, _raw_stream(index))
+        return fn(*args)
+    with torch.cuda.device(index):
+        return fn(*args)
+
+
+def _call(index: int, name: str, *args) -> None:
+    """The library's ``name``(*args, stream) with CUDA device ``index`` current, its status checked."""
+    st = _on_device(index, name, *args, _raw_stream(index))
     if st:
         _lib.check(st, name)
 
@@ -979,8 +983,8 @@ def paged_prompt_attention(q: torch.Tensor, q_starts: torch.Tensor, max_q: int, 
     reference feeds a prompt token by token (run_inference.py:323-350)."""
     index, args, out, _, keep = _attention_args(q, k_cache, v_cache, block_tables, lens, scale, window, out, q_starts,
                                                 max_q)
-    with torch.cuda.device(index):  # few new tokens may share the keys of a long cache out: scratch for this call alone
-        need = int(_lib.lib().ggufmm_paged_prompt_attention_workspace_size(args))
+    # few new tokens may share the keys of a long cache out: scratch for this call alone
+    need = _on_device(index, "ggufmm_paged_prompt_attention_workspace_size", args)
     ws = torch.empty(need, dtype=torch.uint8, device=out.device) if need else None
     _call(index, "ggufmm_paged_prompt_attention", args, None if ws is None else ws.data_ptr(),
           0 if ws is None else ws.numel())
