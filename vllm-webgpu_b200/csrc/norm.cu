@@ -14,6 +14,7 @@
 // between 16-byte boundaries: without gaps they are read by the tensor's aligned groups (8192 rows
 // of 4095: 59 us, 5.7 TB/s; 94 value by value, as rows with odd gaps still go).
 #include "mma16.cuh"
+#include "shifted.cuh"
 
 namespace ggufmm {
 
@@ -136,26 +137,6 @@ __device__ __forceinline__ void weights8(const void* p, int t, int i, float* w) 
   }
 }
 
-// Eight weights from i = 8 g - shift on, out of the two aligned groups that hold them (shift is
-// the same for a whole row). What lies outside the row is anything.
-__device__ __forceinline__ void weights8_shifted(const void* p, int t, int i, int shift, int n, float* w) {
-  const int at = i + shift;
-  float v[16], a[12], b[10];
-  weights8(p, t, at ? at - 8 : 0, v);
-  if (at + 8 <= n) {
-    weights8(p, t, at, v + 8);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[8 + e] = at + e < n ? load_y_rt(p, t, at + e) : 0.f;
-  }
-#pragma unroll
-  for (int e = 0; e < 12; ++e) a[e] = shift & 4 ? v[e] : v[e + 4];
-#pragma unroll
-  for (int e = 0; e < 10; ++e) b[e] = shift & 2 ? a[e] : a[e + 2];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) w[e] = shift & 1 ? b[e + 1] : b[e + 2];
-}
-
 // A row is held in the registers of WARP ? one warp : one CTA, V groups of eight values a
 // thread; XS, RS: bytes of a value of x and of r (0: none). Rows of whole 16-byte groups, or,
 // SHIFT, rows of any width from 8 without a gap: the groups are then those of the whole tensor,
@@ -219,8 +200,11 @@ __global__ void __launch_bounds__(WARP ? 256 : SHIFT ? 512 : 1024, SHIFT && V ==
     if (i < a.n) {
       float w[8];
       if (a.w) {
-        if (SHIFT) weights8_shifted(a.w, a.wt, i, shift, a.n, w);
-        else weights8(a.w, a.wt, i, w);
+        if (SHIFT)
+          shifted8(i, shift, a.n, [&](int j, float* v) { weights8(a.w, a.wt, j, v); },
+                   [&](int j) { return load_y_rt(a.w, a.wt, j); }, w);
+        else
+          weights8(a.w, a.wt, i, w);
 #pragma unroll
         for (int e = 0; e < 8; ++e) w[e] = s[k][e] * inv * (w[e] + a.c);
       } else {
