@@ -93,9 +93,11 @@ int ggufmm_device_status(int clear, void* stream);
  * Poll limit of every bounded wait on the current device (0 restores the
  * default of 2^24 polls, seconds of waiting). A lower limit makes a wait that
  * can never complete -- a peer GPU that never publishes its partials in
- * ggufmm_gemv_allreduce -- give up within milliseconds; tests use it to check
- * that such a call returns, reports the timeout through ggufmm_device_status,
- * and leaves the context usable. Synchronous; call it between launches.
+ * ggufmm_gemv_allreduce -- give up within milliseconds, and a few polls the
+ * wait of ggufmm_paged_prompt_attention for more work (of calls made after it);
+ * tests use it to check that such a call returns, reports the timeout through
+ * ggufmm_device_status, and leaves the context usable. Synchronous; call it
+ * between launches.
  * No reference counterpart: the reference has no device-side waits.
  */
 int ggufmm_set_wait_limit(uint32_t polls);

@@ -74,7 +74,7 @@ struct PShape {
   static constexpr int QB = 128 * DP * 2, KB = BN * DP * 2;
   static constexpr int SLOTS = DP == 64 ? 10 : DP == 128 && QT == 1 ? 6 : 5;  // tiles of keys or values in flight
   static constexpr int BARS = NQ * QB + SLOTS * KB;
-  static constexpr int NBARS = 7 + 2 * SLOTS + 5 * NQ;
+  static constexpr int NBARS = 8 + 2 * SLOTS + 5 * NQ;
   static constexpr int PLAN = (BARS + NBARS * 8 + 15) / 16 * 16;  // Plan, a 16-byte answer, a word
   static constexpr int SMEM = PLAN + 64 + 16 + 16;
   static_assert(SMEM <= 232448, "a CTA's shared memory");
@@ -101,6 +101,7 @@ struct PromptArgs {
   int box;      // rows of a K / V box
   int one_box;  // a V box holds all column blocks of its rows
   float s2;  // scale * log2(e)
+  uint32_t polls;  // of the wait for another unit before it gives up, 0: mbar_wait's limit
 };
 
 // One unit of work: a pair (one) of query tiles of a sequence and kv head.
@@ -335,11 +336,12 @@ __global__ void __launch_bounds__(PShape<DP, QT>::THREADS, 1)
   uint64_t* told = sfree + 1;     // the plan is there
   uint64_t* heard = told + 1;     // it has been read
   uint64_t* next = heard + 1;     // the answer to the question for another unit
-  uint64_t* sfull = next + 1;     // [NQ] a query tile's scores are in the buffer
+  uint64_t* drained = next + 1;   // after a wait that ran out: the products issued until then are done
+  uint64_t* sfull = drained + 1;  // [NQ] a query tile's scores are in the buffer
   uint64_t* odone = sfull + NQ;   // [NQ] a query tile's product with the values is done
   uint64_t* ofree = odone + NQ;   // [NQ] a query tile's output has been read
   uint64_t* pready = ofree + NQ;  // [NQ][2] half of a query tile's weights
-  static_assert(7 + 2 * SLOTS + 5 * NQ == C::NBARS, "the barriers above");
+  static_assert(8 + 2 * SLOTS + 5 * NQ == C::NBARS, "the barriers above");
   Plan* plan = reinterpret_cast<Plan*>(smem + C::PLAN);
   uint4* answer = reinterpret_cast<uint4*>(plan + 1);
   uint32_t* slot = reinterpret_cast<uint32_t*>(answer + 1);
@@ -358,6 +360,7 @@ __global__ void __launch_bounds__(PShape<DP, QT>::THREADS, 1)
     mbar_init(told, 1);
     mbar_init(heard, 3 + 4 * NQ);
     mbar_init(next, 1);
+    mbar_init(drained, 1);
     for (int i = 0; i < NQ; ++i) mbar_init(sfull + i, 1), mbar_init(odone + i, 1), mbar_init(ofree + i, 4);
     for (int i = 0; i < 2 * NQ; ++i) mbar_init(pready + i, 4);
     fence_mbar_init();
@@ -380,6 +383,7 @@ __global__ void __launch_bounds__(PShape<DP, QT>::THREADS, 1)
   // grid must find that all of this grid's CTAs have theirs
   pdl_trigger();
 
+  auto warp_wait = [](uint64_t* bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity)) != 0; };
   // every other warp: the next plan; false where a wait ran out
   auto hear = [&](Plan& p, int count) {
     const bool ok = mbar_wait(told, count & 1);
@@ -486,7 +490,10 @@ __global__ void __launch_bounds__(PShape<DP, QT>::THREADS, 1)
           cuda::ptx::clusterlaunchcontrol_try_cancel(answer, next);
         }
         __syncwarp();
-        ok = mbar_wait(next, asked++ & 1);
+        // (mbar_wait's own polls may each pause for longer than any wait in here takes: a limit on those
+        // does not make one run out)
+        ok = a.polls ? mbar_poll(next, asked & 1, a.polls) : mbar_wait(next, asked & 1);
+        ++asked;
         ok = __all_sync(0xFFFFFFFFu, ok);
         if (!ok) break;
         const longlong2 got = *reinterpret_cast<const longlong2*>(answer);
@@ -507,10 +514,12 @@ __global__ void __launch_bounds__(PShape<DP, QT>::THREADS, 1)
           const int q0 = a.starts[b], n = a.starts[b + 1] - q0;
           if (n < 0 || n > new_tokens(a, q0, n) || a.lens[b] > a.room) atomicOr(&g_device_error, kErrIndex);
         }
-      if (!ok) {  // a wait ran out: the copies still in flight
-        if (works) mbar_wait(qfull, (works - 1) & 1);
+      if (!ok) {  // a wait ran out: the copies and the answer still in flight
+        if (works) mbar_drain(qfull, (works - 1) & 1);
         for (int t = max(0, tiles - 1 - SLOTS / 2); t < tiles; ++t)
-          mbar_wait(full + (2 * t + 1) % SLOTS, (2 * t + 1) / SLOTS & 1);
+          mbar_drain(full + (2 * t + 1) % SLOTS, (2 * t + 1) / SLOTS & 1);
+        if (fixes) mbar_drain(vfix, (fixes - 1) & 1);
+        if (asked) mbar_drain(next, (asked - 1) & 1);
       }
     } else if (warp >= OW + 2) {
       // ---- keys, two warps in turn, by 16-byte copies: a TMA box of one 64-column block of a
@@ -568,7 +577,8 @@ __global__ void __launch_bounds__(PShape<DP, QT>::THREADS, 1)
       }
     } else if (warp == OW + 1) {
       // ---- products --------------------------------------------------------------------
-      // the whole warp walks the tiles, one elected lane issues
+      // the whole warp walks the tiles, one elected lane issues; all lanes agree on how a wait ended,
+      // or some would miss where the others elect
       constexpr uint32_t id_qk = idesc16<DT, BN, false>(), id_pv = idesc16<DT, DP, true>();
       // a V tile: boxes of all column blocks one after the other, or one block after the other
       const uint32_t vblock = a.one_box ? a.box * 128 : BN * 128;
@@ -584,7 +594,7 @@ __global__ void __launch_bounds__(PShape<DP, QT>::THREADS, 1)
       int tiles = 0, works = 0;              // key tiles of the units before, and those units
       auto qk = [&](int i, int t, int sl) {  // scores of query tile i, key tile t
         const int use = (tiles + t) * NQ + i;  // of the score buffer: the one before must be in registers
-        if (use && !mbar_wait(sfree, (use - 1) & 1)) return false;
+        if (use && !warp_wait(sfree, (use - 1) & 1)) return false;
         fence_after();
         const uint64_t qd = q_desc + i * (C::QB >> 4), kd = k_desc + static_cast<uint32_t>(sl * (C::KB >> 4));
         if (elect_one()) {
@@ -602,10 +612,10 @@ __global__ void __launch_bounds__(PShape<DP, QT>::THREADS, 1)
       // multiplied while the second is still being made
       auto pv = [&](int i, int t, int sl) {
         const uint64_t vd = v_desc + static_cast<uint32_t>(sl * (C::KB >> 4));
-        if (t == 0 && works && !mbar_wait(ofree + i, (works - 1) & 1)) return false;
+        if (t == 0 && works && !warp_wait(ofree + i, (works - 1) & 1)) return false;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          if (!mbar_wait(pready + i * 2 + h, (tiles + t) & 1)) return false;
+          if (!warp_wait(pready + i * 2 + h, (tiles + t) & 1)) return false;
           fence_after();
           if (elect_one()) {
 #pragma unroll
@@ -621,7 +631,7 @@ __global__ void __launch_bounds__(PShape<DP, QT>::THREADS, 1)
       uint32_t par = 0;
       auto wait_tile = [&](int& at) {  // the next tile of the ring has arrived
         at = sl;
-        const bool ok = mbar_wait(full + sl, par);
+        const bool ok = warp_wait(full + sl, par);
         fence_after();
         if (++sl == SLOTS) sl = 0, par ^= 1;
         return ok;
@@ -632,7 +642,9 @@ __global__ void __launch_bounds__(PShape<DP, QT>::THREADS, 1)
       };
       Plan p;
       bool ok = true;
-      for (int plans = 0; ok && hear(p, plans) && p.more; ++plans) {
+      for (int plans = 0; ok; ++plans) {
+        ok = hear(p, plans);
+        if (!ok || !p.more) break;
         const int nt = p.nt;
         if (nt <= 0) continue;
         int ks = 0, vs = 0;
@@ -640,7 +652,7 @@ __global__ void __launch_bounds__(PShape<DP, QT>::THREADS, 1)
           if (elect_one()) umma_commit(qfree);
           __syncwarp();
         };
-        ok = mbar_wait(qfull, works & 1) && wait_tile(ks);
+        ok = warp_wait(qfull, works & 1) && wait_tile(ks);
         for (int i = 0; i < NQ; ++i) ok = ok && qk(i, 0, ks);
         if (ok) release(ks);
         if (ok && nt == 1) queries_done();
@@ -663,6 +675,11 @@ __global__ void __launch_bounds__(PShape<DP, QT>::THREADS, 1)
         }
         tiles += nt;
         ++works;
+      }
+      if (!ok) {  // a wait ran out: the products still in flight read and write this CTA's memory
+        if (elect_one()) umma_commit(drained);
+        __syncwarp();
+        mbar_drain(drained, 0);
       }
     }
   } else {
@@ -902,6 +919,8 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Promp
   }
 }
 
+std::atomic<uint32_t> lowered_polls{0};  // ggufmm_set_wait_limit's, 0 where it is not lowered
+
 // How the work of a call is cut: query tiles per sequence, CTAs for them, and, where those
 // leave SMs idle and the cache may be long, shares of the keys for several CTAs each.
 struct Cut {
@@ -969,6 +988,7 @@ cudaError_t launch(const ggufmm_attention_args& p, const Cut& cut, void* workspa
   a.num_pages = static_cast<int>(p.num_pages);
   a.window = p.window < a.room ? static_cast<int>(p.window) : 0;  // one as wide as the table hides nothing
   a.s2 = static_cast<float>(p.scale * 1.4426950408889634);
+  a.polls = lowered_polls.load(std::memory_order_relaxed);
   a.box = 8;  // the largest run of rows up to a tile that divides a page
   while (a.box < C::BN && p.page_size % (2 * a.box) == 0) a.box *= 2;
   CUtensorMap qm, vm;
@@ -1031,6 +1051,9 @@ cudaError_t launch_paged_prompt(const ggufmm_attention_args& p, int sms, void* w
 }
 
 cudaError_t attn_prompt_device_error(int* v, int clear, cudaStream_t st) { return tu_device_error(v, clear, st); }
-cudaError_t attn_prompt_set_wait_limit(uint32_t polls) { return tu_set_wait_limit(polls); }
+cudaError_t attn_prompt_set_wait_limit(uint32_t polls) {
+  lowered_polls.store(polls < kWaitLimit ? polls : 0, std::memory_order_relaxed);
+  return tu_set_wait_limit(polls);
+}
 
 }  // namespace ggufmm

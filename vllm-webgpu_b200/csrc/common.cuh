@@ -122,6 +122,19 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 
+// The same without the pause that try_wait may make (longer than a whole short kernel takes).
+__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
 // Returns false (and flags g_device_error) if the phase never completed.
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
   if (mbar_try_wait(bar, parity)) return true;  // the common case reads no limit
@@ -132,6 +145,20 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
   }
   atomicOr(&g_device_error, kErrWaitTimeout);
   return false;
+}
+
+// The same by polls that do not pause: a wait for what takes a microsecond runs out as well.
+__device__ __forceinline__ bool mbar_poll(uint64_t* bar, uint32_t parity, uint32_t polls) {
+  for (uint32_t i = 0; i < polls; ++i)
+    if (mbar_test_wait(bar, parity)) return true;
+  atomicOr(&g_device_error, kErrWaitTimeout);
+  return false;
+}
+
+// The wait of a kernel that leaves early (a wait of its own ran out) for what it has itself in
+// flight: that needs microseconds, and gets several milliseconds whatever limit is in force.
+__device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
+  for (uint32_t i = 0; i < 1u << 16 && !mbar_test_wait(bar, parity); ++i) __nanosleep(64);
 }
 
 // 1-D bulk copy global -> shared (size and both addresses 16-byte aligned).
