@@ -1,0 +1,119 @@
+"""What ``LlamaB200Model.forward`` takes from a file and a configuration, on the CPU: it applies a
+setting or a tensor, or it refuses it before the first kernel."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import gguf_oracle as O
+
+gguf = pytest.importorskip("gguf")
+
+HID, HEADS, KV, D, INTER, VOCAB = 64, 2, 1, 32, 96, 40
+TENSORS = {"token_embd.weight": (VOCAB, HID), "output.weight": (VOCAB, HID)}
+for _l in range(2):
+    TENSORS |= {f"blk.{_l}.attn_q.weight": (HEADS * D, HID), f"blk.{_l}.attn_k.weight": (KV * D, HID),
+                f"blk.{_l}.attn_v.weight": (KV * D, HID), f"blk.{_l}.attn_output.weight": (HID, HEADS * D),
+                f"blk.{_l}.ffn_gate.weight": (INTER, HID), f"blk.{_l}.ffn_up.weight": (INTER, HID),
+                f"blk.{_l}.ffn_down.weight": (HID, INTER)}
+NORMS = ["output_norm.weight"] + [f"blk.{_l}.{n}_norm.weight" for _l in range(2) for n in ("attn", "ffn")]
+
+
+def write_gguf(path, arch="llama", more=None, **fields):
+    """A whole small model as a GGUF file: all that a Llama layer has, and ``more`` ({name: array}).
+    ``fields``: metadata below the architecture's prefix, dots as two underscores."""
+    w = gguf.GGUFWriter(str(path), arch)
+    w.add_block_count(2)
+    w.add_embedding_length(HID)
+    w.add_feed_forward_length(INTER)
+    w.add_head_count(HEADS)
+    w.add_head_count_kv(KV)
+    w.add_key_length(D)
+    w.add_context_length(4096)
+    w.add_rope_freq_base(500000.0)
+    for name, value in fields.items():
+        key = f"{arch}.{name.replace('__', '.')}"
+        if isinstance(value, str):
+            w.add_string(key, value)
+        elif isinstance(value, int):
+            w.add_uint32(key, value)
+        else:
+            w.add_float32(key, value)
+    for i, (name, (n, k)) in enumerate(TENSORS.items()):
+        w.add_tensor(name, O.make_weights(n, k, O.Q8_0, seed=i), raw_dtype=gguf.GGMLQuantizationType(O.Q8_0))
+    for name in NORMS:
+        w.add_tensor(name, np.ones(HID, np.float32))
+    for name, value in (more or {}).items():
+        w.add_tensor(name, value)
+    w.write_header_to_file()
+    w.write_kv_data_to_file()
+    w.write_tensors_to_file()
+    w.close()
+    return str(path)
+
+
+def _model(path, cfg=None):
+    from vllm_webgpu_b200.models.llama import LlamaB200Model
+    from vllm_webgpu_b200.quant.gguf_loader import gguf_read_config
+    model = LlamaB200Model(gguf_read_config(path) if cfg is None else cfg, device="cpu")
+    model.load_weights(path)
+    return model
+
+
+def _forward(model):
+    from vllm_webgpu_b200.kv_cache import PagedKVCache
+    cache = PagedKVCache(2, 4, KV, D, 16, torch.float16, "cpu")
+    return model.forward(torch.zeros(3, dtype=torch.int64), None, cache.extend(["a"], [3]))
+
+
+def test_a_plain_file_gets_as_far_as_the_kernels(tmp_path):
+    with pytest.raises(ValueError, match="CUDA"):
+        _forward(_model(write_gguf(tmp_path / "m.gguf")))
+
+
+@pytest.mark.parametrize("name,size", [("blk.1.attn_q.bias", HEADS * D), ("blk.0.attn_k.bias", KV * D),
+                                       ("blk.0.attn_v.bias", KV * D), ("blk.1.attn_output.bias", HID),
+                                       ("blk.0.ffn_gate.bias", INTER), ("blk.1.ffn_up.bias", INTER),
+                                       ("blk.0.ffn_down.bias", HID), ("blk.0.attn_norm.bias", HID),
+                                       ("blk.0.post_ffw_norm.weight", HID), ("blk.1.layer_output_scale.weight", 1),
+                                       ("blk.1.attn_sinks.weight", HEADS), ("output.bias", VOCAB),
+                                       ("rope_factors_long.weight", D // 2)])
+def test_a_file_with_a_tensor_that_forward_leaves_out_is_refused(tmp_path, name, size):
+    model = _model(write_gguf(tmp_path / "m.gguf", arch="qwen2", more={name: np.zeros(size, np.float32)}))
+    with pytest.raises(NotImplementedError, match="tensors"):
+        _forward(model)
+
+
+def test_a_bias_is_loaded_under_its_name(tmp_path):
+    bias = np.arange(HEADS * D, dtype=np.float32)
+    model = _model(write_gguf(tmp_path / "m.gguf", arch="qwen2", more={"blk.1.attn_q.bias": bias}))
+    assert torch.equal(model.weights["model.layers.1.self_attn.q_proj.bias"], torch.from_numpy(bias))
+    with pytest.raises(NotImplementedError, match="bias"):
+        model.transformer_layer(1, torch.zeros(3, HID), None, type("Step", (), {"cache": type("Cache", (), {"dtype": torch.float16})}))
+
+
+def test_a_safetensors_bias_is_refused(tmp_path):
+    import json
+    import struct
+    header, data = {}, b""
+    for name, n in (("model.norm.weight", HID), ("model.layers.0.self_attn.q_proj.bias", HEADS * D)):
+        header[name] = {"dtype": "F16", "shape": [n], "data_offsets": [len(data), len(data) + 2 * n]}
+        data += np.ones(n, np.float16).tobytes()
+    head = json.dumps(header).encode()
+    p = tmp_path / "m.safetensors"
+    p.write_bytes(struct.pack("<Q", len(head)) + head + data)
+    with pytest.raises(NotImplementedError, match="q_proj.bias"):
+        _forward(_model(str(p), cfg={"num_hidden_layers": 2}))
+
+
+def test_weights_that_change_are_looked_over_again(tmp_path):
+    model = _model(write_gguf(tmp_path / "m.gguf"))
+    with pytest.raises(ValueError, match="CUDA"):
+        _forward(model)
+    model.weights["model.layers.0.self_attn.v_proj.bias"] = torch.zeros(KV * D)
+    with pytest.raises(NotImplementedError, match="v_proj.bias"):
+        _forward(model)
+    model.load_weights(write_gguf(tmp_path / "n.gguf", more={"blk.0.attn_k.bias": np.zeros(KV * D, np.float32)}))
+    with pytest.raises(NotImplementedError, match="k_proj.bias"):
+        _forward(model)

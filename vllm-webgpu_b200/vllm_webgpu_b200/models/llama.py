@@ -30,6 +30,12 @@ PROJ = {
 }
 
 
+# what ``forward`` reads of a layer, and beside the layers
+LAYER_WEIGHTS = {*PROJ.values(), "input_layernorm.weight", "post_attention_layernorm.weight", "self_attn.q_norm.weight",
+                 "self_attn.k_norm.weight"}
+OTHER_WEIGHTS = {"model.embed_tokens.weight", "model.norm.weight", "lm_head.weight", "rope_freqs.weight"}
+
+
 def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether two tensors share any bytes of storage."""
     if a.device != b.device or a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr():
@@ -163,6 +169,28 @@ class LlamaB200Model(BaseB200Model):
     def _head_dim(self) -> int:
         return int(self._cfg("head_dim") or self._cfg("hidden_size") // self._cfg("num_attention_heads"))
 
+    def _check_model(self) -> None:
+        """Refuse weights that ``forward`` would leave out: a bias, a norm that the Llama layer has
+        not, a tensor that the loader has no name for. Looked over again when weights change."""
+        weights = self.weights
+        seen = self.__dict__.get("_checked")
+        if seen is not None and seen[0] is weights and seen[1] == len(weights):
+            return
+        other = list(getattr(weights, "skipped", ()))
+        for name in weights:
+            parts = name.split(".", 3)
+            if name.startswith("model.layers.") and len(parts) == 4:
+                # (inv_freq: the rotary frequencies that some old files carry, made from the configuration here)
+                if parts[3] not in LAYER_WEIGHTS and not parts[3].endswith("rotary_emb.inv_freq"):
+                    other.append(name)
+            elif name not in OTHER_WEIGHTS:
+                other.append(name)
+        if other:
+            raise NotImplementedError("forward does not apply these of the model's tensors (a bias, a norm or a part that "
+                                      f"the Llama layer has not): {', '.join(sorted(other)[:4])}"
+                                      + (f" and {len(other) - 4} more" if len(other) > 4 else ""))
+        self._checked = (weights, len(weights))
+
     def transformer_layer(self, layer: int, hidden: torch.Tensor, delta, step) -> tuple[torch.Tensor, torch.Tensor]:
         """One layer over the tokens of ``step`` (``PagedKVCache.extend``). The residual
         stream is ``hidden`` [tokens, hidden size] plus ``delta``, the previous layer's FFN
@@ -172,8 +200,8 @@ class LlamaB200Model(BaseB200Model):
         eps, t, dev = float(self._cfg("rms_norm_eps", 1e-5)), hidden.shape[0], hidden.device
         cache, dtype = step.cache, step.cache.dtype
         base = f"model.layers.{layer}."
-        for name in ("q", "k", "v", "o"):
-            if base + f"self_attn.{name}_proj.bias" in self.weights:
+        for name in PROJ.values():
+            if base + name.replace(".weight", ".bias") in self.weights:
                 raise NotImplementedError("projections with a bias are not supported")
 
         def norm(x, name, residual):
@@ -214,6 +242,7 @@ class LlamaB200Model(BaseB200Model):
         reference's forward (vllm_webgpu/models/llama.py:145-237) runs one token of one
         sequence and returns its logits."""
         step = attn_metadata if positions is None else dataclasses.replace(attn_metadata, positions=positions)
+        self._check_model()
         layers = int(self._cfg("num_hidden_layers"))
         table = self.weights["model.embed_tokens.weight"]
         ids = input_ids.reshape(-1)

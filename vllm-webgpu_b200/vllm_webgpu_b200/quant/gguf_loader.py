@@ -47,6 +47,15 @@ def _device(device) -> torch.device:
     return torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
 
 
+class FileWeights(dict):
+    """Weights by name, as a file holds them, and what their names do not say: ``skipped``, the
+    file's tensors that the loader left out."""
+
+    def __init__(self) -> None:
+        super().__init__()
+        self.skipped: list[str] = []
+
+
 def load_safetensors_weights(path: str, device=None, quantize: str | None = None) -> dict:
     """Load a safetensors file to ``device``.
 
@@ -59,7 +68,7 @@ def load_safetensors_weights(path: str, device=None, quantize: str | None = None
         header_len = struct.unpack("<Q", f.read(8))[0]
         header = json.loads(f.read(header_len))
         raw_data = f.read()
-    weights: dict = {}
+    weights = FileWeights()
     for name, meta in header.items():
         if name == "__metadata__":
             continue
@@ -77,6 +86,7 @@ def load_safetensors_weights(path: str, device=None, quantize: str | None = None
             arr = np.clip(np.frombuffer(raw, dtype=np.float32), -65504.0, 65504.0).reshape(shape).astype(np.float16)
         else:
             logger.warning("Unsupported dtype %s for tensor %s, skipping", dtype_str, name)
+            weights.skipped.append(name)
             continue
         t = torch.from_numpy(np.ascontiguousarray(arr)).to(dev)
         if quantize and t.dim() == 2 and name.endswith("_proj.weight"):
@@ -92,9 +102,11 @@ def load_safetensors_weights_sharded(model_dir: str, device=None, quantize: str 
     index_path = Path(model_dir) / "model.safetensors.index.json"
     with open(index_path) as f:
         index = json.load(f)
-    weights: dict = {}
+    weights = FileWeights()
     for shard in sorted(set(index["weight_map"].values())):
-        weights.update(load_safetensors_weights(str(Path(model_dir) / shard), device, quantize))
+        part = load_safetensors_weights(str(Path(model_dir) / shard), device, quantize)
+        weights.update(part)
+        weights.skipped += part.skipped
     return weights
 
 
@@ -121,10 +133,11 @@ _GGUF_BLK = {
     "post_ffw_norm.weight": "post_feedforward_layernorm.weight",
     "layer_output_scale.weight": "self_attn.layer_scale",
 }
-
-
-# Not in the reference's table, but needed for right positions: the divisors of the rotary
-# frequencies that files of long-context models carry.
+# Not in the reference's table: the projections' biases, so that a model can tell that a file has
+# them, and the divisors of the rotary frequencies that files of long-context models carry, needed
+# for right positions.
+_GGUF_BLK |= {g.replace(".weight", ".bias"): h.replace(".weight", ".bias") for g, h in _GGUF_BLK.items()
+              if h.endswith("_proj.weight")}
 _GGUF_ROPE = "rope_freqs.weight"
 
 
@@ -154,12 +167,11 @@ def load_gguf_weights(path: str, device=None) -> dict:
         raise ImportError("Install the 'gguf' package to load GGUF files.") from e
     dev = _device(device)
     reader = gguf.GGUFReader(path)
-    weights: dict = {}
-    skipped = 0
+    weights = FileWeights()
     for tensor in reader.tensors:
         hf_name = _gguf_to_hf_name(tensor.name)
         if hf_name is None:
-            skipped += 1
+            weights.skipped.append(tensor.name)
             continue
         qt = int(tensor.tensor_type)
         shape = tuple(int(v) for v in reversed(list(tensor.shape)))  # GGML ne[] is innermost-first
@@ -177,7 +189,7 @@ def load_gguf_weights(path: str, device=None) -> dict:
         else:
             raise ValueError(f"{tensor.name}: GGUF type {gguf.GGMLQuantizationType(qt).name} is not "
                              f"supported by the B200 kernels (supported: Q4_0, Q8_0, Q4_K, Q6_K, F32, F16, BF16)")
-    logger.info("Loaded %d GGUF tensors (%d skipped) from %s", len(weights), skipped, path)
+    logger.info("Loaded %d GGUF tensors (%d skipped) from %s", len(weights), len(weights.skipped), path)
     return weights
 
 
