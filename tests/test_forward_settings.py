@@ -117,3 +117,11 @@ def test_weights_that_change_are_looked_over_again(tmp_path):
     model.load_weights(write_gguf(tmp_path / "n.gguf", more={"blk.0.attn_k.bias": np.zeros(KV * D, np.float32)}))
     with pytest.raises(NotImplementedError, match="k_proj.bias"):
         _forward(model)
+
+
+@pytest.mark.parametrize("arch,eps", [("qwen3", 1e-6), ("llama", 1e-5), ("qwen2", 3e-6)])
+def test_the_file_gives_the_norms_eps(tmp_path, arch, eps):
+    from vllm_webgpu_b200.quant.gguf_loader import gguf_read_config
+    model = _model(write_gguf(tmp_path / "m.gguf", arch, attention__layer_norm_rms_epsilon=eps))
+    assert model._cfg("rms_norm_eps") == np.float32(eps)
+    assert gguf_read_config(write_gguf(tmp_path / "n.gguf"))["rms_norm_eps"] is None

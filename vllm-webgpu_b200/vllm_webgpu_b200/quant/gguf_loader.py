@@ -195,7 +195,8 @@ def load_gguf_weights(path: str, device=None) -> dict:
 
 def gguf_read_config(path: str) -> dict:
     """Model configuration from GGUF metadata (reference gguf_loader.py:165-228):
-    same keys and defaults."""
+    same keys and defaults, and what ``forward`` needs beyond them, None where the
+    file does not say."""
     try:
         import gguf
     except ImportError as e:
@@ -230,6 +231,7 @@ def gguf_read_config(path: str) -> dict:
         "tie_word_embeddings": False,
         "final_logit_softcapping": _get(f"{p}.final_logit_softcapping"),
         "_gguf_arch_prefix": p,
+        "rms_norm_eps": _get(f"{p}.attention.layer_norm_rms_epsilon"),
     }
     if cfg["head_dim"] is None:
         cfg["head_dim"] = cfg["hidden_size"] // cfg["num_attention_heads"]
