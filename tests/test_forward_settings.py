@@ -125,3 +125,61 @@ def test_the_file_gives_the_norms_eps(tmp_path, arch, eps):
     model = _model(write_gguf(tmp_path / "m.gguf", arch, attention__layer_norm_rms_epsilon=eps))
     assert model._cfg("rms_norm_eps") == np.float32(eps)
     assert gguf_read_config(write_gguf(tmp_path / "n.gguf"))["rms_norm_eps"] is None
+
+
+def _turns(model):
+    """Radians per position of each pair as forward turns them, and the factor."""
+    steps, factor, _ = model._rope_plan()
+    turns = steps.numpy().view(np.uint64).astype(np.float64) * 2.0 ** -64
+    return np.minimum(turns, 1 - turns) * 2 * np.pi, factor
+
+
+def _plain(n=D, theta=500000.0):
+    return theta ** (-2.0 * np.arange(n // 2) / n)
+
+
+def _same(got, want):  # steps are rounded to 2^-64 of a turn, the file's numbers to 32 bits
+    assert np.allclose(got, want, rtol=1e-6, atol=1e-15)
+
+
+def test_the_file_gives_the_stretch_of_positions(tmp_path):
+    got, factor = _turns(_model(write_gguf(tmp_path / "plain.gguf")))
+    _same(got, _plain())
+    assert factor == 1.0
+    for name, fields in (("new", {"rope__scaling__type": "linear", "rope__scaling__factor": 4.0}),
+                         ("old", {"rope__scale_linear": 4.0})):
+        got, factor = _turns(_model(write_gguf(tmp_path / f"{name}.gguf", **fields)))
+        _same(got, _plain() / 4)
+        assert factor == 1.0
+    none = {"rope__scaling__type": "none", "rope__scaling__factor": 4.0}
+    _same(_turns(_model(write_gguf(tmp_path / "none.gguf", **none)))[0], _plain())
+
+
+@pytest.mark.parametrize("more,by,fast,slow", [
+    ({}, 1.0, 32.0, 1.0),
+    ({"rope__scaling__attn_factor": 0.75}, 0.75, 32.0, 1.0),
+    ({"rope__scaling__yarn_beta_fast": 16.0, "rope__scaling__yarn_beta_slow": 2.0}, 1.0, 16.0, 2.0),
+])
+def test_the_file_gives_yarn(tmp_path, more, by, fast, slow):
+    fields = {"rope__scaling__type": "yarn", "rope__scaling__factor": 8.0, "rope__scaling__original_context_length": 2048}
+    got, factor = _turns(_model(write_gguf(tmp_path / "m.gguf", **fields, **more)))
+    f = _plain()
+    # a pair that makes more than ``fast`` turns over the old context stays, below ``slow`` it is
+    # stretched whole; between the two by its index
+    pair = [D * np.log(2048 / (t * 2 * np.pi)) / (2 * np.log(500000.0)) for t in (fast, slow)]
+    low, high = max(np.floor(pair[0]), 0), min(np.ceil(pair[1]), D - 1)
+    ramp = np.clip((np.arange(D // 2) - low) / (high - low), 0, 1)
+    _same(got, f * (1 - ramp) + f / 8 * ramp)
+    assert factor == pytest.approx(by * (0.1 * np.log(8.0) + 1), rel=1e-6)
+
+
+def test_a_stretch_that_is_not_there_is_refused(tmp_path):
+    model = _model(write_gguf(tmp_path / "m.gguf", rope__scaling__type="longrope", rope__scaling__factor=4.0))
+    with pytest.raises(ValueError, match="longrope"):
+        model._rope_plan()
+
+
+def test_the_file_gives_the_rotary_width(tmp_path):
+    got, _ = _turns(_model(write_gguf(tmp_path / "m.gguf", rope__dimension_count=20)))
+    assert got.shape == (10,)
+    _same(got, _plain(20))

@@ -164,7 +164,8 @@ class LlamaB200Model(BaseB200Model):
         return plan
 
     def _rot_dim(self) -> int:
-        return int(self._head_dim() * float(self._cfg("partial_rotary_factor", 1.0)))
+        given = self._cfg("rotary_dim")
+        return int(given) if given is not None else int(self._head_dim() * float(self._cfg("partial_rotary_factor", 1.0)))
 
     def _head_dim(self) -> int:
         return int(self._cfg("head_dim") or self._cfg("hidden_size") // self._cfg("num_attention_heads"))

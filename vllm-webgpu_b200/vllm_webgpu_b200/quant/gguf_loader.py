@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import json
 import logging
+import math
 import struct
 from pathlib import Path
 
@@ -193,6 +194,29 @@ def load_gguf_weights(path: str, device=None) -> dict:
     return weights
 
 
+def _gguf_rope_scaling(get, get_str, context: int) -> dict | None:
+    """The file's stretch of the rotary positions as ``ops.rope_steps`` takes it, from the metadata
+    ``get(name)`` below the architecture's prefix. (llama3's stretch is in the file's
+    rope_freqs.weight.)"""
+    kind, factor = get_str("rope.scaling.type"), get("rope.scaling.factor")
+    if kind is None and get("rope.scale_linear") is not None:  # of older files
+        kind, factor = "linear", get("rope.scale_linear")
+    if kind in (None, "none") or (kind == "linear" and factor in (None, 0, 1)):
+        return None
+    scaling = {"rope_type": kind, "factor": factor or 1.0}
+    if kind == "yarn":
+        scaling["original_max_position_embeddings"] = get("rope.scaling.original_context_length") or context
+        for key, name in (("beta_fast", "rope.scaling.yarn_beta_fast"), ("beta_slow", "rope.scaling.yarn_beta_slow")):
+            if get(name) is not None:
+                scaling[key] = get(name)
+        by = get("rope.scaling.attn_factor")
+        if by is None:
+            by = get("rope.scaling.yarn_attn_factor")
+        if by is not None:  # a factor on yarn's own
+            scaling["attention_factor"] = by * (0.1 * math.log(scaling["factor"]) + 1.0 if scaling["factor"] > 1 else 1.0)
+    return scaling
+
+
 def gguf_read_config(path: str) -> dict:
     """Model configuration from GGUF metadata (reference gguf_loader.py:165-228):
     same keys and defaults, and what ``forward`` needs beyond them, None where the
@@ -215,6 +239,9 @@ def gguf_read_config(path: str) -> dict:
         v = _get(key)
         return bytes(v).decode("utf-8", errors="replace") if isinstance(v, list) else v
 
+    def _of(get):  # below the architecture's prefix
+        return lambda name: get(f"{p}.{name}")
+
     arch = _get("general.architecture")
     p = bytes(arch).decode() if isinstance(arch, list) else str(arch)
     cfg = {
@@ -232,7 +259,9 @@ def gguf_read_config(path: str) -> dict:
         "final_logit_softcapping": _get(f"{p}.final_logit_softcapping"),
         "_gguf_arch_prefix": p,
         "rms_norm_eps": _get(f"{p}.attention.layer_norm_rms_epsilon"),
+        "rotary_dim": _get(f"{p}.rope.dimension_count"),
     }
+    cfg["rope_scaling"] = _gguf_rope_scaling(_of(_get), _of(_get_str), cfg["max_position_embeddings"])
     if cfg["head_dim"] is None:
         cfg["head_dim"] = cfg["hidden_size"] // cfg["num_attention_heads"]
     arch_map = {"llama": "LlamaForCausalLM", "qwen3": "Qwen3ForCausalLM", "qwen2": "Qwen2ForCausalLM",
