@@ -183,3 +183,26 @@ def test_the_file_gives_the_rotary_width(tmp_path):
     got, _ = _turns(_model(write_gguf(tmp_path / "m.gguf", rope__dimension_count=20)))
     assert got.shape == (10,)
     _same(got, _plain(20))
+
+
+def test_llama3_frequencies_are_stretched_once(tmp_path):
+    """A Hugging Face configuration with llama3 scaling beside a GGUF file that carries the same
+    stretch as divisors."""
+    f = _plain()
+    turns = 512 * f / (2 * np.pi)
+    keep = np.clip((turns - 1) / (4 - 1), 0, 1)
+    want = keep * f + (1 - keep) * f / 8
+    divisors = (f / want).astype(np.float32)
+    assert divisors.max() == 8 and divisors.min() == 1
+    path = write_gguf(tmp_path / "m.gguf", more={"rope_freqs.weight": divisors})
+    scaling = {"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 1.0, "high_freq_factor": 4.0,
+               "original_max_position_embeddings": 512}
+    cfg = {"hidden_size": HID, "num_attention_heads": HEADS, "head_dim": D, "rope_theta": 500000.0}
+    _same(_turns(_model(path))[0], want)
+    for key in ("rope_type", "type"):
+        other = {(key if k == "rope_type" else k): v for k, v in scaling.items()}
+        _same(_turns(_model(path, {**cfg, "rope_scaling": other}))[0], want)
+    _same(_turns(_model(write_gguf(tmp_path / "n.gguf"), {**cfg, "rope_scaling": scaling}))[0], want)
+    # another stretch beside divisors is one more: both hold
+    linear = {"rope_type": "linear", "factor": 2.0}
+    _same(_turns(_model(path, {**cfg, "rope_scaling": linear}))[0], want / 2)

@@ -155,8 +155,10 @@ class LlamaB200Model(BaseB200Model):
         plan = self.__dict__.get("_rope")
         if plan is None:
             theta, scaling = float(self._cfg("rope_theta", 10000.0)), self._cfg("rope_scaling")
-            steps, factor = ops.rope_steps(self._rot_dim(), theta, scaling, self.weights.get("rope_freqs.weight"),
-                                           self.device)
+            freqs = self.weights.get("rope_freqs.weight")
+            if freqs is not None and scaling and scaling.get("rope_type", scaling.get("type")) == "llama3":
+                scaling = None  # the divisors are that very stretch, as a GGUF file has it
+            steps, factor = ops.rope_steps(self._rot_dim(), theta, scaling, freqs, self.device)
             # GGUF files of the llama architecture store q and k for pairs (2i, 2i + 1),
             # everything else for pairs (i, i + half)
             inter = self._cfg("rope_interleaved", self._cfg("_gguf_arch_prefix") == "llama")
