@@ -206,3 +206,25 @@ def test_llama3_frequencies_are_stretched_once(tmp_path):
     # another stretch beside divisors is one more: both hold
     linear = {"rope_type": "linear", "factor": 2.0}
     _same(_turns(_model(path, {**cfg, "rope_scaling": linear}))[0], want / 2)
+
+
+def test_the_order_of_pairs_is_the_weights(tmp_path):
+    """GGUF files of the llama architecture hold q and k for pairs (2i, 2i + 1), whatever
+    configuration stands beside them; other files for pairs (i, i + half)."""
+    from vllm_webgpu_b200.models.llama import LlamaB200Model
+    from vllm_webgpu_b200.quant.gguf_loader import FileWeights, gguf_read_config
+    llama, qwen = write_gguf(tmp_path / "l.gguf"), write_gguf(tmp_path / "q.gguf", "qwen3")
+    hf = {"hidden_size": HID, "num_attention_heads": HEADS, "head_dim": D, "rope_theta": 500000.0}
+
+    def order(path, cfg):
+        return _model(path, cfg)._rope_plan()[2]
+    assert order(llama, None) is True and order(qwen, None) is False
+    assert order(llama, hf) is True and order(qwen, hf) is False
+    assert order(qwen, gguf_read_config(llama)) is False
+    assert order(llama, {**hf, "rope_interleaved": False}) is False  # said outright
+    model = LlamaB200Model(gguf_read_config(llama), device="cpu")
+    model.weights = FileWeights()  # of safetensors
+    assert model._rope_plan()[2] is False
+    model = LlamaB200Model(gguf_read_config(llama), device="cpu")
+    model.weights = {}             # put together by hand: the configuration's file
+    assert model._rope_plan()[2] is True

@@ -159,9 +159,11 @@ class LlamaB200Model(BaseB200Model):
             if freqs is not None and scaling and scaling.get("rope_type", scaling.get("type")) == "llama3":
                 scaling = None  # the divisors are that very stretch, as a GGUF file has it
             steps, factor = ops.rope_steps(self._rot_dim(), theta, scaling, freqs, self.device)
-            # GGUF files of the llama architecture store q and k for pairs (2i, 2i + 1),
-            # everything else for pairs (i, i + half)
-            inter = self._cfg("rope_interleaved", self._cfg("_gguf_arch_prefix") == "llama")
+            # GGUF files of the llama architecture store q and k for pairs (2i, 2i + 1), everything
+            # else for pairs (i, i + half): a matter of the weights, and of the configuration only
+            # where the weights do not say what file they are of
+            arch = getattr(self.weights, "architecture", self._cfg("_gguf_arch_prefix"))
+            inter = self._cfg("rope_interleaved", arch == "llama")
             plan = self._rope = (steps, factor, bool(inter))
         return plan
 

@@ -49,11 +49,13 @@ def _device(device) -> torch.device:
 
 
 class FileWeights(dict):
-    """Weights by name, as a file holds them, and what their names do not say: ``skipped``, the
+    """Weights by name, as a file holds them, and what their names do not say: ``architecture``, a
+    GGUF file's (None for safetensors), which decides how its rows are ordered, and ``skipped``, the
     file's tensors that the loader left out."""
 
-    def __init__(self) -> None:
+    def __init__(self, architecture: str | None = None) -> None:
         super().__init__()
+        self.architecture = architecture
         self.skipped: list[str] = []
 
 
@@ -154,6 +156,11 @@ def _gguf_to_hf_name(gguf_name: str) -> str | None:
     return None
 
 
+def _gguf_architecture(reader) -> str:
+    field = reader.fields.get("general.architecture")
+    return "" if field is None else bytes(field.parts[-1]).decode("utf-8", errors="replace")
+
+
 def load_gguf_weights(path: str, device=None) -> dict:
     """Load a GGUF file with HF-style names (reference gguf_loader.py:137-162).
 
@@ -168,7 +175,7 @@ def load_gguf_weights(path: str, device=None) -> dict:
         raise ImportError("Install the 'gguf' package to load GGUF files.") from e
     dev = _device(device)
     reader = gguf.GGUFReader(path)
-    weights = FileWeights()
+    weights = FileWeights(_gguf_architecture(reader))
     for tensor in reader.tensors:
         hf_name = _gguf_to_hf_name(tensor.name)
         if hf_name is None:
