@@ -228,3 +228,47 @@ def test_the_order_of_pairs_is_the_weights(tmp_path):
     model = LlamaB200Model(gguf_read_config(llama), device="cpu")
     model.weights = {}             # put together by hand: the configuration's file
     assert model._rope_plan()[2] is True
+
+
+@pytest.mark.parametrize("cfg,want", [
+    ({}, [0, 0, 0]),
+    ({"sliding_window": None}, [0, 0, 0]),
+    ({"sliding_window": 48}, [48, 48, 48]),                                                   # Mistral
+    ({"sliding_window": 48, "use_sliding_window": False, "max_window_layers": 1}, [0, 0, 0]),  # Qwen2, off
+    ({"sliding_window": 48, "use_sliding_window": True, "max_window_layers": 1}, [0, 48, 48]),
+    ({"sliding_window": 48, "layer_types": ["full_attention", "sliding_attention", "full_attention"]}, [0, 48, 0]),
+])
+@pytest.mark.parametrize("counts", [[1, 1], [5, 1]], ids=["single", "mixed"])
+def test_the_window_reaches_attention(tmp_path, monkeypatch, cfg, want, counts):
+    """A layer's call of attention is given the configuration's window (the kernels stand aside)."""
+    from vllm_webgpu_b200 import ops
+    from vllm_webgpu_b200.kv_cache import PagedKVCache
+    model = _model(write_gguf(tmp_path / "m.gguf"),
+                   {"hidden_size": HID, "num_attention_heads": HEADS, "num_key_value_heads": KV, "head_dim": D, **cfg})
+    model._w = lambda layer, proj: torch.zeros(INTER if proj in ("gate", "up") else HID, HID)
+    seen = []
+
+    def attention(q, *rest, window=0, **kw):
+        seen.append(window)
+        return q
+    monkeypatch.setattr(ops, "paged_attention", attention)
+    monkeypatch.setattr(ops, "paged_prompt_attention", attention)
+    monkeypatch.setattr(ops, "rope_append", lambda q, *rest, **kw: q.contiguous())
+    monkeypatch.setattr(ops, "rms_norm", lambda x, w, eps, residual=None, out_dtype=None: (x, residual) if residual is not None else x)
+    for name in ("project_qkv", "project_ffn_act"):
+        monkeypatch.setattr(type(model), name, lambda self, *a: None)
+    for name in ("project_o", "project_down"):
+        monkeypatch.setattr(type(model), name, lambda self, layer, x, out: out)
+    cache = PagedKVCache(3, 4, KV, D, 16, torch.float16, "cpu")
+    step = cache.extend(["a", "b"], counts)
+    model.weights = {**model.weights, **{f"model.layers.2.{n}_layernorm.weight": torch.ones(HID)
+                                         for n in ("input", "post_attention")}}
+    for layer in range(3):
+        model.transformer_layer(layer, torch.zeros(sum(counts), HID), None, step)
+    assert seen == want
+
+
+def test_the_file_gives_the_window(tmp_path):
+    model = _model(write_gguf(tmp_path / "m.gguf", attention__sliding_window=48))
+    assert [model._window(layer) for layer in range(2)] == [48, 48]
+    assert _model(write_gguf(tmp_path / "n.gguf"))._window(0) == 0

@@ -171,6 +171,18 @@ class LlamaB200Model(BaseB200Model):
         given = self._cfg("rotary_dim")
         return int(given) if given is not None else int(self._head_dim() * float(self._cfg("partial_rotary_factor", 1.0)))
 
+    def _window(self, layer: int) -> int:
+        """How many positions a token of this layer sees (0: all): ``sliding_window``, in the layers
+        that ``layer_types`` or ``max_window_layers`` leave it to, unless ``use_sliding_window``
+        turns it off."""
+        window = self._cfg("sliding_window")
+        if not window or not self._cfg("use_sliding_window", True):
+            return 0
+        types = self._cfg("layer_types")
+        if types is not None:
+            return int(window) if types[layer] == "sliding_attention" else 0
+        return int(window) if layer >= int(self._cfg("max_window_layers", 0)) else 0
+
     def _head_dim(self) -> int:
         return int(self._cfg("head_dim") or self._cfg("hidden_size") // self._cfg("num_attention_heads"))
 
@@ -227,11 +239,12 @@ class LlamaB200Model(BaseB200Model):
         steps, factor, interleaved = self._rope_plan()
         q = ops.rope_append(q, k, v, step.positions, steps, step.slots, cache.k[layer], cache.v[layer],
                             interleaved=interleaved, factor=factor)
+        window = self._window(layer)
         if step.decode:
-            attn = ops.paged_attention(q, cache.k[layer], cache.v[layer], step.block_tables, step.lens)
+            attn = ops.paged_attention(q, cache.k[layer], cache.v[layer], step.block_tables, step.lens, window=window)
         else:
             attn = ops.paged_prompt_attention(q, step.q_starts, step.max_q, cache.k[layer], cache.v[layer],
-                                              step.block_tables, step.lens)
+                                              step.block_tables, step.lens, window=window)
         # the projections' 32-bit sums meet the stream in the norms, rounded once
         o = self.project_o(layer, attn.view(t, heads * d), torch.empty(t, hidden.shape[1], device=dev))
         normed, hidden = norm(o, "post_attention_layernorm.weight", hidden)

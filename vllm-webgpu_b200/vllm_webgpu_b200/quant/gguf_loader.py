@@ -267,6 +267,7 @@ def gguf_read_config(path: str) -> dict:
         "_gguf_arch_prefix": p,
         "rms_norm_eps": _get(f"{p}.attention.layer_norm_rms_epsilon"),
         "rotary_dim": _get(f"{p}.rope.dimension_count"),
+        "sliding_window": _get(f"{p}.attention.sliding_window"),
     }
     cfg["rope_scaling"] = _gguf_rope_scaling(_of(_get), _of(_get_str), cfg["max_position_embeddings"])
     if cfg["head_dim"] is None:
