@@ -272,3 +272,32 @@ def test_the_file_gives_the_window(tmp_path):
     model = _model(write_gguf(tmp_path / "m.gguf", attention__sliding_window=48))
     assert [model._window(layer) for layer in range(2)] == [48, 48]
     assert _model(write_gguf(tmp_path / "n.gguf"))._window(0) == 0
+
+
+def test_rotary_settings_of_newer_configurations(tmp_path):
+    """Configurations that hold theta, the stretch and the rotary part together, as a dict or as
+    the installed transformers' objects."""
+    from types import SimpleNamespace
+    path = write_gguf(tmp_path / "m.gguf")
+    base = {"hidden_size": HID, "num_attention_heads": HEADS, "head_dim": D}
+
+    def turns(**params):
+        cfg = {**base, "rope_parameters": params}
+        got = _turns(_model(path, cfg))[0]
+        assert np.array_equal(got, _turns(_model(path, SimpleNamespace(**cfg)))[0])
+        return got
+    _same(turns(rope_type="default", rope_theta=500000.0), _plain())
+    _same(turns(rope_type="linear", factor=4.0, rope_theta=500000.0), _plain() / 4)
+    _same(turns(rope_type="default", rope_theta=500000.0, partial_rotary_factor=0.5), _plain(D // 2))
+    transformers = pytest.importorskip("transformers")
+    cfg = transformers.LlamaConfig(hidden_size=HID, num_attention_heads=HEADS, num_key_value_heads=KV, head_dim=D,
+                                   rope_parameters={"rope_type": "linear", "factor": 4.0, "rope_theta": 500000.0})
+    _same(_turns(_model(path, cfg))[0], _plain() / 4)
+    cfg = transformers.MistralConfig(hidden_size=HID, num_attention_heads=HEADS, head_dim=D, sliding_window=48)
+    model = _model(path, cfg)
+    assert model._window(0) == 48
+    _same(_turns(model)[0], _plain(theta=10000.0))
+    cfg = transformers.Qwen2Config(hidden_size=HID, num_attention_heads=HEADS, num_hidden_layers=3, sliding_window=48,
+                                   use_sliding_window=True, max_window_layers=2)
+    assert [_model(path, cfg)._window(layer) for layer in range(3)] == [0, 0, 48]
+    assert _model(path, transformers.Qwen2Config(sliding_window=48))._window(0) == 0

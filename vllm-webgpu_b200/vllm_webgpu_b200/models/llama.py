@@ -150,11 +150,16 @@ class LlamaB200Model(BaseB200Model):
         value = cfg.get(name) if isinstance(cfg, dict) else getattr(cfg, name, None)
         return default if value is None else value
 
+    def _rope_cfg(self, name: str, default=None):
+        """A rotary setting: of its own or, as Hugging Face's newer configurations have it, one of
+        ``rope_parameters``."""
+        return self._cfg(name, (self._cfg("rope_parameters") or {}).get(name, default))
+
     def _rope_plan(self):
         """(steps, factor, interleaved) of the model's rotary positions, made once."""
         plan = self.__dict__.get("_rope")
         if plan is None:
-            theta, scaling = float(self._cfg("rope_theta", 10000.0)), self._cfg("rope_scaling")
+            theta, scaling = float(self._rope_cfg("rope_theta", 10000.0)), self._cfg("rope_scaling", self._cfg("rope_parameters"))
             freqs = self.weights.get("rope_freqs.weight")
             if freqs is not None and scaling and scaling.get("rope_type", scaling.get("type")) == "llama3":
                 scaling = None  # the divisors are that very stretch, as a GGUF file has it
@@ -169,7 +174,7 @@ class LlamaB200Model(BaseB200Model):
 
     def _rot_dim(self) -> int:
         given = self._cfg("rotary_dim")
-        return int(given) if given is not None else int(self._head_dim() * float(self._cfg("partial_rotary_factor", 1.0)))
+        return int(given) if given is not None else int(self._head_dim() * float(self._rope_cfg("partial_rotary_factor", 1.0)))
 
     def _window(self, layer: int) -> int:
         """How many positions a token of this layer sees (0: all): ``sliding_window``, in the layers
