@@ -301,3 +301,28 @@ def test_rotary_settings_of_newer_configurations(tmp_path):
                                    use_sliding_window=True, max_window_layers=2)
     assert [_model(path, cfg)._window(layer) for layer in range(3)] == [0, 0, 48]
     assert _model(path, transformers.Qwen2Config(sliding_window=48))._window(0) == 0
+
+
+@pytest.mark.parametrize("arch", ["granite", "phi3", "gemma2", "olmo2"])
+def test_files_of_other_architectures_are_refused(tmp_path, arch):
+    path = write_gguf(tmp_path / "m.gguf", arch)
+    hf = {"hidden_size": HID, "num_attention_heads": HEADS, "head_dim": D, "num_hidden_layers": 2}
+    for cfg in (None, hf):
+        with pytest.raises(NotImplementedError, match=arch):
+            _forward(_model(path, cfg))
+
+
+@pytest.mark.parametrize("setting", [{"final_logit_softcapping": 30.0}, {"attn_logit_softcapping": 50.0},
+                                     {"hidden_act": "gelu_pytorch_tanh"},
+                                     {"layer_types": ["full_attention", "chunked_attention"]},
+                                     {"rope_parameters": {"full_attention": {"rope_theta": 1e6},
+                                                          "sliding_attention": {"rope_theta": 1e4}}}])
+def test_settings_that_forward_leaves_out_are_refused(tmp_path, setting):
+    hf = {"hidden_size": HID, "num_attention_heads": HEADS, "num_key_value_heads": KV, "head_dim": D,
+          "num_hidden_layers": 2, "hidden_act": "silu"}
+    model = _model(write_gguf(tmp_path / "m.gguf"), hf)
+    with pytest.raises(ValueError, match="CUDA"):
+        _forward(model)
+    model.model_config = {**hf, **setting}  # looked over again
+    with pytest.raises(NotImplementedError):
+        _forward(model)

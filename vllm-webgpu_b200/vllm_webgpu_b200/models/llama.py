@@ -34,6 +34,7 @@ PROJ = {
 LAYER_WEIGHTS = {*PROJ.values(), "input_layernorm.weight", "post_attention_layernorm.weight", "self_attn.q_norm.weight",
                  "self_attn.k_norm.weight"}
 OTHER_WEIGHTS = {"model.embed_tokens.weight", "model.norm.weight", "lm_head.weight", "rope_freqs.weight"}
+FORWARD_ARCHITECTURES = ("llama", "qwen2", "qwen3")  # of GGUF files; others differ from these in more than names
 
 
 def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -192,11 +193,11 @@ class LlamaB200Model(BaseB200Model):
         return int(self._cfg("head_dim") or self._cfg("hidden_size") // self._cfg("num_attention_heads"))
 
     def _check_model(self) -> None:
-        """Refuse weights that ``forward`` would leave out: a bias, a norm that the Llama layer has
-        not, a tensor that the loader has no name for. Looked over again when weights change."""
-        weights = self.weights
-        seen = self.__dict__.get("_checked")
-        if seen is not None and seen[0] is weights and seen[1] == len(weights):
+        """Refuse what ``forward`` would leave out: a tensor (a bias, a norm that the Llama layer
+        has not, one that the loader has no name for) or a setting. Looked over again when weights
+        or configuration change."""
+        weights, seen = self.weights, self.__dict__.get("_checked", (None, None, 0))
+        if seen[0] is weights and seen[1] is self.model_config and seen[2] == len(weights):
             return
         other = list(getattr(weights, "skipped", ()))
         for name in weights:
@@ -211,7 +212,21 @@ class LlamaB200Model(BaseB200Model):
             raise NotImplementedError("forward does not apply these of the model's tensors (a bias, a norm or a part that "
                                       f"the Llama layer has not): {', '.join(sorted(other)[:4])}"
                                       + (f" and {len(other) - 4} more" if len(other) > 4 else ""))
-        self._checked = (weights, len(weights))
+        for arch in (getattr(weights, "architecture", None), self._cfg("_gguf_arch_prefix")):
+            if arch is not None and arch not in FORWARD_ARCHITECTURES:
+                raise NotImplementedError(f"forward does not know GGUF files of the architecture {arch!r} "
+                                          f"(it does {', '.join(FORWARD_ARCHITECTURES)})")
+        for name in ("final_logit_softcapping", "attn_logit_softcapping"):
+            if self._cfg(name):
+                raise NotImplementedError(f"forward does not apply {name}")
+        if self._cfg("hidden_act", "silu") not in ("silu", "swish"):
+            raise NotImplementedError(f"forward applies SiLU in the FFN, not {self._cfg('hidden_act')}")
+        types = set(self._cfg("layer_types", ())) - {"full_attention", "sliding_attention"}
+        if types:
+            raise NotImplementedError(f"forward has full and sliding attention, not {', '.join(sorted(types))}")
+        if any(isinstance(v, dict) for v in (self._cfg("rope_parameters") or {}).values()):
+            raise NotImplementedError("forward turns all layers by the same rotary settings")
+        self._checked = (weights, self.model_config, len(weights))
 
     def transformer_layer(self, layer: int, hidden: torch.Tensor, delta, step) -> tuple[torch.Tensor, torch.Tensor]:
         """One layer over the tokens of ``step`` (``PagedKVCache.extend``). The residual
