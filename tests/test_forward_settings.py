@@ -326,3 +326,18 @@ def test_settings_that_forward_leaves_out_are_refused(tmp_path, setting):
     model.model_config = {**hf, **setting}  # looked over again
     with pytest.raises(NotImplementedError):
         _forward(model)
+
+
+def test_other_weights_bring_their_own_rotary_plan(tmp_path):
+    model = _model(write_gguf(tmp_path / "a.gguf"))
+    first = model._rope_plan()
+    assert model._rope_plan() is first
+    divisors = np.full(D // 2, 2.0, np.float32)
+    model.load_weights(write_gguf(tmp_path / "b.gguf", more={"rope_freqs.weight": divisors}))
+    _same(_turns(model)[0], _plain() / 2)
+    model.weights["rope_freqs.weight"] = torch.full((D // 2,), 4.0)
+    _same(_turns(model)[0], _plain() / 4)
+    model.model_config = {**model.model_config, "rope_theta": 10000.0}
+    _same(_turns(model)[0], _plain(theta=10000.0) / 4)
+    model.load_weights(write_gguf(tmp_path / "c.gguf", "qwen3"))
+    assert model._rope_plan()[2] is False

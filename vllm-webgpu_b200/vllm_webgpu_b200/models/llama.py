@@ -157,11 +157,13 @@ class LlamaB200Model(BaseB200Model):
         return self._cfg(name, (self._cfg("rope_parameters") or {}).get(name, default))
 
     def _rope_plan(self):
-        """(steps, factor, interleaved) of the model's rotary positions, made once."""
-        plan = self.__dict__.get("_rope")
-        if plan is None:
+        """(steps, factor, interleaved) of the model's rotary positions, made once for the weights
+        and the configuration that are there."""
+        made_of = (self.weights, self.weights.get("rope_freqs.weight"), self.model_config)
+        plan, of = self.__dict__.get("_rope", (None, ()))
+        if plan is None or any(a is not b for a, b in zip(of, made_of)):
             theta, scaling = float(self._rope_cfg("rope_theta", 10000.0)), self._cfg("rope_scaling", self._cfg("rope_parameters"))
-            freqs = self.weights.get("rope_freqs.weight")
+            freqs = made_of[1]
             if freqs is not None and scaling and scaling.get("rope_type", scaling.get("type")) == "llama3":
                 scaling = None  # the divisors are that very stretch, as a GGUF file has it
             steps, factor = ops.rope_steps(self._rot_dim(), theta, scaling, freqs, self.device)
@@ -170,7 +172,8 @@ class LlamaB200Model(BaseB200Model):
             # where the weights do not say what file they are of
             arch = getattr(self.weights, "architecture", self._cfg("_gguf_arch_prefix"))
             inter = self._cfg("rope_interleaved", arch == "llama")
-            plan = self._rope = (steps, factor, bool(inter))
+            plan = (steps, factor, bool(inter))
+            self._rope = (plan, made_of)
         return plan
 
     def _rot_dim(self) -> int:
