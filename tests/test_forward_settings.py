@@ -341,3 +341,14 @@ def test_other_weights_bring_their_own_rotary_plan(tmp_path):
     _same(_turns(model)[0], _plain(theta=10000.0) / 4)
     model.load_weights(write_gguf(tmp_path / "c.gguf", "qwen3"))
     assert model._rope_plan()[2] is False
+
+
+@pytest.mark.parametrize("more", [{"mscale": 0.7}, {"mscale_all_dim": 1.0}, {"truncate": False}])
+def test_yarn_options_that_rope_steps_leaves_out_are_refused(more):
+    from vllm_webgpu_b200 import ops
+    yarn = {"rope_type": "yarn", "factor": 8.0, "original_max_position_embeddings": 2048}
+    want, factor = ops.rope_steps(D, 10000.0, yarn, device="cpu")
+    same, _ = ops.rope_steps(D, 10000.0, {**yarn, "truncate": True, "mscale": None}, device="cpu")
+    assert torch.equal(want, same) and factor > 1
+    with pytest.raises(ValueError, match=next(iter(more))):
+        ops.rope_steps(D, 10000.0, {**yarn, **more}, device="cpu")

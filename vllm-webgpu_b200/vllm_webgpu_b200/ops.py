@@ -752,6 +752,9 @@ def rope_steps(rot_dim: int, theta: float = 10000.0, scaling: dict | None = None
         keep = np.clip((turns - low) / (high - low), 0.0, 1.0)
         f = keep * f + (1.0 - keep) * f / float(scaling["factor"])
     elif kind == "yarn":
+        for name, plain in (("mscale", None), ("mscale_all_dim", None), ("truncate", True)):
+            if scaling.get(name, plain) not in (None, plain):
+                raise ValueError(f"yarn scaling with {name} = {scaling[name]} is not supported")
         old, by = float(scaling["original_max_position_embeddings"]), float(scaling["factor"])
 
         def pair_with(turns):  # the pair that makes so many turns over the original context
