@@ -969,8 +969,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     index, args, out, sizes, keep = _attention_args(q, k_cache, v_cache, block_tables, lens, scale, window, out, None, 0)
     if workspace is None:
         workspace = _attention_workspace(*sizes, index)
-    elif workspace.get_device() != index:
-        raise ValueError(f"workspace must lie on cuda:{index}")
+    elif workspace.get_device() != index or workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be a contiguous uint8 tensor on cuda:{index} (attention_workspace makes it)")
     _call(index, "ggufmm_paged_attention", args, workspace.data_ptr(), workspace.numel())
     return out
 
