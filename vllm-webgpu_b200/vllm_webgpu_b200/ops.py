@@ -651,7 +651,7 @@ def _norm_rows(t: torch.Tensor, shape, index: int, n: int, m: int, what: str | N
         raise ValueError(f"{what or 'residual'} must be a {tuple(shape)} tensor on cuda:{index}")
     if t.is_contiguous():
         return t, n
-    if t.dim() == 2 and t.stride(1) == 1:
+    if t.dim() == 2 and t.stride(1) == 1 and (m <= 1 or t.stride(0) >= n):
         return t, t.stride(0) if m > 1 else n
     if what is not None:
         raise ValueError(f"{what} must be contiguous, or two-dimensional with contiguous rows")
@@ -921,6 +921,9 @@ def _attention_args(q, k_cache, v_cache, tables, lens, scale, window, out, q_sta
         _require_cuda(q)
     q, shape, qs = _heads(q, "q", index)
     t, hq, d = shape
+    if (t > 1 and qs[0] < d) or (hq > 1 and qs[1] < d):  # rows that lie over one another
+        q = q.contiguous()
+        qs = q.stride()
     (pages, hkv, page, dk), cache_dtype, ks, vs = _cache_strides(k_cache, v_cache, index)
     dtype = q.dtype
     if dk != d or cache_dtype is not dtype:
@@ -937,7 +940,7 @@ def _attention_args(q, k_cache, v_cache, tables, lens, scale, window, out, q_sta
     if tables.dim() != 2 or tables.get_device() != index:
         raise ValueError(f"block_tables must be a [batch, pages] tensor on cuda:{index}")
     b, width = tables.shape
-    if tables.dtype is not torch.int32 or (width > 1 and tables.stride(1) != 1):
+    if tables.dtype is not torch.int32 or (width > 1 and tables.stride(1) != 1) or (b > 1 and tables.stride(0) < width):
         tables = tables.to(torch.int32).contiguous()
     lens = _index(lens, torch.int32, b, "lens", index)
     starts = 0
