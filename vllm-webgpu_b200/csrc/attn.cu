@@ -29,7 +29,7 @@ int check_attention(const ggufmm_attention_args& p, bool prompt) {
   if (s) return s;
   if (p.batch < 0 || p.batch > 65535 || p.total_q < 0 || p.total_q > kI32Max || p.q_heads < 1 || p.q_heads > 65535 ||
       p.q_heads % p.kv_heads || p.q_heads / p.kv_heads > GGUFMM_MAX_GROUP || p.table_width < 0 ||
-      p.table_row < p.table_width || p.table_width * p.page_size > kI32Max / 2 || p.window < 0 || p.window > kI32Max)
+      p.table_width > kI32Max || p.table_row < p.table_width || p.table_width * p.page_size > kI32Max / 2 || p.window < 0 || p.window > kI32Max)
     return GGUFMM_ERR_SHAPE;
   if (prompt ? (p.max_q < 0 || p.max_q > p.total_q) : p.total_q != p.batch) return GGUFMM_ERR_SHAPE;
   if (!std::isfinite(p.scale)) return GGUFMM_ERR_ARG;
