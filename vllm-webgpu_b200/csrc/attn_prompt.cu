@@ -35,8 +35,10 @@
 // Units are those of the sequences' own lengths, found on the device: 2048 new tokens beside 63
 // single ones take 112 us, 235 with units for the longest in every sequence.
 //
-// 8192 tokens of 32 / 8 heads of 128: 416 us, 1321 TFLOP/s, 79% of the measured bf16 burst (called
-// for a second on end, under the power limit, 485 us, 79% of the sustained rate). Per 256 x 128
+// 8192 tokens of 32 / 8 heads of 128: called on end, under the power limit, 491 us, 1120 TFLOP/s, 79%
+// of the sustained bf16 rate; in short bursts 421 us, 1307 TFLOP/s, 79% of the burst rate. 4096 tokens,
+// heads of 64, 80, 96, 128, 192, 256: 104, 112, 112, 118, 268, 252 us, of floors of 41, 52, 62, 83, 124,
+// 165 (widths are padded to 64, 128 or 256). Per 256 x 128
 // scores the tensor core and the exponentials are each busy for about 2050 of 3100 clocks; what
 // is left is each tile's chain of load, maximum, exponentials and hand-over (2500). A
 // quarter of the exponentials as polynomials on the FMA units took 3% longer.
@@ -288,8 +290,9 @@ __device__ __forceinline__ void weights(const float* s, float s2, float z, uint3
     a = exp2_fast(a);
     b = exp2_fast(b);
     sum[c & 1] = add2(sum[c & 1], pair(a, b));
-    // rounded to the cache's type for the product, the sum is not: a relative 2^-9
-    // (2^-12) of each weight, below the rounding of the output
+    // rounded to the cache's type for the product, whose two operands have one type; the sum is
+    // not. That adds as much as the output's own rounding: relative error against 64 bits 0.0019 to
+    // 0.0022 in bf16 where 32-bit weights give 0.0016
     p[c] = pack16<DT>(a, b);
   }
 }

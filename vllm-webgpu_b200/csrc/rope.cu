@@ -98,6 +98,8 @@ __device__ __forceinline__ void store_vals(void* p, int dt, int64_t i, const flo
 // HBM bound: 8192 tokens of 32 / 8 heads of 128 (201 MB) in 35 us, 5.7 TB/s, 89% of the measured
 // copy rate, with two tokens and 128 threads a CTA; 256 threads 45 us (their waits coincide), four
 // tokens 36 us, sines before loads 47 us. A few tokens take 3 us, a launch and two memory latencies.
+// Rotary widths that are no multiple of 8 go value by value: 8192 tokens, heads of 80 with 20 turning
+// (126 MB) 68 us, 1.9 TB/s; all 80 turning 28 us, 4.5 TB/s.
 template <int XT, int N, int TB, int NT>
 __global__ void __launch_bounds__(NT) rope_append_kernel(const __grid_constant__ RopeArgs a) {
   extern __shared__ float2 table[];  // [TB][half]
